@@ -39,7 +39,9 @@ extern "C" {
  * 5 (round 5): + v2s_sum_n, v2s_argmax_step_tail, options gemm_a4 / gemm_a4_grid / gemm_a4_relu / gemm_a4_walk (additions only)
  * 6 (round 6): + v2s_clock_probe, v2s_lmhead_ce_fwd / _bwd / _workspace_floats; the round-4 experiment options gemm_ps / gemm_ps_nst / gemm_w128 are gone
  *   (v2s_set_option returns V2S_ERR_ARG for them) */
-#define V2S_ABI_VERSION 6
+/* 7: + v2s_quant_rows_q8, v2s_rmsnorm_q8, v2s_dequant_q8, v2s_gemm_q8, v2s_kv_append_q8 / v2s_kv_read_q8, v2s_decode_attn_q8 (+ its workspace size),
+ *   v2s_sample_step (additions only) */
+#define V2S_ABI_VERSION 7
 
 int v2s_version(void);
 const char* v2s_last_error(void);
@@ -477,6 +479,94 @@ int v2s_topp_sample_step(const float* logits, int64_t ld, int32_t rows, int32_t 
 int v2s_beam_sample_cand(const float* logits, int64_t ld, int32_t rows, int32_t V, int32_t K, const float* beam_scores, float top_p,
                          float temperature, int32_t top_k, uint32_t seed, float* out_val, int32_t* out_tok, float* out_key,
                          int32_t ban_token, const int32_t* pos_dev, int32_t min_length, const float* row_lse, void* stream);
+/* One sampling step from GIVEN random numbers: temperature, top-k, top-p and min-p, in the order of HF 4.28's warpers, on fp32 or bf16 logits
+ * [rows][ld] (logits_dtype V2S_F32 / V2S_BF16), V <= 131072.  For each row, with the tokens ordered by logit (equal logits: the lower index first):
+ *   w_i = exp((z_i - max z) / temperature), an entry equal to the maximum has w = 1 (so a row of -infinity is uniform; +infinity wins over all);
+ *   top-k keeps the first top_k tokens (0 = all); top-p keeps of those the tokens whose preceding mass is < top_p * their whole mass; min-p keeps
+ *   of those the tokens with w_i >= min_p.  The drawn token is the first one, in index order, at which the running kept mass exceeds u * kept mass.
+ * The weights are 64-bit fixed-point numbers (2^46 = weight one; below 2^-47 a token has none), so masses do not depend on the order of their sums
+ * and every decision is the one exact arithmetic makes, up to 2^-46 of the largest weight.  A row that holds a NaN yields the index of its first
+ * NaN (as v2s_argmax_step does) and a NaN log-probability.
+ *   u: fp32 in [0, 1) (below 0 and NaN count as 0, from 1 on the last kept token is drawn): u[row], or with pos_dev row *pos_dev of a table [u_steps][u_ld]
+ *   (a step behind the table reads its last row), so that one table serves a captured loop.
+ *   logp (may be NULL): log of the drawn token's probability among the kept tokens.  next_tok, unfinished, eos_id, pad_id, seq_out, seq_ld,
+ *   pos_dev, min_length as in v2s_topp_sample_step; unfinished may be NULL (every row draws); a finished row gets pad_id and logp 0; column
+ *   *pos_dev + 1 of seq_out is written if it is below seq_ld. */
+int v2s_sample_step(const void* logits, int32_t logits_dtype, int64_t ld, int32_t rows, int32_t V, double temperature, int32_t top_k, double top_p,
+                    double min_p, const float* u, int64_t u_ld, int32_t u_steps, int64_t* next_tok, float* logp, int32_t* unfinished, int32_t eos_id,
+                    int32_t pad_id, int64_t* seq_out, int64_t seq_ld, const int32_t* pos_dev, int32_t min_length, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * 8-bit decoding: int8 codes with fp32 scales (the values they stand for are scale * code)
+ *   a row y gets  scale = max(amax|y|, 127 * 2^-126) / 127,  code = round_to_even(y / scale);  a row that holds a NaN or an infinity gets scale NaN and
+ *   zero codes, so that every value of it is read back as NaN.
+ * ---------------------------------------------------------------------------------------------- */
+/* codes q[rows][ldq] and scale[rows] of the rows of x (bf16 or fp32 [rows][ldx]): weights once (a scale per output channel), activations per token.
+ * cols a multiple of 8, <= 8192; x 16-byte, q 8-byte aligned, strides multiples of 8. */
+int v2s_quant_rows_q8(const void* x, int32_t x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int32_t rows, int32_t cols, void* stream);
+/* T5LayerNorm (modeling_t5.py:263-277) with the residual addition before it (modeling_t5.py:353,618,654) and the quantisation behind it, one pass:
+ *   s = bf16(x + delta) (delta NULL: s = x), stored to h unless h is NULL (h may be x or delta);  y = w * s * rsqrt(mean(s^2) + eps) in fp32;  q, scale of y. */
+int v2s_rmsnorm_q8(const void* x, int64_t ldx, const void* delta, int64_t ldd, const float* w, void* h, int64_t ldh, int8_t* q, int64_t ldq,
+                   float* scale, int32_t rows, int32_t cols, float eps, void* stream);
+/* y[rows][ldy] (bf16) = scale[row] * q[row][.] */
+int v2s_dequant_q8(const int8_t* q, int64_t ldq, const float* scale, void* y, int64_t ldy, int32_t rows, int32_t cols, void* stream);
+
+/* C[M][N] = act(alpha * sA[m] * sB[n] * sum_k A[m][k] B[n][k] + bias[n]) + residual[m][n]:  y = x W^T of an nn.Linear with A = codes of the tokens
+ * [M][lda], sA their scales, B = codes of the weight [N][ldb] ([out, in], one scale per output channel).  The sums of int8 products are exact int32
+ * (K <= 131056); the scales and the epilogue are fp32, one rounding to C.  M and N arbitrary; K, lda, ldb multiples of 16, ldc, ldr multiples of 8;
+ * A, B, C, residual 16-byte aligned.  Replaces modeling_t5.py:304-311,528-536,581,1714 where int8 operands are wanted. */
+typedef struct v2s_gemm_q8_args {
+  int32_t M, N, K;
+  const int8_t *A, *B;
+  int64_t lda, ldb;
+  const float *sA, *sB;
+  void* C;
+  int64_t ldc;
+  int32_t c_dtype;       /* V2S_BF16 or V2S_F32 */
+  float alpha;
+  const float* bias;     /* [N] or NULL */
+  int32_t act;           /* V2S_ACT_* */
+  const void* residual;  /* bf16 [M][ldr] or NULL; may be C (bf16) */
+  int64_t ldr;
+} v2s_gemm_q8_args;
+int v2s_gemm_q8(const v2s_gemm_q8_args* args, void* stream);
+
+/* int8 key / value cache: codes [.][64] and scales [.], the row of (entry, head, token) is entry * e_rows + head * h_rows + token (one scale per token
+ * and head; the tokens of a head are contiguous).  head width 64. */
+typedef struct v2s_kv_q8 {
+  int8_t* k; float* ks; int8_t* v; float* vs;
+  int64_t e_rows, h_rows;        /* in rows, >= maxlen */
+  int32_t entries, heads, maxlen;
+} v2s_kv_q8;
+/* Quantises T new tokens per entry as they enter the cache, and reads T rows back.  k, v: bf16 [entries][T] rows (strides bs, rs in elements, head h at
+ * column h * 64).  Entry e's token t goes to / comes from cache token (pos ? pos[e] : pos0) + (pos_dev ? *pos_dev : 0) + t; count (device, may be NULL)
+ * limits entry e to its first count[e] tokens.  Tokens outside [0, maxlen) are dropped, rows that take no part stay as they are. */
+int v2s_kv_append_q8(const v2s_kv_q8* cache, const void* k, const void* v, int64_t src_bs, int64_t src_rs, int32_t T, int32_t pos0, const int32_t* pos,
+                     const int32_t* pos_dev, const int32_t* count, void* stream);
+int v2s_kv_read_q8(const v2s_kv_q8* cache, void* k, void* v, int64_t dst_bs, int64_t dst_rs, int32_t T, int32_t pos0, const int32_t* pos,
+                   const int32_t* pos_dev, const int32_t* count, void* stream);
+
+/* One query row per (row, head) against the int8 cache: z_j = scale * <q, k_j> + bias_j, o = softmax(z) v over the entry's keys.
+ * The keys of an entry are the first klen[e] (device, clamped to [0, Nk]), or *pos_dev + 1, or Nk.  Masked keys (key_mask[e][j] == 0) have no part in the
+ * result whatever they hold; a row that sees no key (all masked, or bias -infinity everywhere) gets the mean of its keys' values, as the reference's
+ * finfo.min masks give (modeling_t5.py:996,559); an entry without keys gets zeros.  group query rows (beams) share an entry: B = entries * group.
+ * Pieces of 512 keys are summed by blocks of their own and joined, so a sequence's result does not depend on its batch; Nk > 512 needs
+ * v2s_decode_attn_q8_workspace_floats(B, heads, Nk) floats of workspace, which no other launch in flight may use. */
+typedef struct v2s_decode_attn_q8_args {
+  int32_t B, Nk, group;
+  const void* q; int64_t q_bs;            /* bf16 [B][heads * 64] */
+  v2s_kv_q8 cache;
+  void* o; int64_t o_bs;                  /* bf16 */
+  const float* bias_row; int64_t bias_ld; /* as in v2s_decode_attn_args */
+  const int32_t* pos_dev; int32_t bias_maxlen;
+  const int32_t* klen;
+  const uint8_t* key_mask; int64_t mask_ld;
+  float scale;
+  void* workspace; int64_t workspace_bytes;
+} v2s_decode_attn_q8_args;
+int64_t v2s_decode_attn_q8_workspace_floats(int32_t B, int32_t H, int32_t Nk);
+int v2s_decode_attn_q8(const v2s_decode_attn_q8_args* args, void* stream);
+
 /* *ctr += delta (one thread; closes a captured decode step) */
 int v2s_counter_add(int32_t* ctr, int32_t delta, void* stream);
 

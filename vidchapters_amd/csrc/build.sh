@@ -12,7 +12,7 @@ FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -munsafe-fp
 # v2s_attn hold such instructions in their own asm statements, which this flag would refuse
 NOPK="-Xclang -target-feature -Xclang -packed-fp32-ops"
 flags_of() { case $1 in v2s_gemm|v2s_attn) echo "$FLAGS";; *) echo "$FLAGS $NOPK";; esac; }
-SRCS="v2s_api v2s_gemm v2s_norm v2s_attn v2s_misc v2s_optim v2s_decode v2s_memattn v2s_data"
+SRCS="v2s_api v2s_gemm v2s_norm v2s_attn v2s_misc v2s_optim v2s_decode v2s_memattn v2s_data v2s_q8 v2s_gemm_q8 v2s_sample"
 mkdir -p build
 # the hand-scheduled K loop of gemm_a4_kernel is generated (scoreboarded s_waitcnt counts, MFMA-gap placement): see gen_gemm_a4.py
 if [ ! -f v2s_gemm_a4.inc ] || [ gen_gemm_a4.py -nt v2s_gemm_a4.inc ]; then

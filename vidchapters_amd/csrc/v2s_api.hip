@@ -85,6 +85,9 @@ extern "C" int64_t v2s_sizeof(const char* name) {
     if (strcmp(name, "v2s_attn_args") == 0) return (int64_t)sizeof(v2s_attn_args);
     if (strcmp(name, "v2s_adam_args") == 0) return (int64_t)sizeof(v2s_adam_args);
     if (strcmp(name, "v2s_decode_attn_args") == 0) return (int64_t)sizeof(v2s_decode_attn_args);
+    if (strcmp(name, "v2s_gemm_q8_args") == 0) return (int64_t)sizeof(v2s_gemm_q8_args);
+    if (strcmp(name, "v2s_kv_q8") == 0) return (int64_t)sizeof(v2s_kv_q8);
+    if (strcmp(name, "v2s_decode_attn_q8_args") == 0) return (int64_t)sizeof(v2s_decode_attn_q8_args);
   }
   v2s_set_error("v2s_sizeof: unknown struct '%s'", name ? name : "(null)");
   return -1;
