@@ -69,6 +69,8 @@ const char* v2s_last_error(void);
  *   "gemm_a4_relu"  1 (default): the persistent form also takes forward GEMMs with a ReLU or ReLU + dropout epilogue (the FFN's wi: the
  *                   dropout mask of the library's counter-based generator is recomputed inside the kernel's MFMA gaps), 0: plain epilogues only
  *   "gemm_dbg"      profiling ablations of the tiled kernels (results invalid when non-zero): 1 = no global store, 2 = no epilogue, 3 = no hand-off
+ *   "gemm_q8"       kernel of v2s_gemm_q8: 0 = by size (default), 1 = few rows, 2 / 3 / 4 = 64 x 64 / 128 x 128 / 128 x 256 tiles (results do not
+ *                   depend on it: the sums are exact)
  *   "fp32_io"       DEBUG: 1 = v2s_*norm_fwd/bwd, v2s_ce_bwd and v2s_attn_fwd/bwd take and return FP32 activations (attention: fp32-arithmetic
  *                   reference kernels, dense layout only); parity work against fp32 references (<= 1e-4), never set by the product path
  *   "attn_bwd_part" 0: v2s_attn_bwd launches dQ and dK/dV kernels (default), 1: dQ only, 2: dK/dV only (per-kernel timing)
@@ -513,7 +515,7 @@ int v2s_dequant_q8(const int8_t* q, int64_t ldq, const float* scale, void* y, in
 
 /* C[M][N] = act(alpha * sA[m] * sB[n] * sum_k A[m][k] B[n][k] + bias[n]) + residual[m][n]:  y = x W^T of an nn.Linear with A = codes of the tokens
  * [M][lda], sA their scales, B = codes of the weight [N][ldb] ([out, in], one scale per output channel).  The sums of int8 products are exact int32
- * (K <= 131056); the scales and the epilogue are fp32, one rounding to C.  M and N arbitrary; K, lda, ldb multiples of 16, ldc, ldr multiples of 8;
+ * (K <= 131056); the scales and the epilogue are fp32, one rounding to C.  M and N arbitrary; K, lda, ldb multiples of 16 (lda, ldb <= 2^24), ldc, ldr multiples of 8;
  * A, B, C, residual 16-byte aligned.  Replaces modeling_t5.py:304-311,528-536,581,1714 where int8 operands are wanted. */
 typedef struct v2s_gemm_q8_args {
   int32_t M, N, K;

@@ -144,6 +144,25 @@ def test_gemm_q8(M, N, K, out):
         assert (C[:M, N:] == 7).all() and (C[M:] == 7).all()      # nothing outside the product is written
 
 
+@pytest.mark.parametrize("kind", [1, 2, 3, 4], ids=["few_rows", "64x64", "128x128", "128x256"])
+@pytest.mark.parametrize("M,N,K", [(1, 8, 16), (70, 300, 48), (130, 257, 112), (300, 520, 64), (257, 513, 1040), (128, 512, 4096), (513, 769, 784)])
+def test_gemm_q8_every_kernel_gives_the_same_bits(M, N, K, kind):
+    A, sa = codes(M, K, 3)
+    B, sb = codes(N, K, 4)
+    ld = (N + 7) // 8 * 8
+    res = rnd(M, ld, seed=6)
+    want, mag = product_ref(A, B, sa, sb, 1.0, None, L.ACT_NONE, res[:, :N])
+    auto, C = torch.zeros(M + 1, ld, dtype=BF, device=DEV), torch.zeros(M + 1, ld, dtype=BF, device=DEV)
+    L.gemm_q8(A, B, sa, sb, auto, M, N, K, ldc=ld, residual=res, ldr=ld)
+    L.set_option("gemm_q8", kind)
+    try:
+        L.gemm_q8(A, B, sa, sb, C, M, N, K, ldc=ld, residual=res, ldr=ld)
+    finally:
+        L.set_option("gemm_q8", 0)
+    assert torch.equal(C, auto) and (C[M:] == 0).all()
+    assert ((C[:M, :N].double() - want).abs() <= mag * 7 * U32 + want.abs() * UBF).all()
+
+
 def test_gemm_q8_codes_are_summed_exactly():
     """The largest sums int8 codes can have: all -128, K at its limit; and sums that differ by one."""
     K = 131056

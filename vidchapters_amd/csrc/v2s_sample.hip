@@ -5,8 +5,10 @@
 //   min-p: w_i >= min_p;  draw: the first token in index order whose running kept mass exceeds u * kept mass
 // No sort: the boundary of top-k / top-p is found by a histogram over the distance to the maximum (counts, or masses), which names the one bin
 // that holds it, and by ranking the few tokens of that bin exactly.  Masses are 64-bit integers (2^46 = weight one): their sums are exact, so the
-// result depends neither on the order of the atomics nor on how the row is cut.  A row of 32768 logits stays in the registers of its block and is
-// read once.
+// result depends neither on the order of the atomics nor on how the row is cut.
+// A row of up to 32768 logits is read from memory once and stays in LDS as fp32 (larger ones are read again for every pass, mostly from L2).  The
+// passes over it are bound by VALU issue, not by memory: one instruction per logit costs a block 0.2 us at V = 32228, which is why the weights'
+// exponential is a short polynomial of its own and why small top-k never touches most logits (below).
 #include <math.h>
 #include "v2s_common.h"
 
@@ -14,27 +16,43 @@ namespace {
 
 typedef unsigned long long u64;
 constexpr int NT = 1024, STEP = NT * 4;     // tokens per pass of the block: four consecutive ones per thread
-constexpr int NBIN = 2048, CAP = 1024;
+constexpr int NBIN = 2048, CAP = 512;
+constexpr int ROW_MAX = 8;                  // passes whose logits fit LDS: 32768 fp32 = 128 KiB, next to 24 KiB of tables
+constexpr int SMALL_K = 128, SMALL_N = 256; // top-k by candidate list: every step costs each candidate a walk over the others
 constexpr float BIN_RANGE = 33.0f;          // exp(-33) < 2^-47: what lies further from the maximum has no mass
 constexpr double ONE = 70368744177664.0;    // 2^46: 131072 tokens of weight one sum to 2^63
 
 struct SampleP {
-  const void* logits; long ld; int V;
-  double inv_temp; float bin_scale;
+  const void* logits; long ld; int V, vec;
+  double inv_temp, exp2_scale; float bin_scale;   // 1 / T, log2(e) / T, bins per unit of logit
   int top_k; double top_p, min_p;
   const float* u; long u_ld; int u_steps;
   long* next_tok; float* logp; int* unfinished; int eos_id, pad_id;
   long* seq_out; long seq_ld; const int* pos_dev; int min_length;
 };
 
-__device__ __forceinline__ float logit_of(float v) { return v; }
-__device__ __forceinline__ float logit_of(bf16_t v) { return bf2f(v); }
 // ascending in the order of the tokens: larger logits first, then lower indexes (z is never -0 or NaN here)
 __device__ __forceinline__ u64 order_key(float z, int idx) {
   const uint32_t b = __float_as_uint(z);
   const uint32_t asc = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
   return ((u64)(~asc) << 32) | (uint32_t)idx;
 }
+__device__ __forceinline__ float key_logit(u64 key) {
+  const uint32_t asc = ~(uint32_t)(key >> 32);
+  return __uint_as_float((asc >> 31) ? asc ^ 0x80000000u : ~asc);
+}
+// 2^t for t <= 0: t = k + f, |f| <= 1/2, and the series of 2^f to the 13th power (its remainder is below 2^-57)
+__device__ __forceinline__ double exp2_neg(double t) {
+  t = fmax(t, -100.0);
+  const double k = rint(t), x = (t - k) * 0.69314718055994530942;
+  double s = 1.0 / 6227020800.0;
+  s = fma(s, x, 1.0 / 479001600.0); s = fma(s, x, 1.0 / 39916800.0); s = fma(s, x, 1.0 / 3628800.0); s = fma(s, x, 1.0 / 362880.0);
+  s = fma(s, x, 1.0 / 40320.0); s = fma(s, x, 1.0 / 5040.0); s = fma(s, x, 1.0 / 720.0); s = fma(s, x, 1.0 / 120.0); s = fma(s, x, 1.0 / 24.0);
+  s = fma(s, x, 1.0 / 6.0); s = fma(s, x, 0.5); s = fma(s, x, 1.0); s = fma(s, x, 1.0);
+  return ldexp(s, (int)k);
+}
+// round to nearest: 2^46 w < 2^52, so the sum holds it in its low bits
+__device__ __forceinline__ u64 mass_of(double w) { return (u64)__double_as_longlong(w * ONE + 4503599627370496.0) & 0xfffffffffffffull; }
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += (u64)__shfl_xor((long long)v, o, 64);
@@ -55,59 +73,91 @@ __device__ u64 block_sum64(u64 v, u64* red, int tid) {
   for (int i = 0; i < NT / 64; ++i) s += red[i];
   return s;
 }
+__device__ __forceinline__ void load4(const float* z, int i0, int V, int vec, float (&o)[4]) {
+  if (vec && i0 + 4 <= V) {
+    const float4 v = *reinterpret_cast<const float4*>(z + i0);
+    o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = i0 + i < V ? z[i0 + i] : -INFINITY;
+  }
+}
+__device__ __forceinline__ void load4(const bf16_t* z, int i0, int V, int vec, float (&o)[4]) {
+  if (vec && i0 + 4 <= V) {
+    const uint2 v = *reinterpret_cast<const uint2*>(z + i0);
+    o[0] = __uint_as_float(v.x << 16); o[1] = __uint_as_float(v.x & 0xffff0000u); o[2] = __uint_as_float(v.y << 16); o[3] = __uint_as_float(v.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = i0 + i < V ? bf2f(z[i0 + i]) : -INFINITY;
+  }
+}
 
-// NJ passes of the block hold the row in registers; NJ = 0: the row is read again for every pass (V > 32768)
-template <typename T, int NJ>
+// ROW: the row is held in LDS (zs), else every pass reads it again
+template <typename T, bool ROW>
 __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
+  extern __shared__ __attribute__((aligned(16))) float zs[];
   __shared__ u64 s_mass[NBIN];
-  __shared__ uint32_t s_cnt[NBIN];
   __shared__ u64 s_key[CAP], s_w[CAP];
   __shared__ u64 s_red[NT / 64], s_thr, s_base;
   __shared__ float s_max[NT / 64];
-  __shared__ int s_n, s_bin, s_nan, s_pick;
+  __shared__ int s_n, s_bin, s_nan;
+  uint32_t* const s_cnt = reinterpret_cast<uint32_t*>(s_mass);      // the counts of top-k, before the masses of top-p
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = blockIdx.x, V = p.V;
+  const int row = blockIdx.x, V = p.V, nj = (V + STEP - 1) / STEP;
   const T* z0 = (const T*)p.logits + (long)row * p.ld;
   const int step = p.pos_dev ? *p.pos_dev : 0;
   const int ban = (p.eos_id >= 0 && (p.pos_dev ? step + 1 : 0) < p.min_length) ? p.eos_id : -1;
-  const int nj = NJ ? NJ : (V + STEP - 1) / STEP;
-  float zr[NJ ? NJ : 1][4];
-  int nan_at = V;
-  float zmax = -INFINITY;
 
-  auto load = [&](int j, float (&z)[4]) {
+  auto fetch = [&](int j, float (&z)[4]) {  // logits of pass j as the caller's rules leave them; -0 becomes +0
     const int i0 = j * STEP + tid * 4;
+    load4(z0, i0, V, p.vec, z);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = i0 + i < V && i0 + i != ban ? logit_of(z0[i0 + i]) + 0.0f : -INFINITY;
+    for (int i = 0; i < 4; ++i) z[i] = i0 + i == ban ? -INFINITY : z[i] + 0.0f;
   };
-  auto each = [&](auto f) {                 // f(j, index, logit) for the tokens of this thread, in index order
-    if constexpr (NJ > 0) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { const int idx = j * STEP + tid * 4 + i; if (idx < V) f(j, idx, zr[j][i]); }
+  auto get = [&](int j, float (&z)[4]) {
+    if constexpr (ROW) {
+      const float4 v = *reinterpret_cast<const float4*>(zs + j * STEP + tid * 4);
+      z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w;
     } else {
-      for (int j = 0; j < nj; ++j) {
-        float z[4];
-        load(j, z);
+      fetch(j, z);
+    }
+  };
+  auto each = [&](auto f) {                 // f(index, logit) for the tokens of this thread, in index order
+#pragma unroll 1
+    for (int j = 0; j < nj; ++j) {
+      float z[4];
+      get(j, z);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const int idx = j * STEP + tid * 4 + i; if (idx < V) f(j, idx, z[i]); }
-      }
+      for (int i = 0; i < 4; ++i) { const int idx = j * STEP + tid * 4 + i; if (idx < V) f(idx, z[i]); }
     }
   };
 
-  if constexpr (NJ > 0) {
+  int nan_at = V;
+  float tmax = -INFINITY;                   // maximum of this thread's tokens
+  if constexpr (ROW) {
+    float z[ROW_MAX][4];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) load(j, zr[j]);
+    for (int j = 0; j < ROW_MAX; ++j) if (j < nj) fetch(j, z[j]);   // every load in flight before the first is used
+#pragma unroll
+    for (int j = 0; j < ROW_MAX; ++j)
+      if (j < nj) {
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+          tmax = fmaxf(tmax, z[j][i]);
+          if (z[j][i] != z[j][i]) nan_at = min(nan_at, j * STEP + tid * 4 + i);
+        }
+        *reinterpret_cast<float4*>(zs + j * STEP + tid * 4) = make_float4(z[j][0], z[j][1], z[j][2], z[j][3]);   // read by the same thread only
+      }
+  } else {
+    each([&](int idx, float z) {
+      if (z != z) nan_at = min(nan_at, idx);
+      tmax = fmaxf(tmax, z);
+    });
   }
-  each([&](int, int idx, float z) {
-    if (z != z) nan_at = min(nan_at, idx);
-    zmax = fmaxf(zmax, z);
-  });
-  zmax = wave_max(zmax);
-  if (tid == 0) { s_nan = V; s_pick = -1; s_n = 0; s_bin = NBIN; }
+  float zmax = wave_max(tmax);
+  if (tid == 0) { s_nan = V; s_n = 0; s_bin = NBIN; }
   if (lane == 0) s_max[wave] = zmax;
-  for (int b = tid; b < NBIN; b += NT) { s_cnt[b] = 0; s_mass[b] = 0; }
+  s_mass[tid] = 0; s_mass[tid + NT] = 0;
   __syncthreads();
   if (nan_at < V) atomicMin(&s_nan, nan_at);
 #pragma unroll
@@ -129,12 +179,13 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     if (tid == 0) finish(s_nan, __uint_as_float(0x7fc00000u));
     return;
   }
+  const float uf = p.u[(p.pos_dev ? (long)max(0, min(step, p.u_steps - 1)) * p.u_ld : 0) + row];
+  const double u = (double)fmaxf(uf, 0.f);
 
-  auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * p.bin_scale, (float)(NBIN - 1)); };
-  auto weight = [&](float z) -> double { return z == zmax ? 1.0 : exp(((double)z - (double)zmax) * p.inv_temp); };
-  auto mass = [&](float z) -> u64 {         // round to nearest: 2^46 w < 2^52, so the sum below holds it in its low bits
-    return (u64)__double_as_longlong(weight(z) * ONE + 4503599627370496.0) & 0xfffffffffffffull;
-  };
+  auto far_of = [&](float z) { return z == zmax ? 0.f : (zmax - z) * p.bin_scale; };      // in bins
+  auto bin_of = [&](float z) { return (int)fminf(far_of(z), (float)(NBIN - 1)); };
+  auto weight = [&](float z) -> double { return z == zmax ? 1.0 : exp2_neg(((double)z - (double)zmax) * p.exp2_scale); };
+  auto log_prob = [&](float z, u64 total) { return (float)((z == zmax ? 0.0 : ((double)z - (double)zmax) * p.inv_temp) - log((double)total / ONE)); };
 
   // bin of the boundary: the first one at which the running sum (of counts or masses) reaches the goal; s_base = the sum before it
   auto find_bin = [&](auto value, auto reached) {
@@ -150,12 +201,70 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     else if (!reached(pre + a) && reached(pre + a + b)) { s_bin = 2 * tid + 1; s_base = pre + a; }
     __syncthreads();
   };
-  // the last kept token of that bin, as an order key: the first one at which the running sum of `value` over the bin's tokens in order reaches
-  // the goal.  `in` = tokens that take part at all
+  auto clear = [&]() { s_mass[tid] = 0; s_mass[tid + NT] = 0; __syncthreads(); };
+  const bool cut_k = p.top_k > 0 && p.top_k < V;
+
+  // Small top-k: the k-th largest of the 1024 threads' maxima is a lower bound of the k-th largest logit, so the tokens at or above (the bin of) it
+  // contain the first k, and there are few more of them.  Everything else is decided among these candidates.
+  if (cut_k && p.top_k <= SMALL_K) {
+    const int b0 = bin_of(tmax);
+    if (tid * 4 < V && b0 < NBIN - 1) atomicAdd(&s_cnt[b0], 1u);
+    __syncthreads();
+    const u64 k = (u64)p.top_k;
+    find_bin([&](int b) { return (u64)s_cnt[b]; }, [&](u64 s) { return s >= k; });
+    const int bin = s_bin;
+    if (bin < NBIN - 1) {
+      const float limit = (float)(bin + 1);
+      each([&](int idx, float z) {
+        if (far_of(z) < limit) {
+          const int at = atomicAdd(&s_n, 1);
+          if (at < SMALL_N) s_key[at] = order_key(z, idx);
+        }
+      });
+      __syncthreads();
+      const int n = s_n;
+      if (n <= SMALL_N) {                   // the same for the whole block
+        u64 key = 0, w = 0;
+        double wd = 0.0;
+        float z = 0.f;
+        bool in = false;
+        if (tid < n) {
+          key = s_key[tid];
+          z = key_logit(key);
+          int rank = 0;
+          for (int i = 0; i < n; ++i) rank += s_key[i] < key ? 1 : 0;
+          in = rank < p.top_k;
+          if (in) { wd = weight(z); w = mass_of(wd); }
+          s_w[tid] = w;
+        }
+        __syncthreads();
+        u64 total = 0, pre = 0;
+        if (tid < n)
+          for (int i = 0; i < n; ++i) { const u64 x = s_w[i]; total += x; pre += s_key[i] < key ? x : 0; }
+        __syncthreads();
+        const bool keep = in && w > 0 && wd >= p.min_p && (p.top_p >= 1.0 || (double)pre < p.top_p * (double)total);
+        if (tid < n) s_w[tid] = keep ? w : 0;
+        __syncthreads();
+        if (keep) {
+          u64 run = 0;
+          total = 0;
+          for (int i = 0; i < n; ++i) { const u64 x = s_w[i]; total += x; run += (uint32_t)s_key[i] <= (uint32_t)key ? x : 0; }
+          const double goal = u * (double)total;
+          if (((double)run > goal && !((double)(run - w) > goal)) || (!((double)total > goal) && run == total)) finish((int)(uint32_t)key, log_prob(z, total));
+        }
+        return;
+      }
+    }
+    __syncthreads();
+    clear();
+  }
+
+  // the last kept token of the boundary's bin, as an order key: the first one at which the running sum of `value` over the bin's tokens in order
+  // reaches the goal.  `in` = tokens that take part at all
   auto resolve = [&](auto in, auto value, auto reached) -> u64 {
     const int bin = s_bin;
     const u64 base = s_base;
-    each([&](int, int idx, float z) {
+    each([&](int idx, float z) {
       if (bin_of(z) == bin && in(z, idx)) {
         const int at = atomicAdd(&s_n, 1);
         if (at < CAP) { s_key[at] = order_key(z, idx); s_w[at] = value(z); }
@@ -178,7 +287,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     while (lo < hi) {
       const u64 mid = lo + ((hi - lo) >> 1);
       u64 s = 0;
-      each([&](int, int idx, float z) {
+      each([&](int idx, float z) {
         if (bin_of(z) == bin && in(z, idx) && order_key(z, idx) <= mid) s += value(z);
       });
       s = block_sum64(s, s_red, tid);
@@ -188,67 +297,53 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   };
 
   u64 thr = ~0ull;                          // order key of the last token that top-k and top-p keep
-  if (p.top_k > 0 && p.top_k < V) {
-    each([&](int, int, float z) { const int b = bin_of(z); if (b < NBIN - 1) atomicAdd(&s_cnt[b], 1u); });
+  if (cut_k) {
+    each([&](int, float z) { const int b = bin_of(z); if (b < NBIN - 1) atomicAdd(&s_cnt[b], 1u); });
     __syncthreads();
     const u64 k = (u64)p.top_k;
     find_bin([&](int b) { return (u64)s_cnt[b]; }, [&](u64 s) { return s >= k; });
     if (s_bin < NBIN - 1)                   // otherwise every token with any mass is among the first k
       thr = resolve([](float, int) { return true; }, [](float) { return (u64)1; }, [&](u64 s) { return s >= k; });
     __syncthreads();
+    clear();
   }
   if (p.top_p < 1.0) {
     const u64 kt = thr;
     u64 total = 0;
-    each([&](int, int idx, float z) {
+    each([&](int idx, float z) {
       const int b = bin_of(z);
-      if (b < NBIN - 1 && order_key(z, idx) <= kt) { const u64 m = mass(z); total += m; atomicAdd(&s_mass[b], m); }
+      if (b < NBIN - 1 && order_key(z, idx) <= kt) { const u64 m = mass_of(weight(z)); total += m; atomicAdd(&s_mass[b], m); }
     });
     total = block_sum64(total, s_red, tid);
     const double goal = p.top_p * (double)total;
     const auto reached = [&](u64 s) { return (double)s >= goal; };
     find_bin([&](int b) { return s_mass[b]; }, reached);
-    thr = resolve([&](float z, int idx) { return order_key(z, idx) <= kt; }, mass, reached);
+    thr = resolve([&](float z, int idx) { return order_key(z, idx) <= kt; }, [&](float z) { return mass_of(weight(z)); }, reached);
     __syncthreads();
   }
 
   // kept mass of each segment of 256 consecutive tokens (one wave of one pass); segments in index order are (pass, wave)
   u64* seg = s_mass;                        // [nj][16] <= 512
+  const float thr_z = thr == ~0ull ? -INFINITY : key_logit(thr);
+  const int thr_i = thr == ~0ull ? V : (int)(uint32_t)thr;
   auto kept = [&](float z, int idx) -> u64 {
-    if (bin_of(z) >= NBIN - 1 || order_key(z, idx) > thr) return 0;
+    if (idx >= V || z < thr_z || (z == thr_z && idx > thr_i)) return 0;
     const double w = weight(z);
-    return w >= p.min_p ? (u64)__double_as_longlong(w * ONE + 4503599627370496.0) & 0xfffffffffffffull : 0;
+    return w >= p.min_p ? mass_of(w) : 0;
   };
-  {
+#pragma unroll 1
+  for (int j = 0; j < nj; ++j) {
+    float z[4];
+    get(j, z);
     u64 own = 0;
-    int at = 0;
-    auto flush = [&](int j) {
-      const u64 s = wave_sum64(own);
-      if (lane == 0) seg[j * (NT / 64) + wave] = s;
-      own = 0;
-    };
-    if constexpr (NJ > 0) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { const int idx = j * STEP + tid * 4 + i; if (idx < V) own += kept(zr[j][i], idx); }
-        flush(j);
-      }
-    } else {
-      for (at = 0; at < nj; ++at) {
-        float z[4];
-        load(at, z);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { const int idx = at * STEP + tid * 4 + i; if (idx < V) own += kept(z[i], idx); }
-        flush(at);
-      }
-    }
+    for (int i = 0; i < 4; ++i) own += kept(z[i], j * STEP + tid * 4 + i);
+    own = wave_sum64(own);
+    if (lane == 0) seg[j * (NT / 64) + wave] = own;
   }
   __syncthreads();
   // the segment in which the running mass passes u * total (one wave: up to 512 segments, eight per lane), else the last one with any mass
   const int nseg = nj * (NT / 64);
-  const float uf = p.u[(p.pos_dev ? (long)max(0, min(step, p.u_steps - 1)) * p.u_ld : 0) + row];
-  const double u = (double)fmaxf(uf, 0.f);
   if (wave == 0) {
     u64 own = 0;
     for (int i = 0; i < 8; ++i) { const int sgi = lane * 8 + i; if (sgi < nseg) own += seg[sgi]; }
@@ -272,12 +367,13 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   __syncthreads();
   const int sg = s_bin, sj = sg / (NT / 64);
   if (wave == sg % (NT / 64)) {
-    const double goal = u * (double)s_thr;
+    const u64 total = s_thr;
+    const double goal = u * (double)total;
     float z[4];
-    load(sj, z);
+    get(sj, z);
     u64 m[4], own = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { const int idx = sj * STEP + tid * 4 + i; m[i] = idx < V ? kept(z[i], idx) : 0; own += m[i]; }
+    for (int i = 0; i < 4; ++i) { m[i] = kept(z[i], sj * STEP + tid * 4 + i); own += m[i]; }
     u64 run = s_base + wave_scan64(own, lane) - own;
     int found = -1, last = -1;
     float fz = 0.f, lz = 0.f;
@@ -289,22 +385,20 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     }
     const u64 any = __ballot(found >= 0), have = __ballot(last >= 0);
     const int src = any ? __builtin_ctzll(any) : 63 - __builtin_clzll(have);
-    if (lane == src) {
-      const float zp = any ? fz : lz;
-      const double d = zp == zmax ? 0.0 : ((double)zp - (double)zmax) * p.inv_temp;
-      finish(any ? found : last, (float)(d - log((double)s_thr / ONE)));
-    }
+    if (lane == src) finish(any ? found : last, log_prob(any ? fz : lz, total));
   }
 }
 
-template <typename T> int sample_launch(const SampleP& p, int rows, hipStream_t s) {
+template <typename T> int sample_launch(SampleP& p, int rows, hipStream_t s) {
   const int nj = (p.V + STEP - 1) / STEP;
-  const dim3 grid(rows), block(NT);
-  if (nj <= 1) hipLaunchKernelGGL((sample_kernel<T, 1>), grid, block, 0, s, p);
-  else if (nj <= 2) hipLaunchKernelGGL((sample_kernel<T, 2>), grid, block, 0, s, p);
-  else if (nj <= 4) hipLaunchKernelGGL((sample_kernel<T, 4>), grid, block, 0, s, p);
-  else if (nj <= 8) hipLaunchKernelGGL((sample_kernel<T, 8>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((sample_kernel<T, 0>), grid, block, 0, s, p);
+  p.vec = ((uintptr_t)p.logits % (4 * sizeof(T))) == 0 && p.ld % 4 == 0;
+  if (nj <= ROW_MAX) {
+    static bool attr = false;
+    if (!attr) { (void)hipFuncSetAttribute((const void*)sample_kernel<T, true>, hipFuncAttributeMaxDynamicSharedMemorySize, ROW_MAX * STEP * 4); attr = true; }
+    hipLaunchKernelGGL((sample_kernel<T, true>), dim3(rows), dim3(NT), (size_t)nj * STEP * 4, s, p);
+  } else {
+    hipLaunchKernelGGL((sample_kernel<T, false>), dim3(rows), dim3(NT), 0, s, p);
+  }
   V2S_LAUNCH_CHECK();
   return V2S_OK;
 }
@@ -322,7 +416,7 @@ extern "C" int v2s_sample_step(const void* logits, int32_t logits_dtype, int64_t
   V2S_CHECK(!seq_out || pos_dev, V2S_ERR_ARG, "v2s_sample_step: seq_out needs pos_dev");
   V2S_CHECK(!pos_dev || (u_ld >= rows && u_steps > 0), V2S_ERR_SHAPE, "v2s_sample_step: with pos_dev, u is a table of u_steps > 0 rows of u_ld >= rows numbers");
   SampleP p;
-  p.logits = logits; p.ld = ld; p.V = V; p.inv_temp = 1.0 / temperature; p.bin_scale = (float)((NBIN - 1) / (BIN_RANGE * temperature));
+  p.logits = logits; p.ld = ld; p.V = V; p.inv_temp = 1.0 / temperature; p.exp2_scale = 1.44269504088896340736 / temperature; p.bin_scale = (float)((NBIN - 1) / (BIN_RANGE * temperature));
   p.top_k = top_k; p.top_p = top_p; p.min_p = min_p; p.u = u; p.u_ld = u_ld; p.u_steps = u_steps; p.next_tok = (long*)next_tok; p.logp = logp; p.unfinished = unfinished;
   p.eos_id = eos_id; p.pad_id = pad_id; p.seq_out = (long*)seq_out; p.seq_ld = seq_ld; p.pos_dev = pos_dev; p.min_length = min_length;
   return logits_dtype == V2S_F32 ? sample_launch<float>(p, rows, (hipStream_t)stream) : sample_launch<bf16_t>(p, rows, (hipStream_t)stream);

@@ -763,14 +763,30 @@ def beam_sample_cand(logits, ld, rows, V, K, beam_scores, top_p, temperature, to
 
 
 # --------------------------------------------------------------------------------------------- 8-bit decoding
-def _operand(t, dtype, what: str, need: int = 0, like=None):
-    """Checks one operand: on the GPU that is current (the launch goes to its current stream), of this type, its last dimension contiguous, at
-    least ``need`` elements of storage behind its first one.  Returns its address (None for None)."""
+# A decode step is a chain of launches of a few microseconds, so the wrappers below keep their own cost low: an operand that is contiguous and large
+# enough passes in four comparisons, everything else goes through _strided, which words the refusals.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_F32, _BF16, _I8, _I32, _I64 = torch.float32, torch.bfloat16, torch.int8, torch.int32, torch.int64
+
+
+def _device(t) -> int:
+    """Index of the current device, which every operand has to live on: the launch goes to its current stream."""
+    return torch.cuda.current_device() if t.is_cuda else -2
+
+
+def _operand(t, dtype, dev: int, what: str, need: int = 0):
+    """Address of an operand of this type on device ``dev`` with at least ``need`` elements of storage behind its first one (None for None)."""
     if t is None:
         return None
+    if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= need:
+        return t.data_ptr()
+    return _strided(t, dtype, dev, what, need)
+
+
+def _strided(t, dtype, dev: int, what: str, need: int):
     _need(t, dtype, what)
-    if t.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"{what}: tensor lives on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if t.get_device() != dev:
+        raise RuntimeError(f"{what}: tensor lives on {t.device}, the launch goes to cuda:{dev}")
     if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous")
     have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
@@ -779,93 +795,86 @@ def _operand(t, dtype, what: str, need: int = 0, like=None):
     return t.data_ptr()
 
 
-def _span(rows: int, ld: int, cols: int) -> int:
-    return (rows - 1) * ld + cols
-
-
 def quant_rows_q8(x, q, scale, rows, cols, *, ldx=None, ldq=None):
     """int8 codes ``q`` [rows, ldq] and one fp32 scale per row of the rows of ``x`` (bf16 or fp32): weights once, activations per token."""
-    ldx, ldq = cols if ldx is None else ldx, cols if ldq is None else ldq
-    xt = x.dtype if x.dtype == torch.float32 else torch.bfloat16
-    xp, qp, sp = _operand(x, xt, "quant_rows_q8 x", _span(rows, ldx, cols)), _operand(q, torch.int8, "quant_rows_q8 q", _span(rows, ldq, cols)), \
-        _operand(scale, torch.float32, "quant_rows_q8 scale", rows)
-    _check(lib().v2s_quant_rows_q8(xp, V2S_F32 if xt == torch.float32 else V2S_BF16, ldx, qp, ldq, sp, rows, cols, stream_ptr()), "v2s_quant_rows_q8")
+    ldx, ldq, dev, f32 = ldx or cols, ldq or cols, _device(x), x.dtype is _F32
+    xp = _operand(x, _F32 if f32 else _BF16, dev, "quant_rows_q8 x", (rows - 1) * ldx + cols)
+    qp, sp = _operand(q, _I8, dev, "quant_rows_q8 q", (rows - 1) * ldq + cols), _operand(scale, _F32, dev, "quant_rows_q8 scale", rows)
+    _check(lib().v2s_quant_rows_q8(xp, V2S_F32 if f32 else V2S_BF16, ldx, qp, ldq, sp, rows, cols, _raw_stream(dev)), "v2s_quant_rows_q8")
 
 
 def rmsnorm_q8(x, w, q, scale, rows, cols, eps, *, delta=None, h=None, ldx=None, ldd=None, ldh=None, ldq=None):
     """s = bf16(x + delta) (to ``h`` if given), then T5 RMSNorm and int8 codes ``q`` with one ``scale`` per row, in one pass."""
-    ldx, ldd, ldh, ldq = (cols if v is None else v for v in (ldx, ldd, ldh, ldq))
-    n = "rmsnorm_q8 "
-    xp, wp = _operand(x, torch.bfloat16, n + "x", _span(rows, ldx, cols)), _operand(w, torch.float32, n + "w", cols)
-    dp, hp = _operand(delta, torch.bfloat16, n + "delta", _span(rows, ldd, cols)), _operand(h, torch.bfloat16, n + "h", _span(rows, ldh, cols))
-    qp, sp = _operand(q, torch.int8, n + "q", _span(rows, ldq, cols)), _operand(scale, torch.float32, n + "scale", rows)
-    _check(lib().v2s_rmsnorm_q8(xp, ldx, dp, ldd, wp, hp, ldh, qp, ldq, sp, rows, cols, eps, stream_ptr()), "v2s_rmsnorm_q8")
+    ldx, ldd, ldh, ldq, dev, last = ldx or cols, ldd or cols, ldh or cols, ldq or cols, _device(x), rows - 1
+    xp, wp = _operand(x, _BF16, dev, "rmsnorm_q8 x", last * ldx + cols), _operand(w, _F32, dev, "rmsnorm_q8 w", cols)
+    dp, hp = _operand(delta, _BF16, dev, "rmsnorm_q8 delta", last * ldd + cols), _operand(h, _BF16, dev, "rmsnorm_q8 h", last * ldh + cols)
+    qp, sp = _operand(q, _I8, dev, "rmsnorm_q8 q", last * ldq + cols), _operand(scale, _F32, dev, "rmsnorm_q8 scale", rows)
+    _check(lib().v2s_rmsnorm_q8(xp, ldx, dp, ldd, wp, hp, ldh, qp, ldq, sp, rows, cols, eps, _raw_stream(dev)), "v2s_rmsnorm_q8")
 
 
 def dequant_q8(q, scale, y, rows, cols, *, ldq=None, ldy=None):
     """y[rows, ldy] (bf16) = scale[row] * q[row]: the values that codes stand for."""
-    ldq, ldy = cols if ldq is None else ldq, cols if ldy is None else ldy
-    qp, sp = _operand(q, torch.int8, "dequant_q8 q", _span(rows, ldq, cols)), _operand(scale, torch.float32, "dequant_q8 scale", rows)
-    yp = _operand(y, torch.bfloat16, "dequant_q8 y", _span(rows, ldy, cols))
-    _check(lib().v2s_dequant_q8(qp, ldq, sp, yp, ldy, rows, cols, stream_ptr()), "v2s_dequant_q8")
+    ldq, ldy, dev = ldq or cols, ldy or cols, _device(q)
+    qp, sp = _operand(q, _I8, dev, "dequant_q8 q", (rows - 1) * ldq + cols), _operand(scale, _F32, dev, "dequant_q8 scale", rows)
+    yp = _operand(y, _BF16, dev, "dequant_q8 y", (rows - 1) * ldy + cols)
+    _check(lib().v2s_dequant_q8(qp, ldq, sp, yp, ldy, rows, cols, _raw_stream(dev)), "v2s_dequant_q8")
 
 
 def gemm_q8(A, B, sA, sB, C_out, M, N, K, *, lda=None, ldb=None, ldc=None, alpha=1.0, bias=None, act=ACT_NONE, residual=None, ldr=None):
     """C[M, N] = act(alpha * sA[m] * sB[n] * A(m, :) . B(n, :) + bias) + residual with int8 A (token codes) and B (weight codes [out, in])."""
-    a = GemmQ8Args()
-    a.M, a.N, a.K = M, N, K
-    a.lda, a.ldb = K if lda is None else lda, K if ldb is None else ldb
-    a.ldc, a.ldr = N if ldc is None else ldc, N if ldr is None else ldr
-    n = "gemm_q8 "
-    a.A, a.B = _operand(A, torch.int8, n + "A", _span(M, a.lda, K)), _operand(B, torch.int8, n + "B", _span(N, a.ldb, K))
-    a.sA, a.sB = _operand(sA, torch.float32, n + "sA", M), _operand(sB, torch.float32, n + "sB", N)
-    ct = C_out.dtype if C_out.dtype == torch.float32 else torch.bfloat16
-    a.C = _operand(C_out, ct, n + "C", _span(M, a.ldc, N))
-    a.c_dtype = V2S_F32 if ct == torch.float32 else V2S_BF16
+    a, dev, f32, last = GemmQ8Args(), _device(A), C_out.dtype is _F32, M - 1
+    lda, ldb, ldc, ldr = lda or K, ldb or K, ldc or N, ldr or N
+    a.M, a.N, a.K, a.lda, a.ldb, a.ldc, a.ldr = M, N, K, lda, ldb, ldc, ldr
+    a.A, a.B = _operand(A, _I8, dev, "gemm_q8 A", last * lda + K), _operand(B, _I8, dev, "gemm_q8 B", (N - 1) * ldb + K)
+    a.sA, a.sB = _operand(sA, _F32, dev, "gemm_q8 sA", M), _operand(sB, _F32, dev, "gemm_q8 sB", N)
+    a.C, a.c_dtype = _operand(C_out, _F32 if f32 else _BF16, dev, "gemm_q8 C", last * ldc + N), V2S_F32 if f32 else V2S_BF16
     a.alpha, a.act = alpha, act
-    a.bias, a.residual = _operand(bias, torch.float32, n + "bias", N), _operand(residual, torch.bfloat16, n + "residual", _span(M, a.ldr, N))
+    if bias is not None:
+        a.bias = _operand(bias, _F32, dev, "gemm_q8 bias", N)
+    if residual is not None:
+        a.residual = _operand(residual, _BF16, dev, "gemm_q8 residual", last * ldr + N)
     kt = KernelTimer.active
     if kt is not None:
         e0 = kt.begin()
-    _check(lib().v2s_gemm_q8(C.byref(a), stream_ptr()), "v2s_gemm_q8")
+    _check(lib().v2s_gemm_q8(C.byref(a), _raw_stream(dev)), "v2s_gemm_q8")
     if kt is not None:
         kt.end("gemm_q8" + (f":{M}x{N}x{K}" if kt.detail else ""), 2.0 * M * N * K, e0)
 
 
-def _kv_q8(kq, ks, vq, vs, what: str) -> KvQ8:
+def _kv_q8(kq, ks, vq, vs, dev: int, what: str) -> KvQ8:
     """The cache as four tensors: codes [entries, heads, maxlen, 64] int8 and scales [entries, heads, maxlen] fp32."""
-    if kq.dim() != 4 or kq.shape[3] != 64 or vq.shape != kq.shape or ks.shape != kq.shape[:3] or vs.shape != kq.shape[:3]:
+    c, shape = KvQ8(), kq.shape
+    if len(shape) != 4 or shape[3] != 64 or vq.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
         raise ValueError(f"{what}: a cache is codes [entries, heads, maxlen, 64] and scales [entries, heads, maxlen] for keys and for values")
-    c = KvQ8()
-    c.entries, c.heads, c.maxlen = kq.shape[:3]
-    c.e_rows, c.h_rows = ks.stride(0), ks.stride(1)
-    for codes, scales in ((kq, ks), (vq, vs)):
-        if scales.stride() != (c.e_rows, c.h_rows, 1) or codes.stride() != (c.e_rows * 64, c.h_rows * 64, 64, 1):
-            raise ValueError(f"{what}: codes and scales of a cache share their row strides, the rows of a head are contiguous")
-    c.k, c.ks = _operand(kq, torch.int8, what + " k"), _operand(ks, torch.float32, what + " ks")
-    c.v, c.vs = _operand(vq, torch.int8, what + " v"), _operand(vs, torch.float32, what + " vs")
+    e, h, one = strides = ks.stride()
+    if one != 1 or vs.stride() != strides or kq.stride() != (e * 64, h * 64, 64, 1) or vq.stride() != (e * 64, h * 64, 64, 1):
+        raise ValueError(f"{what}: codes and scales of a cache share their row strides, the rows of a head are contiguous")
+    c.entries, c.heads, c.maxlen, c.e_rows, c.h_rows = shape[0], shape[1], shape[2], e, h
+    c.k, c.ks = _operand(kq, _I8, dev, what + " k"), _operand(ks, _F32, dev, what + " ks")
+    c.v, c.vs = _operand(vq, _I8, dev, what + " v"), _operand(vs, _F32, dev, what + " vs")
     return c
 
 
-def _kv_move(fn: str, k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count):
-    c = _kv_q8(kq, ks, vq, vs, fn)
-    width = c.heads * 64
-    if k.dim() != 3 or k.shape != v.shape or k.shape[0] != c.entries or k.shape[1] < T or k.shape[2] < width or k.stride() != v.stride():
-        raise ValueError(f"{fn}: k and v are [{c.entries}, >= {T}, >= {width}] with the same strides, got {tuple(k.shape)} and {tuple(v.shape)}")
-    kp, vp = _operand(k, torch.bfloat16, fn + " k"), _operand(v, torch.bfloat16, fn + " v")
-    pp, dp, np_ = (_operand(t, torch.int32, f"{fn} {n}", m) for t, n, m in ((pos, "pos", c.entries), (pos_dev, "pos_dev", 1), (count, "count", c.entries)))
-    _check(getattr(lib(), "v2s_" + fn)(C.byref(c), kp, vp, k.stride(0), k.stride(1), T, pos0, pp, dp, np_, stream_ptr()), "v2s_" + fn)
+def _kv_move(fn, name: str, k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count):
+    dev = _device(kq)
+    c = _kv_q8(kq, ks, vq, vs, dev, name)
+    shape, (bs, rs, _) = k.shape, k.stride()
+    if v.shape != shape or shape[0] != c.entries or shape[1] < T or shape[2] < c.heads * 64 or v.stride() != k.stride():
+        raise ValueError(f"{name}: k and v are [{c.entries}, >= {T}, >= {c.heads * 64}] with the same strides, got {tuple(shape)} and {tuple(v.shape)}")
+    _check(fn(C.byref(c), _operand(k, _BF16, dev, name + " k"), _operand(v, _BF16, dev, name + " v"), bs, rs, T, pos0,
+              _operand(pos, _I32, dev, name + " pos", c.entries), _operand(pos_dev, _I32, dev, name + " pos_dev", 1),
+              _operand(count, _I32, dev, name + " count", c.entries), _raw_stream(dev)), "v2s_" + name)
 
 
 def kv_append_q8(k, v, kq, ks, vq, vs, T, *, pos0=0, pos=None, pos_dev=None, count=None):
     """Quantises T new tokens per entry (k, v: bf16 [entries, T, heads * 64]) as they enter the int8 cache, at ``pos`` (int32 [entries]) or ``pos0``,
     plus ``*pos_dev``; ``count`` (int32 [entries]) limits an entry to its first tokens.  Tokens outside the cache are dropped."""
-    _kv_move("kv_append_q8", k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count)
+    _kv_move(lib().v2s_kv_append_q8, "kv_append_q8", k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count)
 
 
 def kv_read_q8(kq, ks, vq, vs, k, v, T, *, pos0=0, pos=None, pos_dev=None, count=None):
     """Reads T tokens per entry back as bf16 rows of the attention's layout; rows that take no part stay as they are."""
-    _kv_move("kv_read_q8", k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count)
+    _kv_move(lib().v2s_kv_read_q8, "kv_read_q8", k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count)
 
 
 def decode_attn_q8_workspace(B, H, Nk, device):
@@ -877,43 +886,45 @@ def decode_attn_q8_workspace(B, H, Nk, device):
 def decode_attn_q8(q, kq, ks, vq, vs, o, Nk, *, group=1, klen=None, pos_dev=None, bias_maxlen=0, bias_row=None, key_mask=None, scale=1.0, workspace=None):
     """o[B, heads * 64] = attention of one query row per (row, head) over the first ``Nk`` (or ``klen[entry]``, or ``*pos_dev + 1``) keys of the int8
     cache; ``group`` consecutive rows of q share an entry.  See include/vid2seq_hip.h for masks and empty rows."""
-    a = DecodeAttnQ8Args()
-    n = "decode_attn_q8"
-    a.cache = _kv_q8(kq, ks, vq, vs, n)
-    E, H = a.cache.entries, a.cache.heads
-    if q.dim() != 2 or o.dim() != 2 or q.shape != o.shape or q.shape[0] != E * group or q.shape[1] != H * 64:
-        raise ValueError(f"{n}: q and o are [{E * group}, {H * 64}], got {tuple(q.shape)} and {tuple(o.shape)}")
-    a.B, a.Nk, a.group = E * group, Nk, group
-    a.q, a.q_bs, a.o, a.o_bs = _operand(q, torch.bfloat16, n + " q"), q.stride(0), _operand(o, torch.bfloat16, n + " o"), o.stride(0)
+    a, dev, n = DecodeAttnQ8Args(), _device(q), "decode_attn_q8"
+    c = a.cache = _kv_q8(kq, ks, vq, vs, dev, n)
+    E, H = c.entries, c.heads
+    B = E * group
+    if q.shape != (B, H * 64) or o.shape != (B, H * 64):
+        raise ValueError(f"{n}: q and o are [{B}, {H * 64}], got {tuple(q.shape)} and {tuple(o.shape)}")
+    a.B, a.Nk, a.group, a.scale = B, Nk, group, scale
+    a.q, a.q_bs, a.o, a.o_bs = _operand(q, _BF16, dev, n + " q"), q.stride(0), _operand(o, _BF16, dev, n + " o"), o.stride(0)
     if bias_row is not None:
         if bias_row.dim() != 2 or bias_row.shape[0] != H:
             raise ValueError(f"{n}: bias_row is [heads, keys], got {tuple(bias_row.shape)}")
         a.bias_ld = bias_row.stride(0) if H > 1 else bias_row.shape[1]
-        a.bias_row = _operand(bias_row, torch.float32, n + " bias_row", _span(H, a.bias_ld, 2 * bias_maxlen - 1 if pos_dev is not None else Nk))
+        a.bias_row = _operand(bias_row, _F32, dev, n + " bias_row", (H - 1) * a.bias_ld + (2 * bias_maxlen - 1 if pos_dev is not None else Nk))
     if key_mask is not None:
         if key_mask.dim() != 2 or key_mask.shape[0] != E:
             raise ValueError(f"{n}: key_mask is [entries, keys], got {tuple(key_mask.shape)}")
         a.mask_ld = key_mask.stride(0) if E > 1 else key_mask.shape[1]
-        a.key_mask = _operand(key_mask, torch.uint8, n + " key_mask", _span(E, a.mask_ld, Nk))
-    a.pos_dev, a.bias_maxlen, a.klen = _operand(pos_dev, torch.int32, n + " pos_dev", 1), bias_maxlen, _operand(klen, torch.int32, n + " klen", E)
-    a.scale = scale
+        a.key_mask = _operand(key_mask, torch.uint8, dev, n + " key_mask", (E - 1) * a.mask_ld + Nk)
+    if pos_dev is not None:
+        a.pos_dev, a.bias_maxlen = _operand(pos_dev, _I32, dev, n + " pos_dev", 1), bias_maxlen
+    if klen is not None:
+        a.klen = _operand(klen, _I32, dev, n + " klen", E)
     if workspace is not None:
-        a.workspace, a.workspace_bytes = _operand(workspace, torch.float32, n + " workspace"), workspace.numel() * 4
-    _check(lib().v2s_decode_attn_q8(C.byref(a), stream_ptr()), "v2s_decode_attn_q8")
+        a.workspace, a.workspace_bytes = _operand(workspace, _F32, dev, n + " workspace"), workspace.numel() * 4
+    _check(lib().v2s_decode_attn_q8(C.byref(a), _raw_stream(dev)), "v2s_decode_attn_q8")
 
 
 def sample_step(logits, rows, V, u, next_tok, *, ld=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logp=None, unfinished=None, eos_id=-1, pad_id=0,
                 seq_out=None, seq_ld=0, pos_dev=None, min_length=0):
     """One token per row of ``logits`` (fp32 or bf16 [rows, ld]) from temperature, top-k, top-p, min-p and the given numbers ``u`` (fp32 [rows] in
     [0, 1), or [steps, rows] with ``pos_dev``): every draw is a function of its arguments.  ``logp``: log-probability of the token among the kept ones."""
-    n = "sample_step "
-    lt = logits.dtype if logits.dtype == torch.float32 else torch.bfloat16
-    ld = (logits.stride(0) if logits.dim() == 2 and rows > 1 else V) if ld is None else ld
-    if u.dim() != (2 if pos_dev is not None else 1) or u.shape[-1] < rows:
+    n, dev, f32 = "sample_step", _device(logits), logits.dtype is _F32
+    ld = ld or (logits.stride(0) if logits.dim() == 2 and rows > 1 else V)
+    if u.dim() != (1 if pos_dev is None else 2) or u.shape[-1] < rows:
         raise ValueError(f"sample_step: u is [rows], or [steps, rows] with pos_dev, got {tuple(u.shape)} for {rows} rows")
-    steps, u_ld = (u.shape[0], u.stride(0) if u.shape[0] > 1 else u.shape[1]) if u.dim() == 2 else (0, 0)
-    lp = _operand(logits, lt, n + "logits", _span(rows, ld, V))
-    up, tp, pp = _operand(u, torch.float32, n + "u", rows), _operand(next_tok, torch.int64, n + "next_tok", rows), _operand(logp, torch.float32, n + "logp", rows)
-    fp, sp, dp = _operand(unfinished, torch.int32, n + "unfinished", rows), _operand(seq_out, torch.int64, n + "seq_out", rows * seq_ld), _operand(pos_dev, torch.int32, n + "pos_dev", 1)
-    _check(lib().v2s_sample_step(lp, V2S_F32 if lt == torch.float32 else V2S_BF16, ld, rows, V, temperature, top_k, top_p, min_p, up, u_ld, steps, tp, pp, fp,
-                                 eos_id, pad_id, sp, seq_ld, dp, min_length, stream_ptr()), "v2s_sample_step")
+    steps, u_ld = (0, 0) if pos_dev is None else (u.shape[0], u.stride(0) if u.shape[0] > 1 else u.shape[1])
+    zp = _operand(logits, _F32 if f32 else _BF16, dev, n + " logits", (rows - 1) * ld + V)
+    up, tp, pp = _operand(u, _F32, dev, n + " u", rows), _operand(next_tok, _I64, dev, n + " next_tok", rows), _operand(logp, _F32, dev, n + " logp", rows)
+    fp, sp = _operand(unfinished, _I32, dev, n + " unfinished", rows), _operand(seq_out, _I64, dev, n + " seq_out", rows * seq_ld)
+    dp = _operand(pos_dev, _I32, dev, n + " pos_dev", 1)
+    _check(lib().v2s_sample_step(zp, V2S_F32 if f32 else V2S_BF16, ld, rows, V, temperature, top_k, top_p, min_p, up, u_ld, steps, tp, pp, fp, eos_id, pad_id, sp,
+                                 seq_ld, dp, min_length, _raw_stream(dev)), "v2s_sample_step")
