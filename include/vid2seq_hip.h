@@ -552,7 +552,7 @@ int v2s_kv_read_q8(const v2s_kv_q8* cache, void* k, void* v, int64_t dst_bs, int
  * The keys of an entry are the first klen[e] (device, clamped to [0, Nk]), or *pos_dev + 1, or Nk.  Masked keys (key_mask[e][j] == 0) have no part in the
  * result whatever they hold; a row that sees no key (all masked, or bias -infinity everywhere) gets the mean of its keys' values, as the reference's
  * finfo.min masks give (modeling_t5.py:996,559); an entry without keys gets zeros.  group query rows (beams) share an entry: B = entries * group.
- * Pieces of 512 keys are summed by blocks of their own and joined, so a sequence's result does not depend on its batch; Nk > 512 needs
+ * Pieces of 1280 keys are summed by blocks of their own and joined, so a sequence's result does not depend on its batch; Nk > 1280 needs
  * v2s_decode_attn_q8_workspace_floats(B, heads, Nk) floats of workspace, which no other launch in flight may use. */
 typedef struct v2s_decode_attn_q8_args {
   int32_t B, Nk, group;

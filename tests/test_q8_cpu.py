@@ -75,8 +75,8 @@ def test_attention_refusals():
                      (dict(bias_row=P, bias_ld=200, pos_dev=P, bias_maxlen=39), "bias"), (dict(key_mask=P, mask_ld=39), "mask_ld"), (dict(q_bs=120), "shorter"), (dict(q_bs=132), "multiple of 8"),
                      (dict(q=P + 8), "aligned")):
         refused(call(**kw), word)
-    long = dict(cache=cache(e_rows=2000, h_rows=1000, maxlen=1000), Nk=1000)
-    need = L.lib().v2s_decode_attn_q8_workspace_floats(3, 2, 1000)
+    long = dict(cache=cache(e_rows=4000, h_rows=2000, maxlen=2000), Nk=2000)
+    need = L.lib().v2s_decode_attn_q8_workspace_floats(3, 2, 2000)
     assert need > 0 and L.lib().v2s_decode_attn_q8_workspace_floats(3, 2, 40) == 0
     refused(call(**long), "workspace")
     refused(call(**long, workspace=P, workspace_bytes=need * 4 - 1), "workspace")

@@ -304,7 +304,8 @@ def make_cache(E, H, n, seed):
 
 
 @pytest.mark.parametrize("E,G,H,n", [(1, 1, 1, 1), (2, 1, 3, 2), (3, 1, 12, 63), (2, 2, 4, 64), (2, 3, 2, 65), (64, 1, 12, 100), (2, 4, 12, 511), (2, 5, 2, 512),
-                                     (3, 1, 2, 513), (2, 8, 3, 1100), (1, 4, 16, 5000), (4, 1, 2, 1537), (1, 12, 2, 700), (1, 17, 1, 1030)])
+                                     (3, 1, 2, 513), (2, 8, 3, 1100), (1, 4, 16, 5000), (4, 1, 2, 1537), (1, 12, 2, 700), (1, 17, 1, 1030), (2, 1, 2, 1280), (2, 16, 2, 1281),
+                                     (1, 33, 2, 2561)])
 @pytest.mark.parametrize("form", ["plain", "len", "mask_bias", "all"])
 def test_decode_attn_q8(E, G, H, n, form):
     cache = make_cache(E, H, n, n + G)
@@ -317,7 +318,7 @@ def test_decode_attn_q8(E, G, H, n, form):
         bias = torch.randn(H, n + 5, generator=g).to(DEV)
         bias[:, ::7] = -math.inf
         if n > 600:
-            mask[0, :600] = 0                # a whole piece without a visible key
+            mask[0, :min(n - 20, 1300)] = 0      # whole pieces without a visible key
     o = attend(q, cache, n, group=G, klen=klen, key_mask=mask, bias_row=bias, scale=0.5)
     want, tol = attn_ref(q, *cache, 0.5, G, klen, mask, bias)
     assert ((o.double() - want).abs() <= tol).all(), float(((o.double() - want).abs() / tol).max())
@@ -325,7 +326,7 @@ def test_decode_attn_q8(E, G, H, n, form):
 
 def test_decode_attn_q8_rows_without_keys_and_hidden_garbage():
     """No keys: zeros.  No visible key: the mean.  Masked keys and keys behind the length hold NaN and infinities: no part of any result."""
-    for n in (40, 700):
+    for n in (40, 700, 1500):
         E, G, H = 5, 2, 3
         cache = make_cache(E, H, n, n)
         q = rnd(E * G, H * 64, seed=1)
@@ -365,12 +366,12 @@ def test_decode_attn_q8_large_and_lowest_scores():
 
 def test_decode_attn_q8_counter_bias_and_batch_independence():
     """pos_dev: *pos_dev + 1 keys and the bias row of that position; a sequence alone gives the bits it gives in a batch."""
-    E, H, n = 6, 4, 900
+    E, H, n = 6, 4, 1400
     cache = make_cache(E, H, n, 6)
     q = rnd(E, H * 64, seed=5)
     diag = rnd(H, 2 * n - 1, seed=7, dtype=torch.float32)
     ctr = torch.zeros(1, dtype=torch.int32, device=DEV)
-    for t in (0, 1, 511, 512, 899):
+    for t in (0, 1, 511, 512, 1279, 1280, 1399):
         ctr.fill_(t)
         o = attend(q, cache, n, pos_dev=ctr, bias_row=diag, bias_maxlen=n)
         row = diag[:, n - 1 - t:2 * n - 1 - t].contiguous()

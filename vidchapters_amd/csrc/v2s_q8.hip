@@ -10,6 +10,7 @@
 namespace {
 
 typedef signed char i8;
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 constexpr float Q8_TINY = 127.0f * 1.17549435e-38f;
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(256) void kv_read_q8_kernel(const KvQ8 p) {
 // A masked key is not part of the sums at all (whatever its codes and scale hold); a query that sees no key -- all masked, or a bias of
 // -infinity everywhere -- gets the mean of its keys' values, as softmax over equal scores gives (modeling_t5.py:996,559), and a query without
 // keys gets zeros.
-constexpr int PIECE = 512;            // keys per block; fixed, so that a sequence's result does not depend on its batch
+constexpr int PIECE = 1280;           // keys per block; fixed, so that a sequence's result does not depend on its batch
 constexpr float LOG2E = 1.44269504088896340736f;
 
 struct AttnQ8 {
@@ -252,157 +253,190 @@ __device__ __forceinline__ int attn_q8_keys(const AttnQ8& p, int e) {
 // exp(m - M) of a running maximum; the difference is taken first, so that scores of any finite size are told apart
 __device__ __forceinline__ float rescale(float m, float M) { return m == M ? 1.f : __builtin_amdgcn_exp2f((m - M) * LOG2E); }
 
-template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-
-// mean of the values of n keys of one (entry, head) by a block of 256 threads; lds: 256 floats.  The rare row without a visible key.
+// mean of the values of n keys of one (entry, head) by the first 256 threads of a block; lds: 256 floats.  The rare row without a visible key.
 __device__ float attn_q8_mean(const i8* vq, const float* vs, int n, float* lds) {
   const int d = threadIdx.x & 63, part = threadIdx.x >> 6;
   float s = 0.f;
-  for (int k = part; k < n; k += 4) s += vs[k] * (float)vq[(long)k * 64 + d];
+  if (part < 4)
+    for (int k = part; k < n; k += 4) s += vs[k] * (float)vq[(long)k * 64 + d];
   __syncthreads();
-  lds[threadIdx.x] = s;
+  if (part < 4) lds[threadIdx.x] = s;
   __syncthreads();
   s = lds[d] + lds[64 + d] + lds[128 + d] + lds[192 + d];
   __syncthreads();
   return n > 0 ? s / (float)n : 0.f;
 }
 
-// block = 4 waves = up to PIECE keys of one (entry, head) against G of its queries.  lane = (key slot lane >> 2, 16 dimensions lane & 3): one
-// wave load is 16 whole keys (1 KiB)
-template <int G>
-__global__ __launch_bounds__(256) void attn_q8_kernel(const AttnQ8 p) {
-  __shared__ float s_m[G][4], s_l[G][4], s_o[G][4][64], s_red[256];
-  __shared__ unsigned long long s_bits[PIECE / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slot = lane >> 2, c = lane & 3;
+// eight codes as bf16, exactly
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
+  float f[8];
+  q8_unpack4(lo, f); q8_unpack4(hi, f + 4);
+  uint4 r;
+  r.x = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);
+  r.y = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u);
+  r.z = __builtin_amdgcn_perm(__float_as_uint(f[5]), __float_as_uint(f[4]), 0x07060302u);
+  r.w = __builtin_amdgcn_perm(__float_as_uint(f[7]), __float_as_uint(f[6]), 0x07060302u);
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// Block = 4 waves = up to PIECE keys of one (entry, head) against up to 16 of its queries, on the matrix pipe; a wave takes 64 keys at a time.
+//   scores   S^T[key][query] = K[key][d] . Q^T[d][query] by v_mfma_f32_16x16x32_bf16: codes are exact in bf16, so the products are exact and the sums
+//            fp32.  A lane loads 16 contiguous codes of a key (one load of the wave: 16 whole keys); tile t of a group of 32 keys holds the keys
+//            8 (row >> 2) + 4 t + (row & 3), so that the eight scores a lane gets of its query are those of the consecutive keys 8 g .. 8 g + 7
+//            (g = lane >> 4), which is the B operand of the second product without any movement.
+//   output   O^T[d][query] += V^T[d][key] . P^T[key][query]: the value codes pass through LDS, the transposing read (ds_read_b64_tr_b8) returns the
+//            codes of eight keys for one d.  The weights carry the values' scales and are split into bf16 high and low parts (16 bits, two products).
+// The running maximum of a query is shared by its four lanes (two exchanges per 64 keys); scales and bias of the piece wait in LDS, where a key
+// without a part has bias -infinity and scales of zero.
+// A value-per-lane form without the matrix pipe was bound by VALU issue at four queries (127 us at 4 x 4 queries x 16 heads x 40000 keys).
+constexpr int VPITCH = 80;            // bytes per key of the value tile: the 16-byte rows of a transposing read fall into different banks
+__global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
+  __shared__ __attribute__((aligned(16))) float s_ks[PIECE], s_vs[PIECE], s_b[PIECE];
+  __shared__ __attribute__((aligned(16))) char s_v[4][64 * VPITCH];       // value tiles, then the waves' sums
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ uint32_t s_any;           // chunks of 64 keys that hold a visible one
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 15, g = lane >> 4;
   const int gc = blockIdx.x % p.gchunks, eh = blockIdx.x / p.gchunks;
   const int h = eh % p.H, e = eh / p.H;
   const int piece = blockIdx.y, k0 = piece * PIECE;
   const int n = attn_q8_keys(p, e);
   if (k0 >= n && piece > 0) return;
-  const int end = min(n - k0, PIECE);
-  const int g0 = gc * G, ng = min(G, p.G - g0);
-  const long base = (long)e * p.e_rows + (long)h * p.h_rows;
+  const int end = min(n - k0, PIECE), nch = (end + 63) >> 6;
+  const int g0 = gc * 16, ng = min(16, p.G - g0);
+  const long base = (long)e * p.e_rows + (long)h * p.h_rows + k0;
   const i8 *kq = p.kq + base * 64, *vq = p.vq + base * 64;
   const float *ks = p.ks + base, *vs = p.vs + base;
   const float* bias = nullptr;
-  if (p.bias) bias = p.bias + (long)h * p.bias_ld + (p.pos_dev ? p.bias_maxlen - 1 - *p.pos_dev : 0);
-  // visible keys of the piece, one bit each
-  for (int r = 0; r < PIECE / 256; ++r) {
-    const int k = r * 256 + tid;
+  if (p.bias) bias = p.bias + (long)h * p.bias_ld + k0 + (p.pos_dev ? p.bias_maxlen - 1 - *p.pos_dev : 0);
+
+  if (tid == 0) s_any = 0;
+  __syncthreads();
+  bf16x8 qf[2];
+  {
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (qi < ng) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (long)(e * p.G + g0 + qi) * p.q_bs + h * 64 + g * 16);
+      a = src[0]; b = src[1];
+    }
+    qf[0] = __builtin_bit_cast(bf16x8, a); qf[1] = __builtin_bit_cast(bf16x8, b);
+  }
+  for (int r = 0; r < nch; r += 4) {
+    const int k = r * 64 + tid;
     bool see = k < end;
     if (see && p.mask) see = p.mask[(long)e * p.mask_ld + k0 + k] != 0;
-    const unsigned long long b = __ballot(see);
-    if (lane == 0) s_bits[r * 4 + wave] = b;
-  }
-  float qv[G][16];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const long qr = (long)(e * p.G + g0 + (g < ng ? g : 0)) * p.q_bs + h * 64 + c * 16;
-    ld8(p.q + qr, qv[g]); ld8(p.q + qr + 8, qv[g] + 8);
-  }
-  __syncthreads();
-  float m[G], l[G], acc[G][16];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    m[g] = -INFINITY; l[g] = 0.f;
-#pragma unroll
-    for (int d = 0; d < 16; ++d) acc[g][d] = 0.f;
-  }
-  for (int ch = wave; ch < PIECE / 64; ch += 4) {
-    const unsigned long long bits = s_bits[ch];
-    if (bits == 0) continue;
-    uint4 kr[4], vr[4];
-    float sk[4], sv[4], bz[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int k = ch * 64 + j * 16 + slot;
-      k = k0 + (k < end ? k : end - 1);
-      kr[j] = *reinterpret_cast<const uint4*>(kq + (long)k * 64 + c * 16);
-      vr[j] = *reinterpret_cast<const uint4*>(vq + (long)k * 64 + c * 16);
-      sk[j] = ks[k]; sv[j] = vs[k];
-      bz[j] = bias ? bias[k] : 0.f;
-    }
-    float sc[G][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[16];
-      q8_unpack4(kr[j].x, f); q8_unpack4(kr[j].y, f + 4); q8_unpack4(kr[j].z, f + 8); q8_unpack4(kr[j].w, f + 12);
-      const bool see = (bits >> (j * 16 + slot)) & 1ull;
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float d = 0.f;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) d = fmaf(qv[g][t], f[t], d);
-        d = dpp_add<0xB1>(d);                       // the four lanes of a key: quad permutes [1,0,3,2] and [2,3,0,1]
-        d = dpp_add<0x4E>(d);
-        sc[g][j] = see ? d * sk[j] * p.scale + bz[j] : -INFINITY;
-      }
-      if (!see) sv[j] = 0.f;                        // what a masked key holds never reaches the sums
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float mn = fmaxf(fmaxf(fmaxf(sc[g][0], sc[g][1]), fmaxf(sc[g][2], sc[g][3])), m[g]);
-      const float a = rescale(m[g], mn);
-      m[g] = mn;
-      l[g] *= a;
-#pragma unroll
-      for (int d = 0; d < 16; ++d) acc[g][d] *= a;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float w = sc[g][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sc[g][j] - mn) * LOG2E);
-        l[g] += w;
-        sc[g][j] = w * sv[j];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[16];
-      q8_unpack4(vr[j].x, f); q8_unpack4(vr[j].y, f + 4); q8_unpack4(vr[j].z, f + 8); q8_unpack4(vr[j].w, f + 12);
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int d = 0; d < 16; ++d) acc[g][d] = fmaf(sc[g][j], f[d], acc[g][d]);
-    }
-  }
-  // the 16 key slots of the wave, then the waves
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    float M = m[g];
-#pragma unroll
-    for (int o = 4; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    const float a = rescale(m[g], M);
-    float L = l[g] * a;
-    L = dpp_add<0x128>(L); L = dpp_add<0x124>(L);   // row_ror 8 and 4 keep lane & 3
-    L += __shfl_xor(L, 16, 64); L += __shfl_xor(L, 32, 64);
-#pragma unroll
-    for (int d = 0; d < 16; ++d) {
-      float s = acc[g][d] * a;
-      s = dpp_add<0x128>(s); s = dpp_add<0x124>(s);
-      s += __shfl_xor(s, 16, 64); s += __shfl_xor(s, 32, 64);
-      if (slot == 0) s_o[g][wave][c * 16 + d] = s;
-    }
-    if (lane == 0) { s_m[g][wave] = M; s_l[g][wave] = L; }
+    float b = -INFINITY;
+    if (see) b = bias ? bias[k] : 0.f;
+    see = !(b == -INFINITY);
+    const float sk = see ? ks[k] * p.scale : 0.f, sv = see ? vs[k] : 0.f;
+    if (k < PIECE) { s_ks[k] = sk; s_vs[k] = sv; s_b[k] = b; }
+    const unsigned long long any = __ballot(see);
+    if (lane == 0 && any != 0) atomicOr(&s_any, 1u << (r + wave));
   }
   __syncthreads();
-  bool none = false;                                 // a query of this block without a visible key (single-piece form only)
+
+  f32x4 acc[4];
 #pragma unroll
-  for (int g = 0; g < G; ++g) none |= s_l[g][0] + s_l[g][1] + s_l[g][2] + s_l[g][3] == 0.f;
-  float mean = 0.f;
-  if (none && p.np == 1) mean = attn_q8_mean(vq, vs, n, s_red);
+  for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  char* const vt = s_v[wave];
+  // (requesting the next chunk's codes ahead was slower: it costs a quarter of the waves, and these hide the loads of each other)
+  for (uint32_t rest = __builtin_amdgcn_readfirstlane(s_any) & (0x11111111u << wave); rest; rest &= rest - 1) {
+    const int ch = __builtin_ctz(rest);
+    u32x4 kr[4], vr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {       // keys behind the end load the last one: their scales are zero
+      const int kk = ch * 64 + (i >> 1) * 32 + 8 * (qi >> 2) + 4 * (i & 1) + (qi & 3), kv = ch * 64 + i * 16 + (lane >> 2);
+      kr[i] = *reinterpret_cast<const u32x4*>(kq + (uint32_t)(min(kk, end - 1) * 64 + g * 16));
+      vr[i] = *reinterpret_cast<const u32x4*>(vq + (uint32_t)(min(kv, end - 1) * 64 + (lane & 3) * 16));
+    }
+    float sc[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(kr[i][0], kr[i][1]), qf[0], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(kr[i][2], kr[i][3]), qf[1], d, 0, 0, 0);
+      const int at = ch * 64 + (i >> 1) * 32 + 8 * g + 4 * (i & 1);
+      const float4 sk = *reinterpret_cast<const float4*>(s_ks + at), b = *reinterpret_cast<const float4*>(s_b + at);
+      const float z0 = fmaf(d[0], sk.x, b.x);
+      const float z1 = fmaf(d[1], sk.y, b.y);
+      const float z2 = fmaf(d[2], sk.z, b.z);
+      const float z3 = fmaf(d[3], sk.w, b.w);
+      sc[4 * i + 0] = b.x == -INFINITY ? b.x : z0; sc[4 * i + 1] = b.y == -INFINITY ? b.y : z1;       // whatever a query holds
+      sc[4 * i + 2] = b.z == -INFINITY ? b.z : z2; sc[4 * i + 3] = b.w == -INFINITY ? b.w : z3;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(vt + (i * 16 + (lane >> 2)) * VPITCH + (lane & 3) * 16) = vr[i];
+    float mn = sc[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mn = fmaxf(mn, sc[i]);
+    mn = fmaxf(mn, __shfl_xor(mn, 16, 64));
+    mn = fmaxf(mn, __shfl_xor(mn, 32, 64));
+    mn = fmaxf(mn, m);
+    const float a = rescale(m, mn);
+    m = mn;
+    l *= a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= a;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      float w[8];
+      const float4 v0 = *reinterpret_cast<const float4*>(s_vs + ch * 64 + kb * 32 + 8 * g), v1 = *reinterpret_cast<const float4*>(s_vs + ch * 64 + kb * 32 + 8 * g + 4);
+      const float sv[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float z = sc[kb * 8 + i];
+        const float x = z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((z - m) * LOG2E);
+        l += x;
+        w[i] = x * sv[i];
+      }
+      uint4 hi, lo;
+      hi = pack8(w);
+      float hf[8];
+      unpack8(hi, hf);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] -= hf[i];
+      lo = pack8(w);
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        typedef __attribute__((ext_vector_type(2))) int i32x2;
+        const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((V2S_LDS i32x2*)(vt + (kb * 32 + 8 * g + (qi >> 1)) * VPITCH + dt * 16 + (qi & 1) * 8));
+        const bf16x8 vf = codes_bf16((uint32_t)c[0], (uint32_t)c[1]);
+        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, hi), acc[dt], 0, 0, 0);
+        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, lo), acc[dt], 0, 0, 0);
+      }
+    }
+  }
+  // join the waves: [query][64] sums per wave in the wave's own tile
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  float* const so = reinterpret_cast<float*>(vt);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<f32x4*>(so + qi * 64 + dt * 16 + g * 4) = acc[dt];
+  if (g == 0) { s_m[wave][qi] = m; s_l[wave][qi] = l; }
+  __syncthreads();
+  if (p.np == 1) {
+    bool none = false;                  // a query of this block without a visible key
+    for (int q = 0; q < ng; ++q) none |= s_l[0][q] + s_l[1][q] + s_l[2][q] + s_l[3][q] == 0.f;
+    if (none) {                         // the same for every thread of the block
+      const float mean = attn_q8_mean(vq, vs, n, s_b);
+      for (int t = tid; t < ng * 64; t += 256) {
+        const int q = t >> 6;
+        if (s_l[0][q] + s_l[1][q] + s_l[2][q] + s_l[3][q] == 0.f) p.o[((long)e * p.G + g0 + q) * p.o_bs + h * 64 + (t & 63)] = f2bf(mean);
+      }
+    }
+  }
   for (int t = tid; t < ng * 64; t += 256) {
-    const int g = t >> 6, d = t & 63;
-    float M = s_m[g][0];
-    for (int w = 1; w < 4; ++w) M = fmaxf(M, s_m[g][w]);
+    const int q = t >> 6, d = t & 63;
+    const float M = fmaxf(fmaxf(s_m[0][q], s_m[1][q]), fmaxf(s_m[2][q], s_m[3][q]));
     float L = 0.f, O = 0.f;
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float a = rescale(s_m[g][w], M);
-      L += s_l[g][w] * a; O += s_o[g][w][d] * a;
+      const float a = rescale(s_m[w][q], M);
+      L += s_l[w][q] * a; O += reinterpret_cast<const float*>(s_v[w])[q * 64 + d] * a;
     }
-    const long b = (long)e * p.G + g0 + g;
+    const long b = (long)e * p.G + g0 + q;
     if (p.np == 1) {
-      p.o[b * p.o_bs + h * 64 + d] = f2bf(L == 0.f ? mean : O / L);
+      if (L != 0.f) p.o[b * p.o_bs + h * 64 + d] = f2bf(O / L);
     } else {
       float* w = p.ws + ((b * p.H + h) * p.np + piece) * 66;
       w[d] = O;
@@ -411,26 +445,147 @@ __global__ __launch_bounds__(256) void attn_q8_kernel(const AttnQ8 p) {
   }
 }
 
+// One query per entry: block = 4 waves = up to PIECE keys of one (entry, head).  lane = (key slot lane >> 2, 16 dimensions lane & 3): a load of the wave is
+// 16 whole keys (1 KiB).  On the matrix pipe fifteen of the sixteen query columns would be empty while every lane still converts the codes and
+// computes a softmax, so the fp32 pipe needs a third fewer instructions here.
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int W1 = 4;
+__global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {
+  __shared__ float s_m[W1], s_l[W1], s_o[W1][64], s_red[256];
+  __shared__ unsigned long long s_bits[(PIECE / 64 + W1 - 1) / W1 * W1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), slot = lane >> 2, c = lane & 3;
+  const int h = blockIdx.x % p.H, e = blockIdx.x / p.H;
+  const int piece = blockIdx.y, k0 = piece * PIECE;
+  const int n = attn_q8_keys(p, e);
+  if (k0 >= n && piece > 0) return;
+  const int end = min(n - k0, PIECE), nch = (end + 63) >> 6;
+  const long base = (long)e * p.e_rows + (long)h * p.h_rows + k0;
+  const i8 *kq = p.kq + base * 64, *vq = p.vq + base * 64;
+  const float *ks = p.ks + base, *vs = p.vs + base;
+  const float* bias = nullptr;
+  if (p.bias) bias = p.bias + (long)h * p.bias_ld + k0 + (p.pos_dev ? p.bias_maxlen - 1 - *p.pos_dev : 0);
+  float qv[16];
+  const long qr = (long)e * p.q_bs + h * 64 + c * 16;
+  ld8(p.q + qr, qv); ld8(p.q + qr + 8, qv + 8);
+  if (p.mask) {                                      // visible keys, one bit each
+    for (int r = 0; r < nch; r += W1) {
+      const int k = r * 64 + tid;
+      const unsigned long long b = __ballot(k < end && p.mask[(long)e * p.mask_ld + k0 + min(k, end - 1)] != 0);
+      if (lane == 0) s_bits[r + wave] = b;
+    }
+    __syncthreads();
+  }
+  float m = -INFINITY, l = 0.f, acc[16];
+#pragma unroll
+  for (int d = 0; d < 16; ++d) acc[d] = 0.f;
+  for (int ch = wave; ch < nch; ch += W1) {
+    const int left = end - ch * 64;
+    unsigned long long bits = left >= 64 ? ~0ull : (1ull << left) - 1;
+    if (p.mask) bits = s_bits[ch];
+    if (__builtin_amdgcn_readfirstlane((uint32_t)bits | (uint32_t)(bits >> 32)) == 0) continue;
+    u32x4 kr[4], vr[4];
+    float sk[4], sv[4], bz[4], sc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t k = (uint32_t)min(ch * 64 + j * 16 + slot, end - 1);
+      kr[j] = *reinterpret_cast<const u32x4*>(kq + k * 64 + c * 16);
+      vr[j] = *reinterpret_cast<const u32x4*>(vq + k * 64 + c * 16);
+      sk[j] = ks[k]; sv[j] = vs[k];
+      bz[j] = bias ? bias[k] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float d = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f[4];
+        q8_unpack4(kr[j][i], f);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) d = fmaf(qv[4 * i + t], f[t], d);
+      }
+      d = dpp_add<0xB1>(d);                          // the four lanes of a key: quad permutes [1,0,3,2] and [2,3,0,1]
+      d = dpp_add<0x4E>(d);
+      const bool see = (bits >> (j * 16 + slot)) & 1ull && !(bz[j] == -INFINITY);
+      const float z = fmaf(d, sk[j] * p.scale, bz[j]);
+      sc[j] = see ? z : -INFINITY;
+      sv[j] = see ? sv[j] : 0.f;                     // what a masked key holds never reaches the sums
+    }
+    const float mn = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), m);
+    const float a = rescale(m, mn);
+    m = mn;
+    l *= a;
+#pragma unroll
+    for (int d = 0; d < 16; ++d) acc[d] *= a;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float w = sc[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sc[j] - mn) * LOG2E);
+      l += w;
+      const float x = w * sv[j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f[4];
+        q8_unpack4(vr[j][i], f);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[4 * i + t] = fmaf(x, f[t], acc[4 * i + t]);
+      }
+    }
+  }
+  // the 16 key slots of the wave, then the waves
+  float M = m;
+#pragma unroll
+  for (int o = 4; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float a = rescale(m, M);
+  float L = l * a;
+  L = dpp_add<0x128>(L); L = dpp_add<0x124>(L);      // row_ror 8 and 4 keep lane & 3
+  L += __shfl_xor(L, 16, 64); L += __shfl_xor(L, 32, 64);
+#pragma unroll
+  for (int d = 0; d < 16; ++d) {
+    float x = acc[d] * a;
+    x = dpp_add<0x128>(x); x = dpp_add<0x124>(x);
+    x += __shfl_xor(x, 16, 64); x += __shfl_xor(x, 32, 64);
+    if (slot == 0) s_o[wave][c * 16 + d] = x;
+  }
+  if (lane == 0) { s_m[wave] = M; s_l[wave] = L; }
+  __syncthreads();
+  M = s_m[0];
+  for (int w = 1; w < W1; ++w) M = fmaxf(M, s_m[w]);
+  L = 0.f;
+  float O = 0.f;
+  for (int w = 0; w < W1; ++w) { const float x = rescale(s_m[w], M); L += s_l[w] * x; O += s_o[w][lane] * x; }
+  float r = O / L;
+  if (L == 0.f && p.np == 1) r = attn_q8_mean(vq, vs, n, s_red);       // the same for every thread of the block
+  if (wave != 0) return;
+  if (p.np == 1) {
+    p.o[(long)e * p.o_bs + h * 64 + lane] = f2bf(r);
+  } else {
+    float* w = p.ws + ((long)blockIdx.x * p.np + piece) * 66;
+    w[lane] = O;
+    if (lane == 0) { w[64] = M; w[65] = L; }
+  }
+}
+
 // joins the pieces of one (query, head): 4 waves take the pieces in turn
 __global__ __launch_bounds__(256) void attn_q8_join_kernel(const AttnQ8 p) {
-  __shared__ float s_m[4], s_l[4], s_o[4][64], s_red[256];
+  __shared__ float s_l[4], s_o[4][64], s_red[256];
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, e = b / p.G;
   const int d = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = attn_q8_keys(p, e), np = (n + PIECE - 1) / PIECE;
   const float* w = p.ws + (long)blockIdx.x * p.np * 66;
-  float M = -INFINITY, L = 0.f, O = 0.f;
+  float M = -INFINITY, L = 0.f, O = 0.f;              // the maximum first: the pieces' sums can then be read without waiting for each other
+  for (int i = d; i < np; i += 64) M = fmaxf(M, w[i * 66 + 64]);
+  M = wave_max(M);
+#pragma unroll 8
   for (int i = wave; i < np; i += 4) {
-    const float mi = w[i * 66 + 64], li = w[i * 66 + 65], oi = w[i * 66 + d];
-    const float mn = fmaxf(M, mi), a = rescale(M, mn), c = rescale(mi, mn);
-    L = L * a + li * c; O = O * a + oi * c;
-    M = mn;
+    const float a = rescale(w[i * 66 + 64], M);
+    L += w[i * 66 + 65] * a; O += w[i * 66 + d] * a;
   }
   s_o[wave][d] = O;
-  if (d == 0) { s_m[wave] = M; s_l[wave] = L; }
+  if (d == 0) s_l[wave] = L;
   __syncthreads();
-  M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  L = 0.f; O = 0.f;
-  for (int i = 0; i < 4; ++i) { const float a = rescale(s_m[i], M); L += s_l[i] * a; O += s_o[i][d] * a; }
+  L = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  O = s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d];
   float r = O / L;
   if (L == 0.f) {                                    // the same for every thread of the block
     const long base = (long)e * p.e_rows + (long)h * p.h_rows;
@@ -568,14 +723,12 @@ extern "C" int v2s_decode_attn_q8(const v2s_decode_attn_q8_args* a, void* stream
   const int64_t need = v2s_decode_attn_q8_workspace_floats(a->B, c.heads, a->Nk) * 4;
   V2S_CHECK(need == 0 || (a->workspace && a->workspace_bytes >= need && aligned(a->workspace, 4)), V2S_ERR_ARG,
             "v2s_decode_attn_q8: %lld bytes of workspace needed for %d keys, got %lld", (long long)need, a->Nk, (long long)(a->workspace ? a->workspace_bytes : 0));
-  const int per = G >= 4 ? 4 : (G >= 2 ? 2 : 1);
-  p.gchunks = (G + per - 1) / per;
+  p.gchunks = (G + 15) / 16;
   V2S_CHECK((int64_t)c.entries * c.heads * p.gchunks <= 0x7fffffff && p.np <= 65535, V2S_ERR_SHAPE, "v2s_decode_attn_q8: too many rows or keys for one launch");
   const dim3 grid((unsigned)(c.entries * c.heads * p.gchunks), (unsigned)p.np);
   hipStream_t s = (hipStream_t)stream;
-  if (per == 4) hipLaunchKernelGGL(attn_q8_kernel<4>, grid, dim3(256), 0, s, p);
-  else if (per == 2) hipLaunchKernelGGL(attn_q8_kernel<2>, grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL(attn_q8_kernel<1>, grid, dim3(256), 0, s, p);
+  if (G == 1) hipLaunchKernelGGL(attn_q8_one_kernel, grid, dim3(W1 * 64), 0, s, p);
+  else hipLaunchKernelGGL(attn_q8_kernel, grid, dim3(256), 0, s, p);
   V2S_LAUNCH_CHECK();
   if (p.np > 1) {
     hipLaunchKernelGGL(attn_q8_join_kernel, dim3((unsigned)(a->B * c.heads)), dim3(256), 0, s, p);

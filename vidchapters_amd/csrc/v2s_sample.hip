@@ -41,18 +41,28 @@ __device__ __forceinline__ float key_logit(u64 key) {
   const uint32_t asc = ~(uint32_t)(key >> 32);
   return __uint_as_float((asc >> 31) ? asc ^ 0x80000000u : ~asc);
 }
-// 2^t for t <= 0: t = k + f, |f| <= 1/2, and the series of 2^f to the 13th power (its remainder is below 2^-57)
-__device__ __forceinline__ double exp2_neg(double t) {
+// 2^r for |r| <= 1 by the series of exp(r ln 2), 2^46 * 2^t for t <= 0 by a table of 2^(i / 64) and the first terms of the same series: t = n / 64 + r,
+// |r| <= 1 / 128 (remainder below 2^-54).  Sixteen instructions in 64 bits; the series alone took 25, the library's exp over 40.
+constexpr double LN2 = 0.69314718055994530942;
+__device__ double exp2_series(double r) {
+  const double x = r * LN2;
+  double s = 1.0;
+#pragma unroll 1
+  for (int i = 19; i > 0; --i) s = fma(s * (1.0 / i), x, 1.0);
+  return s;
+}
+__device__ __forceinline__ double exp2_mass(double t, const double* tab) {
+  constexpr double MAGIC = 105553116266496.0;      // 1.5 * 2^46: adding it leaves multiples of 1 / 64
+  constexpr double C1 = LN2, C2 = C1 * LN2 / 2, C3 = C2 * LN2 / 3, C4 = C3 * LN2 / 4, C5 = C4 * LN2 / 5;
   t = fmax(t, -100.0);
-  const double k = rint(t), x = (t - k) * 0.69314718055994530942;
-  double s = 1.0 / 6227020800.0;
-  s = fma(s, x, 1.0 / 479001600.0); s = fma(s, x, 1.0 / 39916800.0); s = fma(s, x, 1.0 / 3628800.0); s = fma(s, x, 1.0 / 362880.0);
-  s = fma(s, x, 1.0 / 40320.0); s = fma(s, x, 1.0 / 5040.0); s = fma(s, x, 1.0 / 720.0); s = fma(s, x, 1.0 / 120.0); s = fma(s, x, 1.0 / 24.0);
-  s = fma(s, x, 1.0 / 6.0); s = fma(s, x, 0.5); s = fma(s, x, 1.0); s = fma(s, x, 1.0);
-  return ldexp(s, (int)k);
+  const double t2 = t + MAGIC;
+  const int n = __double2loint(t2);
+  const double r = t - (t2 - MAGIC);
+  const double s = fma(fma(fma(fma(fma(C5, r, C4), r, C3), r, C2), r, C1), r, 1.0);
+  return tab[n & 63] * s * __hiloint2double(((n >> 6) + 46 + 1023) << 20, 0);
 }
 // round to nearest: 2^46 w < 2^52, so the sum holds it in its low bits
-__device__ __forceinline__ u64 mass_of(double w) { return (u64)__double_as_longlong(w * ONE + 4503599627370496.0) & 0xfffffffffffffull; }
+__device__ __forceinline__ u64 mass_of(double w46) { return (u64)__double_as_longlong(w46 + 4503599627370496.0) & 0xfffffffffffffull; }
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += (u64)__shfl_xor((long long)v, o, 64);
@@ -92,12 +102,16 @@ __device__ __forceinline__ void load4(const bf16_t* z, int i0, int V, int vec, f
   }
 }
 
+__device__ __forceinline__ float load1(const float* z) { return *z; }
+__device__ __forceinline__ float load1(const bf16_t* z) { return bf2f(*z); }
+
 // ROW: the row is held in LDS (zs), else every pass reads it again
 template <typename T, bool ROW>
 __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   extern __shared__ __attribute__((aligned(16))) float zs[];
   __shared__ u64 s_mass[NBIN];
   __shared__ u64 s_key[CAP], s_w[CAP];
+  __shared__ double s_tab[64];
   __shared__ u64 s_red[NT / 64], s_thr, s_base;
   __shared__ float s_max[NT / 64];
   __shared__ int s_n, s_bin, s_nan;
@@ -122,6 +136,10 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
       fetch(j, z);
     }
   };
+  auto one = [&](int idx) -> float {
+    if constexpr (ROW) return zs[idx];
+    else return idx == ban ? -INFINITY : load1(z0 + idx) + 0.0f;
+  };
   auto each = [&](auto f) {                 // f(index, logit) for the tokens of this thread, in index order
 #pragma unroll 1
     for (int j = 0; j < nj; ++j) {
@@ -134,6 +152,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
 
   int nan_at = V;
   float tmax = -INFINITY;                   // maximum of this thread's tokens
+  if (tid < 64) s_tab[tid] = exp2_series(tid / 64.0);
   if constexpr (ROW) {
     float z[ROW_MAX][4];
 #pragma unroll
@@ -184,7 +203,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
 
   auto far_of = [&](float z) { return z == zmax ? 0.f : (zmax - z) * p.bin_scale; };      // in bins
   auto bin_of = [&](float z) { return (int)fminf(far_of(z), (float)(NBIN - 1)); };
-  auto weight = [&](float z) -> double { return z == zmax ? 1.0 : exp2_neg(((double)z - (double)zmax) * p.exp2_scale); };
+  const double dmax = (double)zmax, min_w = p.min_p * ONE;
+  auto weight = [&](float z) -> double { return exp2_mass(z == zmax ? 0.0 : ((double)z - dmax) * p.exp2_scale, s_tab); };      // 2^46 w
   auto log_prob = [&](float z, u64 total) { return (float)((z == zmax ? 0.0 : ((double)z - (double)zmax) * p.inv_temp) - log((double)total / ONE)); };
 
   // bin of the boundary: the first one at which the running sum (of counts or masses) reaches the goal; s_base = the sum before it
@@ -242,7 +262,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
         if (tid < n)
           for (int i = 0; i < n; ++i) { const u64 x = s_w[i]; total += x; pre += s_key[i] < key ? x : 0; }
         __syncthreads();
-        const bool keep = in && w > 0 && wd >= p.min_p && (p.top_p >= 1.0 || (double)pre < p.top_p * (double)total);
+        const bool keep = in && w > 0 && wd >= min_w && (p.top_p >= 1.0 || (double)pre < p.top_p * (double)total);
         if (tid < n) s_w[tid] = keep ? w : 0;
         __syncthreads();
         if (keep) {
@@ -296,50 +316,63 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     return lo;
   };
 
-  u64 thr = ~0ull;                          // order key of the last token that top-k and top-p keep
+  // the last token that top-k and top-p keep, and whether a token is not behind it
+  float thr_z = -INFINITY;
+  int thr_i = V;
+  auto upto = [&](float z, int idx) { return z > thr_z || (z == thr_z && idx <= thr_i); };
+  auto set_thr = [&](u64 key) { thr_z = key_logit(key); thr_i = (int)(uint32_t)key; };
   if (cut_k) {
     each([&](int, float z) { const int b = bin_of(z); if (b < NBIN - 1) atomicAdd(&s_cnt[b], 1u); });
     __syncthreads();
     const u64 k = (u64)p.top_k;
     find_bin([&](int b) { return (u64)s_cnt[b]; }, [&](u64 s) { return s >= k; });
     if (s_bin < NBIN - 1)                   // otherwise every token with any mass is among the first k
-      thr = resolve([](float, int) { return true; }, [](float) { return (u64)1; }, [&](u64 s) { return s >= k; });
+      set_thr(resolve([](float, int) { return true; }, [](float) { return (u64)1; }, [&](u64 s) { return s >= k; }));
     __syncthreads();
     clear();
   }
   if (p.top_p < 1.0) {
-    const u64 kt = thr;
     u64 total = 0;
     each([&](int idx, float z) {
       const int b = bin_of(z);
-      if (b < NBIN - 1 && order_key(z, idx) <= kt) { const u64 m = mass_of(weight(z)); total += m; atomicAdd(&s_mass[b], m); }
+      if (b < NBIN - 1 && upto(z, idx)) { const u64 m = mass_of(weight(z)); total += m; atomicAdd(&s_mass[b], m); }
     });
     total = block_sum64(total, s_red, tid);
     const double goal = p.top_p * (double)total;
     const auto reached = [&](u64 s) { return (double)s >= goal; };
     find_bin([&](int b) { return s_mass[b]; }, reached);
-    thr = resolve([&](float z, int idx) { return order_key(z, idx) <= kt; }, [&](float z) { return mass_of(weight(z)); }, reached);
+    set_thr(resolve(upto, [&](float z) { return mass_of(weight(z)); }, reached));
     __syncthreads();
+    clear();
   }
 
-  // kept mass of each segment of 256 consecutive tokens (one wave of one pass); segments in index order are (pass, wave)
-  u64* seg = s_mass;                        // [nj][16] <= 512
-  const float thr_z = thr == ~0ull ? -INFINITY : key_logit(thr);
-  const int thr_i = thr == ~0ull ? V : (int)(uint32_t)thr;
   auto kept = [&](float z, int idx) -> u64 {
-    if (idx >= V || z < thr_z || (z == thr_z && idx > thr_i)) return 0;
+    if (idx >= V || !upto(z, idx)) return 0;
     const double w = weight(z);
-    return w >= p.min_p ? mass_of(w) : 0;
+    return w >= min_w ? mass_of(w) : 0;
   };
+  // Kept mass of each segment of 256 consecutive tokens (one wave of one pass), segments in index order: [nj][16] <= 512.  The comparison runs over all
+  // tokens, the exponential only over those that passed it (a thread walks its own, eight passes at a time), the masses of one pass of a thread go to
+  // the segment at once.
+  u64* const seg = s_mass;
 #pragma unroll 1
-  for (int j = 0; j < nj; ++j) {
-    float z[4];
-    get(j, z);
-    u64 own = 0;
+  for (int j0 = 0; j0 < nj; j0 += 8) {
+    uint32_t pass = 0;
+#pragma unroll 1
+    for (int j = j0; j < min(nj, j0 + 8); ++j) {
+      float z[4];
+      get(j, z);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) own += kept(z[i], j * STEP + tid * 4 + i);
-    own = wave_sum64(own);
-    if (lane == 0) seg[j * (NT / 64) + wave] = own;
+      for (int i = 0; i < 4; ++i) { const int idx = j * STEP + tid * 4 + i; pass |= idx < V && upto(z[i], idx) ? 1u << ((j - j0) * 4 + i) : 0u; }
+    }
+    u64 own = 0;
+    while (pass) {
+      const int b = __builtin_ctz(pass), j = j0 + (b >> 2);
+      pass &= pass - 1;
+      const double w = weight(one(j * STEP + tid * 4 + (b & 3)));
+      own += w >= min_w ? mass_of(w) : 0;
+      if (!pass || j0 + (__builtin_ctz(pass) >> 2) != j) { atomicAdd(&seg[j * (NT / 64) + wave], own); own = 0; }
+    }
   }
   __syncthreads();
   // the segment in which the running mass passes u * total (one wave: up to 512 segments, eight per lane), else the last one with any mass
