@@ -23,69 +23,97 @@ struct GemmQ8 {
   int tilesM, tilesN;
 };
 
-// scales and biases of W consecutive columns of a lane (columns behind N: zero)
-template <int W> struct Cols { float s[W], b[W]; };
-template <int W> __device__ __forceinline__ Cols<W> cols(const GemmQ8& p, int n) {
-  Cols<W> c;
-#pragma unroll
-  for (int r = 0; r < W; ++r) {
-    c.s[r] = n + r < p.N ? p.sB[n + r] : 0.f;
-    c.b[r] = p.bias && n + r < p.N ? p.bias[n + r] : 0.f;
-  }
-  return c;
-}
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 template <int W> struct Raw;                                              // W bf16 values as loaded and stored
 template <> struct Raw<4> { typedef u32x2 T; };
 template <> struct Raw<8> { typedef u32x4 T; };
-// epilogue and store of W columns n .. n + W - 1 of row m; v = alpha * sA[m] * sum; res = the residual there (all of them inside N)
-template <int W> __device__ __forceinline__ void finish(const GemmQ8& p, float (&v)[W], const Cols<W>& c, const typename Raw<W>::T& res, int m, int n) {
+// scales and biases of W consecutive columns of a lane (columns behind N take the last one's: they are not stored)
+template <int W> struct Cols { float s[W], b[W]; };
+template <int W> __device__ __forceinline__ Cols<W> cols(const GemmQ8& p, int n) {
+  Cols<W> c;
 #pragma unroll
-  for (int r = 0; r < W; ++r) v[r] = v[r] * c.s[r] + c.b[r];
-  if (p.act == V2S_ACT_RELU) {
+  for (int r = 0; r < W; ++r) c.s[r] = p.sB[min(n + r, p.N - 1)];
 #pragma unroll
-    for (int r = 0; r < W; ++r) v[r] = v[r] < 0.f ? 0.f : v[r];           // keeps NaN
-  } else if (p.act == V2S_ACT_GELU) {
-#pragma unroll 1
-    for (int r = 0; r < W; ++r) v[r] = gelu_f(v[r]);
+  for (int r = 0; r < W; ++r) c.b[r] = 0.f;
+  if (p.bias) {
+#pragma unroll
+    for (int r = 0; r < W; ++r) c.b[r] = p.bias[min(n + r, p.N - 1)];
   }
-  const long at = (long)m * p.ldc + n;
-  if (n + W <= p.N) {
-    if (p.residual) {
-#pragma unroll
-      for (int r = 0; r < W / 2; ++r) { v[2 * r] += __uint_as_float(res[r] << 16); v[2 * r + 1] += __uint_as_float(res[r] & 0xffff0000u); }
-    }
-    if (p.c_f32) {
-#pragma unroll
-      for (int r = 0; r < W / 4; ++r) *reinterpret_cast<float4*>((float*)p.C + at + 4 * r) = make_float4(v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]);
-    } else {
-      typename Raw<W>::T o;
-#pragma unroll
-      for (int r = 0; r < W / 2; ++r) o[r] = pack2bf(v[2 * r], v[2 * r + 1]);
-      *reinterpret_cast<typename Raw<W>::T*>((bf16_t*)p.C + at) = o;
-    }
-  } else {
-#pragma unroll 1
-    for (int r = 0; r < W && n + r < p.N; ++r) {
-      float x = v[r];
-      if (p.residual) x += bf2f(p.residual[(long)m * p.ldr + n + r]);
-      if (p.c_f32) ((float*)p.C)[at + r] = x;
-      else ((bf16_t*)p.C)[at + r] = f2bf(x);
-    }
-  }
+  return c;
 }
 template <int W> __device__ __forceinline__ typename Raw<W>::T residual_of(const GemmQ8& p, int m, int n) {
   typename Raw<W>::T z = {};
-  if (p.residual && m < p.M && n + W <= p.N) z = *reinterpret_cast<const typename Raw<W>::T*>(p.residual + (long)m * p.ldr + n);
+  if (m < p.M && n + W <= p.N) z = *reinterpret_cast<const typename Raw<W>::T*>(p.residual + (long)m * p.ldr + n);
   return z;
+}
+// exact-erf GELU without branches: v Phi(v) with erfc(|v| / sqrt 2) = (a1 t + ... + a5 t^5) exp(-v^2 / 2), t = 1 / (1 + p |v| / sqrt 2) (Abramowitz and
+// Stegun 7.1.26, absolute error below 1.5e-7, that is 1.3 fp32 roundings of v); the library's erf is three times as long
+__device__ __forceinline__ float gelu_q8(float v) {
+  const float x = fabsf(v) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+  const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float tail = 0.5f * v * q * __builtin_amdgcn_exp2f(x * x * -1.44269504088896340736f);      // v (1 - Phi(|v|))
+  return v < 0.f ? tail : v - tail;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
+}
+// W values v = alpha * sA[m] * sum with their columns' scales and biases: activation
+template <int W, bool GELU> __device__ __forceinline__ void activate(const GemmQ8& p, float (&v)[W], const Cols<W>& c) {
+#pragma unroll
+  for (int r = 0; r < W; ++r) v[r] = v[r] * c.s[r] + c.b[r];
+  if (GELU && p.act == V2S_ACT_GELU) {
+#pragma unroll
+    for (int r = 0; r < W; ++r) v[r] = gelu_q8(v[r]);
+  }
+  if (p.act == V2S_ACT_RELU) {
+#pragma unroll
+    for (int r = 0; r < W; ++r) v[r] = v[r] < 0.f ? 0.f : v[r];           // keeps NaN
+  }
+}
+template <int W> __device__ __forceinline__ void add_residual(float (&v)[W], const typename Raw<W>::T& res) {
+#pragma unroll
+  for (int r = 0; r < W / 2; ++r) { v[2 * r] += __uint_as_float(res[r] << 16); v[2 * r + 1] += __uint_as_float(res[r] & 0xffff0000u); }
+}
+template <int W> __device__ __forceinline__ typename Raw<W>::T pack(const float (&v)[W]) {
+  typename Raw<W>::T o;
+#pragma unroll
+  for (int r = 0; r < W / 2; ++r) o[r] = pack_bf16(v[2 * r], v[2 * r + 1]);
+  return o;
+}
+// the rest of the epilogue of four columns n .. n + 3 of row m, cut by N
+__device__ __forceinline__ void finish4(const GemmQ8& p, float (&v)[4], const Cols<4>& c, int m, int n) {
+  activate<4, true>(p, v, c);
+  const long at = (long)m * p.ldc + n;
+  if (n + 4 <= p.N) {
+    if (p.residual) add_residual<4>(v, residual_of<4>(p, m, n));
+    if (p.c_f32) *reinterpret_cast<float4*>((float*)p.C + at) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<u32x2*>((bf16_t*)p.C + at) = pack<4>(v);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 3; ++r)
+      if (n + r < p.N) {
+        if (p.residual) v[r] += bf2f(p.residual[(long)m * p.ldr + n + r]);
+        if (p.c_f32) ((float*)p.C)[at + r] = v[r];
+        else ((bf16_t*)p.C)[at + r] = f2bf(v[r]);
+      }
+  }
 }
 
 // ---- tiles -------------------------------------------------------------------------------------------------------------------------------
-// BM x BN tile, 4 waves of (BM / 2) x (BN / 2); K in stages of 64 codes through a ring of three LDS images [BM + BN rows][64 bytes] that the LDS-DMA
-// fills (global_load_lds, 1 KiB = 16 rows per wave and instruction; two stages in flight, counted waits, one barrier per stage).
-// A row's four 16-byte groups are stored at group ^ (((row >> 2) & 1) << 1), which spreads the eight rows that a fragment read serves at once.
-// K need not be a multiple of 64: in the last stage lanes whose group lies behind K load the row's first group again (in bounds), and A's fragments
+// BM x BN tile, WM x WN waves; K in stages of 128 codes (a cache line per row: with 64-byte pieces the L2 served twice the requests and the 8192^3
+// product ran at 1617 TOPS instead of 2363) through two LDS images [BM + BN rows][128 bytes] that the LDS-DMA fills (global_load_lds, 1 KiB = 8 rows
+// per wave and instruction), one barrier per stage, D = 3 steps before its end: by then every fragment of the stage has been read (they run three steps ahead
+// of their products), so its image is free for stage s + 2, and the first reads of stage s + 1 wait under the last products.
+// A row's eight 16-byte groups are stored at group ^ f(row): the sixteen rows of a fragment read fall into different banks.
+// Fragment j of B takes the rows (r >> 2) * 4 NI + 4 j + (r & 3) of the wave's 16 NI, so that a lane ends up with 4 NI consecutive columns of a row and
+// stores them straight from its accumulators: no pass through LDS, no barrier.
+// Blocks are persistent: the first two stages of the next tile are requested before the write-out of the current one and arrive under it; the counted
+// waits let its stores drain under those two stages.
+// K need not be a multiple of 128: in the last stage lanes whose group lies behind K load the row's first group again (in bounds), and A's fragments
 // are zeroed there.
 __device__ __forceinline__ uint32_t lds_off(const void* p) { return (uint32_t)(uintptr_t)(V2S_LDS const char*)p; }
 // one instruction: 16 bytes per lane from base + off to LDS at dst + lane * 16
@@ -94,112 +122,239 @@ __device__ __forceinline__ void dma16(uint32_t off, const void* base, uint32_t d
   asm volatile("s_mov_b32 %[keep], m0\n\ts_mov_b32 m0, %[dst]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[off], %[base]\n\ts_mov_b32 m0, %[keep]"
                : [keep] "=&s"(keep) : [dst] "s"(dst), [base] "s"(base), [off] "v"(off) : "memory");
 }
+// every DMA but the youngest N operations of this wave has landed and its LDS reads are done; then the same for the block
+template <int N> __device__ __forceinline__ void wait_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-template <int BM, int BN>
+template <int BM_, int BN_, int WM_, int WN_, int OCC_>
 struct Tile {
-  static constexpr int DA = BM / 64, DB = BN / 64;          // DMA instructions per wave and stage
-  static constexpr int MI = BM / 32, NI = BN / 32;          // 16 x 16 fragments per wave
-  static constexpr int STG = (BM + BN) * 64, NST = 3;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, OCC = OCC_, BK = 128;      // OCC: blocks per CU
+  static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
+  static constexpr int DA = BM / 8 / WAVES, DB = BN / 8 / WAVES;            // DMA instructions per wave and stage
+  static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;                // 16 x 16 fragments per wave
+  static constexpr int STORES = MI * NI / 2;                                // 16-byte stores per wave of a whole bf16 tile
+  static constexpr int OUT = 16 * NI * 32;                                   // bytes of 16 bf16 rows of a wave
+  static constexpr int STG = (BM + BN) * BK, LDS = 2 * STG + WAVES * OUT + (BM + 2 * BN) * 4;
+  static __device__ __forceinline__ int swzA(int row) { return (row >> 1) & 7; }
+  static __device__ __forceinline__ int swzB(int row) { return ((row >> 1) & 1) | ((row / (NI * 4) & 3) << 1); }
 };
 
-template <int BM, int BN>
-__global__ __launch_bounds__(256, 2) void gemm_q8_tile_kernel(const GemmQ8 p) {
-  using G = Tile<BM, BN>;
-  constexpr int DA = G::DA, DB = G::DB, MI = G::MI, NI = G::NI, STG = G::STG;
+template <class G>
+__global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_tile_kernel(const GemmQ8 p) {
+  constexpr int BM = G::BM, BN = G::BN, BK = G::BK, DA = G::DA, DB = G::DB, MI = G::MI, NI = G::NI, STG = G::STG, DD = DA + DB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int id = xcd_remap(blockIdx.x, p.tilesM * p.tilesN);
-  const int m0 = id / p.tilesN * BM, n0 = id % p.tilesN * BN;
-  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-  const int nst = (p.K + 63) >> 6, krem = p.K - (nst - 1) * 64;
+  float* const s_a = reinterpret_cast<float*>(smem + 2 * STG + G::WAVES * G::OUT);      // scales of the tile's rows, scales and bias of its columns
+  float* const s_b = s_a + BM;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / G::WN * (MI * 16), wn = wave % G::WN * (NI * 16);
+  const int nst = (p.K + BK - 1) / BK, krem = p.K - (nst - 1) * BK;
+  const int ntiles = p.tilesM * p.tilesN, nwg = gridDim.x;
   const uint32_t sbase = lds_off(smem);
-
-  uint32_t oa[DA], ob[DB];
-  const int rl = lane >> 2, gl = (lane & 3) ^ (((rl >> 2) & 1) << 1);       // row within a 1 KiB piece, the group this lane loads
-#pragma unroll
-  for (int i = 0; i < DA; ++i) oa[i] = (uint32_t)min((wave * DA + i) * 16 + rl, p.M - 1 - m0) * (uint32_t)p.lda + gl * 16;
-#pragma unroll
-  for (int i = 0; i < DB; ++i) ob[i] = (uint32_t)min((wave * DB + i) * 16 + rl, p.N - 1 - n0) * (uint32_t)p.ldb + gl * 16;
-  const i8* ga = p.A + (long)m0 * p.lda;
-  const i8* gb = p.B + (long)n0 * p.ldb;
-  auto issue = [&](int s) {
-    const uint32_t slot = sbase + (s % 3) * STG;
-    const uint32_t back = s == nst - 1 && gl * 16 >= krem ? gl * 16 : 0;
-#pragma unroll
-    for (int i = 0; i < DA; ++i) dma16(oa[i] - back, ga + (long)s * 64, slot + (wave * DA + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < DB; ++i) dma16(ob[i] - back, gb + (long)s * 64, slot + BM * 64 + (wave * DB + i) * 1024);
-  };
-  i32x4 acc[MI][NI];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  const int rl = lane >> 3, pos = lane & 7;             // row within a 1 KiB piece, 16-byte position within the row
   const int fr = lane & 15, fg = lane >> 4;
-  const int foff = fr * 64 + ((fg ^ (((fr >> 2) & 1) << 1)) * 16);          // fragment rows start at multiples of 16
+  int aoff[2], boff[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    aoff[k] = (wm + fr) * BK + ((k * 4 + fg) ^ G::swzA(fr)) * 16;
+    const int br = (fr >> 2) * (NI * 4) + (fr & 3);
+    boff[k] = (BM + wn + br) * BK + ((k * 4 + fg) ^ G::swzB(br)) * 16;
+  }
 
+  int m0 = 0, n0 = 0;
+  uint32_t oa[DA], ob[DB];
+  const i8 *ga = nullptr, *gb = nullptr;
+  // tile of this block in round r: blocks of one XCD work on neighbouring tiles, four tile rows deep
+  auto place = [&](int r) {
+    const int id = r * nwg + xcd_remap(blockIdx.x, min(nwg, ntiles - r * nwg));
+    const int per = 4 * p.tilesN, grp = id / per, in = id - grp * per, deep = min(4, p.tilesM - grp * 4);
+    m0 = (grp * 4 + in % deep) * BM;
+    n0 = in / deep * BN;
+#pragma unroll
+    for (int i = 0; i < DA; ++i) {
+      const int row = (wave * DA + i) * 8 + rl;
+      oa[i] = (uint32_t)min(row, p.M - 1 - m0) * (uint32_t)p.lda + (pos ^ G::swzA(row)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+      const int row = (wave * DB + i) * 8 + rl;
+      ob[i] = (uint32_t)min(row, p.N - 1 - n0) * (uint32_t)p.ldb + (pos ^ G::swzB(row)) * 16;
+    }
+    ga = p.A + (long)m0 * p.lda;
+    gb = p.B + (long)n0 * p.ldb;
+  };
+  auto issue = [&](int s) {
+    const uint32_t slot = sbase + (s & 1) * STG;
+    const bool cut = s == nst - 1 && krem < BK;
+#pragma unroll
+    for (int i = 0; i < DA; ++i) {
+      const int g = (pos ^ G::swzA((wave * DA + i) * 8 + rl)) * 16;
+      dma16(cut && g >= krem ? oa[i] - g : oa[i], ga + (long)s * BK, slot + (wave * DA + i) * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+      const int g = (pos ^ G::swzB((wave * DB + i) * 8 + rl)) * 16;
+      dma16(cut && g >= krem ? ob[i] - g : ob[i], gb + (long)s * BK, slot + BM * BK + (wave * DB + i) * 1024);
+    }
+  };
+
+  place(0);
   issue(0);
   if (nst > 1) issue(1);
-  for (int s = 0; s < nst; ++s) {
-    // stage s has landed for this wave (stage s + 1 may be in flight) and its reads of the stage before are done; then the same for the block
-    if (s + 1 < nst) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(DA + DB) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 2 < nst) issue(s + 2);
-    const char* sa = smem + (s % 3) * STG + wm * 64 + foff;
-    const char* sb = smem + (s % 3) * STG + BM * 64 + wn * 64 + foff;
-    i32x4 af[MI], bf[NI];
-#pragma unroll
-    for (int i = 0; i < MI; ++i) af[i] = *reinterpret_cast<const i32x4*>(sa + i * 1024);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) bf[j] = *reinterpret_cast<const i32x4*>(sb + j * 1024);
-    if (s == nst - 1 && krem < 64) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-        if (fg * 16 >= krem) af[i] = i32x4{0, 0, 0, 0};
-    }
+  bool stored = false;                      // at least STORES stores of this wave are younger than the stages 0 and 1
+  for (int r = 0; r * nwg + (int)blockIdx.x < ntiles; ++r) {
+    i32x4 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af[i], acc[i][j], 0, 0, 0);
-  }
-  // write-out in passes of 64 rows (two fragment rows of every wave) through LDS: the accumulators become fp32 with the row's scale on the way in, and
-  // leave as 8 consecutive columns per lane, whole cache lines per row.  A lane keeps its columns, so their scales are loaded once; the residual of a
-  // pass is requested before its values are staged
-  constexpr int PB = BN + 4, CPR = BN / 8, RPI = 256 / CPR, NIT = 64 / RPI;        // pitch (floats), chunks per row, rows per iteration, iterations
-  static_assert(64 * PB * 4 <= G::NST * STG, "a pass fits the ring");
-  float* cs = reinterpret_cast<float*>(smem);
-  const int n = n0 + (threadIdx.x % CPR) * 8, lr = threadIdx.x / CPR;
-  const Cols<8> c = cols<8>(p, n);
-  float sa[MI];
+      for (int j = 0; j < NI; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    constexpr int SPT = (BM + BN + G::THREADS - 1) / G::THREADS, BPT = (BN + G::THREADS - 1) / G::THREADS;
+    float sc[SPT], bi[BPT];
+    // fragments: A's run D steps ahead of their products through a ring of four, B's k groups alternate between two sets
+    constexpr int D = MI < 3 ? MI : 3;
+    i32x4 af[4], bf[2][NI];
+    auto read = [&](int s, int u) {         // step u of a stage: fragment u % MI of A in k group u / MI (with its first one, B's of that group)
+      const char* st = smem + (s & 1) * STG;
+      const int k = u / MI;
+      if (u % MI == 0) {
 #pragma unroll
-  for (int i = 0; i < MI; ++i) sa[i] = p.alpha * p.sA[min(m0 + wm + i * 16 + fr, p.M - 1)];
-#pragma unroll
-  for (int ps = 0; ps < MI / 2; ++ps) {
-    // staged row r of the pass is row (r >> 5) * BM / 2 + ps * 32 + (r & 31) of the tile
-    auto row_of = [&](int r) { return m0 + (r >> 5) * (BM / 2) + ps * 32 + (r & 31); };
-    u32x4 res[NIT];
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) res[it] = residual_of<8>(p, row_of(it * RPI + lr), n);
-    __syncthreads();
-#pragma unroll
-    for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const i32x4 v = acc[ps * 2 + ii][j];
-        const float x = sa[ps * 2 + ii];
-        *reinterpret_cast<float4*>(cs + ((wave >> 1) * 32 + ii * 16 + fr) * PB + wn + j * 16 + fg * 4) =
-            make_float4((float)v[0] * x, (float)v[1] * x, (float)v[2] * x, (float)v[3] * x);
+        for (int j = 0; j < NI; ++j) bf[k][j] = *reinterpret_cast<const i32x4*>(st + boff[k] + j * 4 * BK);
       }
-    __syncthreads();
+      af[u % 4] = *reinterpret_cast<const i32x4*>(st + aoff[k] + u % MI * 16 * BK);
+    };
+    auto multiply = [&](int u) {
 #pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int r = it * RPI + lr, m = row_of(r);
-      if (m < p.M && n < p.N) {
-        const float4 x = *reinterpret_cast<const float4*>(cs + r * PB + (threadIdx.x % CPR) * 8), y = *reinterpret_cast<const float4*>(cs + r * PB + (threadIdx.x % CPR) * 8 + 4);
-        float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-        finish<8>(p, v, c, res[it], m, n);
+      for (int j = 0; j < NI; ++j) acc[u % MI][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[u / MI][j], af[u % 4], acc[u % MI][j], 0, 0, 0);
+    };
+    if (nst > 1) { if (stored) wait_barrier<DD + G::STORES>(); else wait_barrier<DD>(); }
+    else if (stored) wait_barrier<G::STORES>();
+    else wait_barrier<0>();
+#pragma unroll
+    for (int u = 0; u < D; ++u) read(0, u);
+    for (int s = 0; s < nst - 1; ++s) {
+#pragma unroll
+      for (int u = 0; u < 2 * MI; ++u) {
+        if (u == 2 * MI - D) {              // the reads of stage s are done, stage s + 1 has landed: the image of stage s is free
+          if (s == 0 && stored) wait_barrier<G::STORES>(); else wait_barrier<0>();
+          if (s + 2 < nst) issue(s + 2);
+        }
+        if (u + D < 2 * MI) read(s, u + D); else read(s + 1, u + D - 2 * MI);
+        multiply(u);
+        if ((u + D) % MI == 0) __builtin_amdgcn_sched_group_barrier(0x100, NI + 1, 0); else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, NI, 0);
       }
     }
+    // last stage, the scales of the write-out on their way under it
+#pragma unroll
+    for (int x = 0; x < SPT; ++x) {
+      const int i = tid + x * G::THREADS;
+      sc[x] = i < BM ? p.sA[min(m0 + i, p.M - 1)] * p.alpha : p.sB[min(n0 + i - BM, p.N - 1)];
+    }
+#pragma unroll
+    for (int x = 0; x < BPT; ++x) bi[x] = p.bias ? p.bias[min(n0 + tid + x * G::THREADS, p.N - 1)] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 2 * MI; ++u) {
+      if (u + D < 2 * MI) read(nst - 1, u + D);
+      if (krem < BK && (u / MI * 4 + fg) * 16 >= krem) af[u % 4] = i32x4{0, 0, 0, 0};
+      multiply(u);
+    }
+#pragma unroll
+    for (int x = 0; x < SPT; ++x) if (tid + x * G::THREADS < BM + BN) s_a[tid + x * G::THREADS] = sc[x];
+#pragma unroll
+    for (int x = 0; x < BPT; ++x) if (tid + x * G::THREADS < BN) s_b[BN + tid + x * G::THREADS] = bi[x];
+    const int m0w = m0 + wm, n0w = n0 + wn, tm = m0w + fr, tn = n0w + fg * (NI * 4);
+    const bool more = (r + 1) * nwg + (int)blockIdx.x < ntiles;
+    wait_barrier<0>();                      // scales visible, both stage images free
+    if (m0 + BM <= p.M && n0 + BN <= p.N && !p.c_f32 && p.act != V2S_ACT_GELU) {
+      // whole bf16 tile: the next one's first stages are requested, then 16 rows of the wave at a time -- a lane finishes its 4 NI columns of one row, and
+      // the rows pass through LDS of the wave's own so that its stores write whole cache lines.  The residual is requested one step ahead
+      if (more) {
+        place(r + 1);
+        issue(0);
+        if (nst > 1) issue(1);
+      }
+      stored = true;
+      constexpr int Q = NI / 2, CPL = NI * 2;                               // groups of 8 columns of a lane, 16-byte chunks per row
+      char* const out = smem + 2 * STG + wave * G::OUT;
+      const float *sb = s_b + wn + fg * (NI * 4), *sa = s_a + wm + fr;
+      const int sw = fr & (CPL - 1);
+      bf16_t* dst[Q];
+      const char* src[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int row = (q * 64 + lane) / CPL, ch = lane % CPL;
+        dst[q] = (bf16_t*)p.C + (long)(m0w + row) * p.ldc + n0w + ch * 8;
+        src[q] = out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16;
+      }
+      const bf16_t* rp = p.residual ? p.residual + (long)tm * p.ldr + tn : nullptr;
+      u32x4 res[Q];
+      if (p.residual) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) res[q] = *reinterpret_cast<const u32x4*>(rp + q * 8);
+      }
+      Cols<8> c[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) { c[q].s[x] = sb[q * 8 + x]; c[q].b[x] = sb[BN + q * 8 + x]; }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const float a = sa[i * 16];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          float v[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = (float)acc[i][q * 2 + (x >> 2)][x & 3] * a;
+          activate<8, false>(p, v, c[q]);
+          if (p.residual) {
+            add_residual<8>(v, res[q]);
+            if (i + 1 < MI) res[q] = *reinterpret_cast<const u32x4*>(rp + (long)(i + 1) * 16 * p.ldr + q * 8);
+          }
+          *reinterpret_cast<u32x4*>(out + fr * (NI * 32) + ((fg * Q + q) ^ sw) * 16) = pack<8>(v);
+        }
+#pragma unroll
+        for (int q = 0; q < Q; ++q) *reinterpret_cast<u32x4*>(dst[q] + (long)i * 16 * p.ldc) = *reinterpret_cast<const u32x4*>(src[q]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      continue;
+    }
+    // any other tile: as fp32 through the stage images (a half of the wave's rows at a time where they do not hold it all), then four columns per lane
+    constexpr int HALVES = BM * BN * 4 > 2 * STG ? 2 : 1, HI = MI / HALVES, HR = BM / HALVES, CH = BN / 4;
+    static_assert(HR * BN * 4 <= 2 * STG, "a half fits the stage images");
+    float* const cs = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int hf = 0; hf < HALVES; ++hf) {
+#pragma unroll
+      for (int i = 0; i < HI; ++i) {
+        const float a = s_a[wm + (hf * HI + i) * 16 + fr];
+        const int row = wm / HALVES + i * 16 + fr;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const i32x4 v = acc[hf * HI + i][j];
+          *reinterpret_cast<float4*>(cs + row * BN + ((((wn + fg * (NI * 4)) >> 2) + j) ^ (row & 7)) * 4) =
+              make_float4((float)v[0] * a, (float)v[1] * a, (float)v[2] * a, (float)v[3] * a);
+        }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int x = tid; x < HR * CH; x += G::THREADS) {
+        const int row = x / CH, ch = x % CH, n = n0 + ch * 4;
+        const int m = m0 + row / (HI * 16) * (MI * 16) + hf * (HI * 16) + row % (HI * 16);
+        if (m < p.M && n < p.N) {
+          const float4 f = *reinterpret_cast<const float4*>(cs + row * BN + (ch ^ (row & 7)) * 4);
+          float v[4] = {f.x, f.y, f.z, f.w};
+          Cols<4> c;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) { c.s[y] = s_b[ch * 4 + y]; c.b[y] = s_b[BN + ch * 4 + y]; }
+          finish4(p, v, c, m, n);
+        }
+      }
+      __syncthreads();
+    }
+    if (more) {
+      place(r + 1);
+      issue(0);
+      if (nst > 1) issue(1);
+    }
+    stored = false;
   }
 }
 
@@ -259,18 +414,18 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_q8_skinny_kernel(const GemmQ8
     if (m < p.M && n < p.N) {
       const float sa = p.alpha * p.sA[m];
       float x[4] = {(float)v[0] * sa, (float)v[1] * sa, (float)v[2] * sa, (float)v[3] * sa};
-      finish<4>(p, x, cols<4>(p, n), residual_of<4>(p, m, n), m, n);
+      finish4(p, x, cols<4>(p, n), m, n);
     }
   }
 }
 
-template <int BM, int BN> int tile_launch(GemmQ8& p, hipStream_t s) {
-  constexpr int LDS = Tile<BM, BN>::STG * Tile<BM, BN>::NST;
+template <class G> int tile_launch(GemmQ8& p, hipStream_t s) {
   static bool attr = false;
-  if (!attr) { (void)hipFuncSetAttribute((const void*)gemm_q8_tile_kernel<BM, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); attr = true; }
-  p.tilesM = (p.M + BM - 1) / BM; p.tilesN = (p.N + BN - 1) / BN;
-  V2S_CHECK((int64_t)p.tilesM * p.tilesN <= 0x7fffffff, V2S_ERR_SHAPE, "v2s_gemm_q8: too many tiles for one launch");
-  hipLaunchKernelGGL((gemm_q8_tile_kernel<BM, BN>), dim3(p.tilesM * p.tilesN), dim3(256), LDS, s, p);
+  if (!attr) { (void)hipFuncSetAttribute((const void*)gemm_q8_tile_kernel<G>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS); attr = true; }
+  p.tilesM = (p.M + G::BM - 1) / G::BM; p.tilesN = (p.N + G::BN - 1) / G::BN;
+  const int64_t tiles = (int64_t)p.tilesM * p.tilesN;
+  V2S_CHECK(tiles <= 0x3fffffff, V2S_ERR_SHAPE, "v2s_gemm_q8: too many tiles for one launch");
+  hipLaunchKernelGGL((gemm_q8_tile_kernel<G>), dim3((unsigned)(tiles < 256 * G::OCC ? tiles : 256 * G::OCC)), dim3(G::THREADS), G::LDS, s, p);
   V2S_LAUNCH_CHECK();
   return V2S_OK;
 }
@@ -301,9 +456,10 @@ extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   int kind = v2s_opt_gemm_q8();
   if (kind == 0) kind = p.M <= 64 ? 1 : (tiles(128, 256) >= 512 ? 4 : (tiles(128, 128) >= 256 ? 3 : 2));
-  if (kind == 4) return tile_launch<128, 256>(p, s);
-  if (kind == 3) return tile_launch<128, 128>(p, s);
-  if (kind == 2) return tile_launch<64, 64>(p, s);
+  if (kind == 5) return tile_launch<Tile<128, 256, 2, 4, 1>>(p, s);
+  if (kind == 4) return tile_launch<Tile<256, 256, 2, 4, 1>>(p, s);
+  if (kind == 3) return tile_launch<Tile<128, 128, 2, 2, 2>>(p, s);
+  if (kind == 2) return tile_launch<Tile<64, 64, 2, 2, 4>>(p, s);
   const bool wide = p.N >= 8192, deep = p.K > 1024;
   V2S_CHECK((p.M + 15) / 16 <= 65535, V2S_ERR_SHAPE, "v2s_gemm_q8: too many rows for the few-row kernels");
   if (p.M <= 16) return deep ? skinny_launch<8, 1, 1>(p, s) : (wide ? skinny_launch<4, 1, 4>(p, s) : skinny_launch<4, 1, 1>(p, s));
