@@ -138,8 +138,13 @@ struct Tile {
   static __device__ __forceinline__ int swzB(int row) { return ((row >> 1) & 1) | ((row / (NI * 4) & 3) << 1); }
 };
 
-template <class G>
+// what a kernel's write-out can do: bf16 with none / ReLU, the same with a residual, everything (the registers of the 256 x 256 tile hold one of the first
+// two without spilling)
+enum { EPI_PLAIN, EPI_RESIDUAL, EPI_ANY };
+
+template <class G, int EPI>
 __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_tile_kernel(const GemmQ8 p) {
+  const bool has_res = EPI == EPI_RESIDUAL || (EPI == EPI_ANY && p.residual), f32 = EPI == EPI_ANY && p.c_f32;
   constexpr int BM = G::BM, BN = G::BN, BK = G::BK, DA = G::DA, DB = G::DB, MI = G::MI, NI = G::NI, STG = G::STG, DD = DA + DB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const s_a = reinterpret_cast<float*>(smem + 2 * STG + G::WAVES * G::OUT);      // scales of the tile's rows, scales and bias of its columns
@@ -263,33 +268,35 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
     const int m0w = m0 + wm, n0w = n0 + wn, tm = m0w + fr, tn = n0w + fg * (NI * 4);
     const bool more = (r + 1) * nwg + (int)blockIdx.x < ntiles;
     wait_barrier<0>();                      // scales visible, both stage images free
-    if (m0 + BM <= p.M && n0 + BN <= p.N && !p.c_f32 && p.act != V2S_ACT_GELU) {
-      // whole bf16 tile: the next one's first stages are requested, then 16 rows of the wave at a time -- a lane finishes its 4 NI columns of one row, and
-      // the rows pass through LDS of the wave's own so that its stores write whole cache lines.  The residual is requested one step ahead
+    if (n0 + BN <= p.N || p.N % 8 == 0) {
+      // the next tile's first stages are requested, then 16 rows of the wave at a time: a lane finishes its 4 NI columns of one row, and the rows pass
+      // through LDS of the wave's own (fp32 ones in two halves) so that its stores write whole cache lines.  The residual is requested AHEAD steps early
+      constexpr int Q = NI / 2, CPL = NI * 2, AHEAD = MI < 4 ? MI : 4;      // groups of 8 columns of a lane, 16-byte chunks per row
+      const bf16_t* rp = p.residual + (long)tm * p.ldr + tn;
+      u32x4 res[AHEAD][Q];
+      auto fetch = [&](int i) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          res[i % AHEAD][q] = u32x4{0, 0, 0, 0};
+          if (tm + i * 16 < p.M && tn + q * 8 < p.N) res[i % AHEAD][q] = *reinterpret_cast<const u32x4*>(rp + (long)i * 16 * p.ldr + q * 8);
+        }
+      };
+      if (has_res) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fetch(i);
+      }
+      const int mlim = p.M - m0w, nlim = p.N - n0w;
+      stored = m0 + BM <= p.M && n0 + BN <= p.N;
       if (more) {
         place(r + 1);
         issue(0);
         if (nst > 1) issue(1);
       }
-      stored = true;
-      constexpr int Q = NI / 2, CPL = NI * 2;                               // groups of 8 columns of a lane, 16-byte chunks per row
       char* const out = smem + 2 * STG + wave * G::OUT;
       const float *sb = s_b + wn + fg * (NI * 4), *sa = s_a + wm + fr;
       const int sw = fr & (CPL - 1);
-      bf16_t* dst[Q];
-      const char* src[Q];
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int row = (q * 64 + lane) / CPL, ch = lane % CPL;
-        dst[q] = (bf16_t*)p.C + (long)(m0w + row) * p.ldc + n0w + ch * 8;
-        src[q] = out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16;
-      }
-      const bf16_t* rp = p.residual ? p.residual + (long)tm * p.ldr + tn : nullptr;
-      u32x4 res[Q];
-      if (p.residual) {
-#pragma unroll
-        for (int q = 0; q < Q; ++q) res[q] = *reinterpret_cast<const u32x4*>(rp + q * 8);
-      }
+      const int ch = lane % CPL, row0 = lane / CPL;      // what the lane stores: chunk ch of the rows row0 + q * 64 / CPL
+      const long at = (long)(m0w + row0) * p.ldc + n0w + ch * (f32 ? 4 : 8);
       Cols<8> c[Q];
 #pragma unroll
       for (int q = 0; q < Q; ++q)
@@ -298,25 +305,47 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const float a = sa[i * 16];
+        float v[Q][8];
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-          float v[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[x] = (float)acc[i][q * 2 + (x >> 2)][x & 3] * a;
-          activate<8, false>(p, v, c[q]);
-          if (p.residual) {
-            add_residual<8>(v, res[q]);
-            if (i + 1 < MI) res[q] = *reinterpret_cast<const u32x4*>(rp + (long)(i + 1) * 16 * p.ldr + q * 8);
-          }
-          *reinterpret_cast<u32x4*>(out + fr * (NI * 32) + ((fg * Q + q) ^ sw) * 16) = pack<8>(v);
+          for (int x = 0; x < 8; ++x) v[q][x] = (float)acc[i][q * 2 + (x >> 2)][x & 3] * a;
+          activate<8, EPI == EPI_ANY>(p, v[q], c[q]);
+          if (has_res) add_residual<8>(v[q], res[i % AHEAD][q]);
         }
+        if (has_res && i + AHEAD < MI) fetch(i + AHEAD);
+        if (!f32) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) *reinterpret_cast<u32x4*>(dst[q] + (long)i * 16 * p.ldc) = *reinterpret_cast<const u32x4*>(src[q]);
+          for (int q = 0; q < Q; ++q) *reinterpret_cast<u32x4*>(out + fr * (NI * 32) + ((fg * Q + q) ^ sw) * 16) = pack<8>(v[q]);
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            const int row = row0 + q * (64 / CPL);
+            const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
+            if (i * 16 + row < mlim && ch * 8 < nlim) *reinterpret_cast<u32x4*>((bf16_t*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc) = o;
+          }
+        } else {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            if (fg >> 1 == hf) {
+#pragma unroll
+              for (int x = 0; x < NI; ++x)
+                *reinterpret_cast<float4*>(out + fr * (NI * 32) + (((fg & 1) * NI + x) ^ sw) * 16) =
+                    make_float4(v[x >> 1][(x & 1) * 4], v[x >> 1][(x & 1) * 4 + 1], v[x >> 1][(x & 1) * 4 + 2], v[x >> 1][(x & 1) * 4 + 3]);
+            }
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+              const int row = row0 + q * (64 / CPL);
+              const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
+              if (i * 16 + row < mlim && hf * (NI * 8) + ch * 4 < nlim)
+                *reinterpret_cast<u32x4*>((float*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc + hf * (NI * 8)) = o;
+            }
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       continue;
     }
-    // any other tile: as fp32 through the stage images (a half of the wave's rows at a time where they do not hold it all), then four columns per lane
+    // a tile whose columns N cuts within a group of 8: as fp32 through the stage images (a half of the wave's rows at a time where they do not hold it all), then four columns per lane
     constexpr int HALVES = BM * BN * 4 > 2 * STG ? 2 : 1, HI = MI / HALVES, HR = BM / HALVES, CH = BN / 4;
     static_assert(HR * BN * 4 <= 2 * STG, "a half fits the stage images");
     float* const cs = reinterpret_cast<float*>(smem);
@@ -419,15 +448,22 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_q8_skinny_kernel(const GemmQ8
   }
 }
 
-template <class G> int tile_launch(GemmQ8& p, hipStream_t s) {
+template <class G, int EPI> int tile_launch(GemmQ8& p, hipStream_t s) {
   static bool attr = false;
-  if (!attr) { (void)hipFuncSetAttribute((const void*)gemm_q8_tile_kernel<G>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS); attr = true; }
+  if (!attr) { (void)hipFuncSetAttribute((const void*)gemm_q8_tile_kernel<G, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS); attr = true; }
   p.tilesM = (p.M + G::BM - 1) / G::BM; p.tilesN = (p.N + G::BN - 1) / G::BN;
   const int64_t tiles = (int64_t)p.tilesM * p.tilesN;
   V2S_CHECK(tiles <= 0x3fffffff, V2S_ERR_SHAPE, "v2s_gemm_q8: too many tiles for one launch");
-  hipLaunchKernelGGL((gemm_q8_tile_kernel<G>), dim3((unsigned)(tiles < 256 * G::OCC ? tiles : 256 * G::OCC)), dim3(G::THREADS), G::LDS, s, p);
+  hipLaunchKernelGGL((gemm_q8_tile_kernel<G, EPI>), dim3((unsigned)(tiles < 256 * G::OCC ? tiles : 256 * G::OCC)), dim3(G::THREADS), G::LDS, s, p);
   V2S_LAUNCH_CHECK();
   return V2S_OK;
+}
+typedef Tile<256, 256, 2, 4, 1> Tile256;
+typedef Tile<128, 128, 2, 2, 2> Tile128;
+typedef Tile<64, 64, 2, 2, 4> Tile64;
+template <class G> int tile_any(GemmQ8& p, bool plain, hipStream_t s) {
+  if (!plain) return tile_launch<G, EPI_ANY>(p, s);
+  return p.residual ? tile_launch<G, EPI_RESIDUAL>(p, s) : tile_launch<G, EPI_PLAIN>(p, s);
 }
 template <int WAVES, int MT, int NT> int skinny_launch(const GemmQ8& p, hipStream_t s) {
   hipLaunchKernelGGL((gemm_q8_skinny_kernel<WAVES, MT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, s, p);
@@ -456,10 +492,10 @@ extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   int kind = v2s_opt_gemm_q8();
   if (kind == 0) kind = p.M <= 64 ? 1 : (tiles(128, 256) >= 512 ? 4 : (tiles(128, 128) >= 256 ? 3 : 2));
-  if (kind == 5) return tile_launch<Tile<128, 256, 2, 4, 1>>(p, s);
-  if (kind == 4) return tile_launch<Tile<256, 256, 2, 4, 1>>(p, s);
-  if (kind == 3) return tile_launch<Tile<128, 128, 2, 2, 2>>(p, s);
-  if (kind == 2) return tile_launch<Tile<64, 64, 2, 2, 4>>(p, s);
+  const bool plain = !p.c_f32 && p.act != V2S_ACT_GELU;
+  if (kind == 4 && plain) return p.residual ? tile_launch<Tile256, EPI_RESIDUAL>(p, s) : tile_launch<Tile256, EPI_PLAIN>(p, s);
+  if (kind >= 3) return tile_any<Tile128>(p, plain, s);
+  if (kind == 2) return tile_any<Tile64>(p, plain, s);
   const bool wide = p.N >= 8192, deep = p.K > 1024;
   V2S_CHECK((p.M + 15) / 16 <= 65535, V2S_ERR_SHAPE, "v2s_gemm_q8: too many rows for the few-row kernels");
   if (p.M <= 16) return deep ? skinny_launch<8, 1, 1>(p, s) : (wide ? skinny_launch<4, 1, 4>(p, s) : skinny_launch<4, 1, 1>(p, s));
