@@ -186,19 +186,20 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
     ga = p.A + (long)m0 * p.lda;
     gb = p.B + (long)n0 * p.ldb;
   };
-  auto issue = [&](int s) {
+  auto piece = [&](int s, int x) {          // one of the DA + DB DMA instructions of a stage
     const uint32_t slot = sbase + (s & 1) * STG;
-    const bool cut = s == nst - 1 && krem < BK;
-#pragma unroll
-    for (int i = 0; i < DA; ++i) {
-      const int g = (pos ^ G::swzA((wave * DA + i) * 8 + rl)) * 16;
-      dma16(cut && g >= krem ? oa[i] - g : oa[i], ga + (long)s * BK, slot + (wave * DA + i) * 1024);
+    const int lim = s == nst - 1 ? krem : BK;
+    if (x < DA) {
+      const int g = (pos ^ G::swzA((wave * DA + x) * 8 + rl)) * 16;
+      dma16(oa[x] - (g >= lim ? g : 0), ga + (long)s * BK, slot + (wave * DA + x) * 1024);
+    } else {
+      const int y = x - DA, g = (pos ^ G::swzB((wave * DB + y) * 8 + rl)) * 16;
+      dma16(ob[y] - (g >= lim ? g : 0), gb + (long)s * BK, slot + BM * BK + (wave * DB + y) * 1024);
     }
+  };
+  auto issue = [&](int s) {
 #pragma unroll
-    for (int i = 0; i < DB; ++i) {
-      const int g = (pos ^ G::swzB((wave * DB + i) * 8 + rl)) * 16;
-      dma16(cut && g >= krem ? ob[i] - g : ob[i], gb + (long)s * BK, slot + BM * BK + (wave * DB + i) * 1024);
-    }
+    for (int x = 0; x < DD; ++x) piece(s, x);
   };
 
   place(0);
@@ -235,13 +236,28 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
 #pragma unroll
     for (int u = 0; u < D; ++u) read(0, u);
     for (int s = 0; s < nst - 1; ++s) {
+      const bool head = s >= 1, tail = s + 2 < nst;
 #pragma unroll
       for (int u = 0; u < 2 * MI; ++u) {
-        if (u == 2 * MI - D) {              // the reads of stage s are done, stage s + 1 has landed: the image of stage s is free
+        // the requests of a stage go out PER a step (all at once they queue up in front of the block's products): the first ones behind the barrier, the
+        // rest in the first steps of the next stage
+        constexpr int PER = MI == 8 ? 1 : 2;
+        const int t = u - (2 * MI - D);     // steps behind the barrier
+        if (t == 0) {                       // the reads of stage s are done, stage s + 1 has landed: the image of stage s is free
           if (s == 0 && stored) wait_barrier<G::STORES>(); else wait_barrier<0>();
-          if (s + 2 < nst) issue(s + 2);
         }
         if (u + D < 2 * MI) read(s, u + D); else read(s + 1, u + D - 2 * MI);
+        if (t >= 0) {
+          if (tail) {
+#pragma unroll
+            for (int x = t * PER; x < (t + 1) * PER && x < DD; ++x) piece(s + 2, x);
+          }
+        } else if ((u + D) * PER < DD) {
+          if (head) {
+#pragma unroll
+            for (int x = (u + D) * PER; x < (u + D + 1) * PER && x < DD; ++x) piece(s + 1, x);
+          }
+        }
         multiply(u);
         if ((u + D) % MI == 0) __builtin_amdgcn_sched_group_barrier(0x100, NI + 1, 0); else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x8, NI, 0);
