@@ -337,7 +337,7 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
           for (int q = 0; q < Q; ++q) {
             const int row = row0 + q * (64 / CPL);
             const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
-            if (i * 16 + row < mlim && ch * 8 < nlim) *reinterpret_cast<u32x4*>((bf16_t*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc) = o;
+            if (i * 16 + row < mlim && ch * 8 < nlim) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>((bf16_t*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc));
           }
         } else {
 #pragma unroll
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
               const int row = row0 + q * (64 / CPL);
               const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
               if (i * 16 + row < mlim && hf * (NI * 8) + ch * 4 < nlim)
-                *reinterpret_cast<u32x4*>((float*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc + hf * (NI * 8)) = o;
+                __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>((float*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc + hf * (NI * 8)));
             }
           }
         }
@@ -505,10 +505,15 @@ extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   p.C = a->C; p.ldc = a->ldc; p.c_f32 = a->c_dtype == V2S_F32; p.alpha = a->alpha; p.bias = a->bias; p.act = a->act;
   p.residual = (const bf16_t*)a->residual; p.ldr = a->ldr; p.tilesM = p.tilesN = 0;
   hipStream_t s = (hipStream_t)stream;
-  auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  // Rounds of the chip's blocks times the time of one (us, n = stages of 128): 256 x 256 tiles 6.5 + 1.5 n, 128 x 128 3.0 + 0.95 n, 64 x 64 1.9 + 0.66 n, fitted to
+  // N = 2304, K = 16 .. 3200: at K = 768, M = 1000 / 2000 / 8000 / 27501 they take 14.4 / 14.5 / 32.1 / 64.9, 8.0 / 10.1 / 22.5 / 70.7 and 7.3 / 10.1 / 27.2 / 108 us.
+  // Up to 64 rows a launch is bound by the latency of its weights, and the few-row kernels ask for all of them at once (64 x 2304 x 768: 4.4 us, 64 x 64 tiles 5.2).
+  auto rounds = [&](int t, int slots) { return (double)(((int64_t)((p.M + t - 1) / t) * ((p.N + t - 1) / t) + slots - 1) / slots); };
+  const double n = (p.K + 127) / 128;
+  const double t4 = rounds(256, 256) * (6.5 + 1.5 * n), t3 = rounds(128, 512) * (3.0 + 0.95 * n), t2 = rounds(64, 1024) * (1.9 + 0.66 * n);
   int kind = v2s_opt_gemm_q8();
-  if (kind == 0) kind = p.M <= 64 ? 1 : (tiles(128, 256) >= 512 ? 4 : (tiles(128, 128) >= 256 ? 3 : 2));
   const bool plain = !p.c_f32 && p.act != V2S_ACT_GELU;
+  if (kind == 0) kind = p.M <= 64 ? 1 : (plain && t4 <= t3 && t4 <= t2 ? 4 : (t3 <= t2 ? 3 : 2));
   if (kind == 4 && plain) return p.residual ? tile_launch<Tile256, EPI_RESIDUAL>(p, s) : tile_launch<Tile256, EPI_PLAIN>(p, s);
   if (kind >= 3) return tile_any<Tile128>(p, plain, s);
   if (kind == 2) return tile_any<Tile64>(p, plain, s);

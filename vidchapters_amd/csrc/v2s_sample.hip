@@ -7,8 +7,9 @@
 // that holds it, and by ranking the few tokens of that bin exactly.  Masses are 64-bit integers (2^46 = weight one): their sums are exact, so the
 // result depends neither on the order of the atomics nor on how the row is cut.
 // A row of up to 32768 logits is read from memory once and stays in LDS as fp32 (larger ones are read again for every pass, mostly from L2).  The
-// passes over it are bound by VALU issue, not by memory: one instruction per logit costs a block 0.2 us at V = 32228, which is why the weights'
-// exponential is a short polynomial of its own and why small top-k never touches most logits (below).
+// passes over it are bound by VALU issue, not by memory: one instruction per logit costs a block 0.2 us at V = 32228.  Hence: the weights' exponential
+// is a table and five terms of its own, small top-k never touches most logits, and the last pass compares all tokens but weighs only those it keeps.
+// 64 rows of 32228 logits, top-k 50 and top-p 0.95: SAMPLE_TOPK; 256 rows, top-p 0.92 and min-p: SAMPLE_NUCLEUS, a third of it the exact masses.
 #include <math.h>
 #include "v2s_common.h"
 
@@ -23,7 +24,7 @@ constexpr float BIN_RANGE = 33.0f;          // exp(-33) < 2^-47: what lies furth
 constexpr double ONE = 70368744177664.0;    // 2^46: 131072 tokens of weight one sum to 2^63
 
 struct SampleP {
-  const void* logits; long ld; int V, vec;
+  const void* logits; long ld; int V, vec, cpt, log_cpt;
   double inv_temp, exp2_scale; float bin_scale;   // 1 / T, log2(e) / T, bins per unit of logit
   int top_k; double top_p, min_p;
   const float* u; long u_ld; int u_steps;
@@ -54,7 +55,6 @@ __device__ double exp2_series(double r) {
 __device__ __forceinline__ double exp2_mass(double t, const double* tab) {
   constexpr double MAGIC = 105553116266496.0;      // 1.5 * 2^46: adding it leaves multiples of 1 / 64
   constexpr double C1 = LN2, C2 = C1 * LN2 / 2, C3 = C2 * LN2 / 3, C4 = C3 * LN2 / 4, C5 = C4 * LN2 / 5;
-  t = fmax(t, -100.0);
   const double t2 = t + MAGIC;
   const int n = __double2loint(t2);
   const double r = t - (t2 - MAGIC);
@@ -83,6 +83,14 @@ __device__ u64 block_sum64(u64 v, u64* red, int tid) {
   for (int i = 0; i < NT / 64; ++i) s += red[i];
   return s;
 }
+// u64 sums of a loop of independent LDS reads, eight in flight
+template <class F> __device__ __forceinline__ void list_loop(int n8, F f) {
+#pragma unroll 1
+  for (int i = 0; i < n8; i += 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f(i + j);
+  }
+}
 __device__ __forceinline__ void load4(const float* z, int i0, int V, int vec, float (&o)[4]) {
   if (vec && i0 + 4 <= V) {
     const float4 v = *reinterpret_cast<const float4*>(z + i0);
@@ -102,79 +110,84 @@ __device__ __forceinline__ void load4(const bf16_t* z, int i0, int V, int vec, f
   }
 }
 
-__device__ __forceinline__ float load1(const float* z) { return *z; }
-__device__ __forceinline__ float load1(const bf16_t* z) { return bf2f(*z); }
-
-// ROW: the row is held in LDS (zs), else every pass reads it again
+// ROW: the row is held in LDS (zs): a thread owns 4 CPT consecutive tokens, CPT = 1, 2, 4 or 8 groups of four, group c of thread t at place c ^ t of its
+// own (eight threads then read eight different banks).  Else every pass reads the row again, four consecutive tokens per thread and step.
 template <typename T, bool ROW>
 __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   extern __shared__ __attribute__((aligned(16))) float zs[];
   __shared__ u64 s_mass[NBIN];
-  __shared__ u64 s_key[CAP], s_w[CAP];
+  __shared__ u64 s_key[CAP + 8], s_w[CAP + 8];
   __shared__ double s_tab[64];
   __shared__ u64 s_red[NT / 64], s_thr, s_base;
   __shared__ float s_max[NT / 64];
   __shared__ int s_n, s_bin, s_nan;
   uint32_t* const s_cnt = reinterpret_cast<uint32_t*>(s_mass);      // the counts of top-k, before the masses of top-p
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = blockIdx.x, V = p.V, nj = (V + STEP - 1) / STEP;
+  const int row = blockIdx.x, V = p.V, cpt = p.cpt;
+  const int nj = ROW ? cpt : (V + STEP - 1) / STEP;
   const T* z0 = (const T*)p.logits + (long)row * p.ld;
   const int step = p.pos_dev ? *p.pos_dev : 0;
   const int ban = (p.eos_id >= 0 && (p.pos_dev ? step + 1 : 0) < p.min_length) ? p.eos_id : -1;
+  int edge = 0;                             // 1: the maximum is +infinity, its tokens share everything; -1: every token is -infinity, all are equal
 
-  auto fetch = [&](int j, float (&z)[4]) {  // logits of pass j as the caller's rules leave them; -0 becomes +0
-    const int i0 = j * STEP + tid * 4;
-    load4(z0, i0, V, p.vec, z);
+  auto fetch = [&](int g, float (&z)[4]) {  // group g of four tokens as the caller's rules leave them; -0 becomes +0, behind the row -infinity
+    load4(z0, g * 4, V, p.vec, z);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = i0 + i == ban ? -INFINITY : z[i] + 0.0f;
+    for (int i = 0; i < 4; ++i) z[i] = g * 4 + i == ban ? -INFINITY : z[i] + 0.0f;
   };
+  auto settle = [&](float z, int idx) { return edge > 0 ? (z == INFINITY ? 0.f : -INFINITY) : (edge < 0 && idx < V ? 0.f : z); };
+  auto group = [&](int j) { return ROW ? tid * cpt + j : j * NT + tid; };
+  auto place = [&](int g) { return (g & ~(cpt - 1)) | ((g ^ (g >> p.log_cpt)) & (cpt - 1)); };
   auto get = [&](int j, float (&z)[4]) {
     if constexpr (ROW) {
-      const float4 v = *reinterpret_cast<const float4*>(zs + j * STEP + tid * 4);
+      const float4 v = *reinterpret_cast<const float4*>(zs + place(group(j)) * 4);
       z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w;
     } else {
-      fetch(j, z);
+      fetch(group(j), z);
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = settle(z[i], group(j) * 4 + i);
+      }
     }
-  };
-  auto one = [&](int idx) -> float {
-    if constexpr (ROW) return zs[idx];
-    else return idx == ban ? -INFINITY : load1(z0 + idx) + 0.0f;
   };
   auto each = [&](auto f) {                 // f(index, logit) for the tokens of this thread, in index order
 #pragma unroll 1
     for (int j = 0; j < nj; ++j) {
       float z[4];
       get(j, z);
+      const int idx = group(j) * 4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { const int idx = j * STEP + tid * 4 + i; if (idx < V) f(idx, z[i]); }
+      for (int i = 0; i < 4; ++i) f(idx + i, z[i]);
     }
   };
 
   int nan_at = V;
-  float tmax = -INFINITY;                   // maximum of this thread's tokens
-  if (tid < 64) s_tab[tid] = exp2_series(tid / 64.0);
+  float tmax = -INFINITY;                   // maximum of the tokens this thread has read
   if constexpr (ROW) {
     float z[ROW_MAX][4];
 #pragma unroll
-    for (int j = 0; j < ROW_MAX; ++j) if (j < nj) fetch(j, z[j]);   // every load in flight before the first is used
+    for (int j = 0; j < ROW_MAX; ++j) if (j < cpt) fetch(j * NT + tid, z[j]);       // every load in flight before the first is used
+    if (tid < 64) s_tab[tid] = exp2_series(tid / 64.0);
 #pragma unroll
     for (int j = 0; j < ROW_MAX; ++j)
-      if (j < nj) {
+      if (j < cpt) {
+        const int g = j * NT + tid;
 #pragma unroll
         for (int i = 3; i >= 0; --i) {
           tmax = fmaxf(tmax, z[j][i]);
-          if (z[j][i] != z[j][i]) nan_at = min(nan_at, j * STEP + tid * 4 + i);
+          if (z[j][i] != z[j][i]) nan_at = min(nan_at, g * 4 + i);
         }
-        *reinterpret_cast<float4*>(zs + j * STEP + tid * 4) = make_float4(z[j][0], z[j][1], z[j][2], z[j][3]);   // read by the same thread only
+        *reinterpret_cast<float4*>(zs + place(g) * 4) = make_float4(z[j][0], z[j][1], z[j][2], z[j][3]);
       }
   } else {
+    if (tid < 64) s_tab[tid] = exp2_series(tid / 64.0);
     each([&](int idx, float z) {
       if (z != z) nan_at = min(nan_at, idx);
       tmax = fmaxf(tmax, z);
     });
   }
   float zmax = wave_max(tmax);
-  if (tid == 0) { s_nan = V; s_n = 0; s_bin = NBIN; }
+  if (tid == 0) { s_nan = V; s_n = 0; }
   if (lane == 0) s_max[wave] = zmax;
   s_mass[tid] = 0; s_mass[tid + NT] = 0;
   __syncthreads();
@@ -198,14 +211,28 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     if (tid == 0) finish(s_nan, __uint_as_float(0x7fc00000u));
     return;
   }
+  if (!(fabsf(zmax) < INFINITY)) {
+    edge = zmax > 0.f ? 1 : -1;
+    tmax = settle(tmax, 0);                 // (a thread behind the row counts as one more token; the list below is gathered from the tokens)
+    if constexpr (ROW) {
+      for (int j = 0; j < nj; ++j) {
+        float z[4];
+        get(j, z);
+        const int g = group(j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = settle(z[i], g * 4 + i);
+        *reinterpret_cast<float4*>(zs + place(g) * 4) = make_float4(z[0], z[1], z[2], z[3]);
+      }
+    }
+    zmax = 0.f;
+  }
   const float uf = p.u[(p.pos_dev ? (long)max(0, min(step, p.u_steps - 1)) * p.u_ld : 0) + row];
-  const double u = (double)fmaxf(uf, 0.f);
+  const double u = (double)fmaxf(uf, 0.f), dmax = (double)zmax, min_w = p.min_p * ONE;
 
-  auto far_of = [&](float z) { return z == zmax ? 0.f : (zmax - z) * p.bin_scale; };      // in bins
+  auto far_of = [&](float z) { return (zmax - z) * p.bin_scale; };                        // in bins; the last bin holds what has no mass
   auto bin_of = [&](float z) { return (int)fminf(far_of(z), (float)(NBIN - 1)); };
-  const double dmax = (double)zmax, min_w = p.min_p * ONE;
-  auto weight = [&](float z) -> double { return exp2_mass(z == zmax ? 0.0 : ((double)z - dmax) * p.exp2_scale, s_tab); };      // 2^46 w
-  auto log_prob = [&](float z, u64 total) { return (float)((z == zmax ? 0.0 : ((double)z - (double)zmax) * p.inv_temp) - log((double)total / ONE)); };
+  auto weight = [&](float z) -> double { return exp2_mass(((double)z - dmax) * p.exp2_scale, s_tab); };      // 2^46 w
+  auto log_prob = [&](float z, u64 total) { return (float)(((double)z - dmax) * p.inv_temp - log((double)total / ONE)); };
 
   // bin of the boundary: the first one at which the running sum (of counts or masses) reaches the goal; s_base = the sum before it
   auto find_bin = [&](auto value, auto reached) {
@@ -216,7 +243,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     if (tid == 0) { s_bin = NBIN - 1; s_n = 0; }
     __syncthreads();
     u64 pre = inc - (a + b);
-    for (int i = 0; i < wave; ++i) pre += s_red[i];
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) pre += i < wave ? s_red[i] : 0;
     if (!reached(pre) && reached(pre + a)) { s_bin = 2 * tid; s_base = pre; }
     else if (!reached(pre + a) && reached(pre + a + b)) { s_bin = 2 * tid + 1; s_base = pre + a; }
     __syncthreads();
@@ -228,7 +256,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   // contain the first k, and there are few more of them.  Everything else is decided among these candidates.
   if (cut_k && p.top_k <= SMALL_K) {
     const int b0 = bin_of(tmax);
-    if (tid * 4 < V && b0 < NBIN - 1) atomicAdd(&s_cnt[b0], 1u);
+    if (b0 < NBIN - 1) atomicAdd(&s_cnt[b0], 1u);
     __syncthreads();
     const u64 k = (u64)p.top_k;
     find_bin([&](int b) { return (u64)s_cnt[b]; }, [&](u64 s) { return s >= k; });
@@ -242,9 +270,11 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
         }
       });
       __syncthreads();
-      const int n = s_n;
-      if (n <= SMALL_N) {                   // the same for the whole block
-        u64 key = 0, w = 0;
+      const int n = s_n, n8 = (n + 7) & ~7;
+      if (n >= p.top_k && n <= SMALL_N) {   // the same for the whole block
+        if (tid >= n && tid < n8) s_key[tid] = ~0ull;
+        __syncthreads();
+        u64 key = ~0ull, w = 0;
         double wd = 0.0;
         float z = 0.f;
         bool in = false;
@@ -252,15 +282,14 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
           key = s_key[tid];
           z = key_logit(key);
           int rank = 0;
-          for (int i = 0; i < n; ++i) rank += s_key[i] < key ? 1 : 0;
+          list_loop(n8, [&](int i) { rank += s_key[i] < key ? 1 : 0; });
           in = rank < p.top_k;
           if (in) { wd = weight(z); w = mass_of(wd); }
-          s_w[tid] = w;
         }
+        if (tid < n8) s_w[tid] = w;
         __syncthreads();
         u64 total = 0, pre = 0;
-        if (tid < n)
-          for (int i = 0; i < n; ++i) { const u64 x = s_w[i]; total += x; pre += s_key[i] < key ? x : 0; }
+        if (tid < n) list_loop(n8, [&](int i) { const u64 x = s_w[i]; total += x; pre += s_key[i] < key ? x : 0; });
         __syncthreads();
         const bool keep = in && w > 0 && wd >= min_w && (p.top_p >= 1.0 || (double)pre < p.top_p * (double)total);
         if (tid < n) s_w[tid] = keep ? w : 0;
@@ -268,7 +297,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
         if (keep) {
           u64 run = 0;
           total = 0;
-          for (int i = 0; i < n; ++i) { const u64 x = s_w[i]; total += x; run += (uint32_t)s_key[i] <= (uint32_t)key ? x : 0; }
+          list_loop(n8, [&](int i) { const u64 x = s_w[i]; total += x; run += (uint32_t)s_key[i] <= (uint32_t)key ? x : 0; });
           const double goal = u * (double)total;
           if (((double)run > goal && !((double)(run - w) > goal)) || (!((double)total > goal) && run == total)) finish((int)(uint32_t)key, log_prob(z, total));
         }
@@ -284,36 +313,41 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   auto resolve = [&](auto in, auto value, auto reached) -> u64 {
     const int bin = s_bin;
     const u64 base = s_base;
+    const float lo = (float)bin, hi = (float)(bin + 1);
     each([&](int idx, float z) {
-      if (bin_of(z) == bin && in(z, idx)) {
+      const float far = far_of(z);
+      if (far >= lo && far < hi && in(z, idx)) {
         const int at = atomicAdd(&s_n, 1);
         if (at < CAP) { s_key[at] = order_key(z, idx); s_w[at] = value(z); }
       }
     });
     __syncthreads();
-    const int n = s_n;
+    const int n = s_n, n8 = (n + 7) & ~7;
     if (n <= CAP) {
+      if (tid >= n && tid < n8) { s_key[tid] = ~0ull; s_w[tid] = 0; }
+      __syncthreads();
       if (tid < n) {
         const u64 key = s_key[tid], w = s_w[tid];
         u64 pre = base;
-        for (int i = 0; i < n; ++i) pre += s_key[i] < key ? s_w[i] : 0;
+        list_loop(n8, [&](int i) { pre += s_key[i] < key ? s_w[i] : 0; });
         if (!reached(pre) && reached(pre + w)) s_thr = key;
       }
       __syncthreads();
       return s_thr;
     }
     // too many tokens within one bin (a plateau of equal logits): bisection on the order key
-    u64 lo = 0, hi = ~0ull;                 // sum(keys <= hi) reaches the goal
-    while (lo < hi) {
-      const u64 mid = lo + ((hi - lo) >> 1);
+    u64 first = 0, last = ~0ull;            // sum(keys <= last) reaches the goal
+    while (first < last) {
+      const u64 mid = first + ((last - first) >> 1);
       u64 s = 0;
       each([&](int idx, float z) {
-        if (bin_of(z) == bin && in(z, idx) && order_key(z, idx) <= mid) s += value(z);
+        const float far = far_of(z);
+        if (far >= lo && far < hi && in(z, idx) && order_key(z, idx) <= mid) s += value(z);
       });
       s = block_sum64(s, s_red, tid);
-      if (reached(base + s)) hi = mid; else lo = mid + 1;
+      if (reached(base + s)) last = mid; else first = mid + 1;
     }
-    return lo;
+    return first;
   };
 
   // the last token that top-k and top-p keep, and whether a token is not behind it
@@ -333,102 +367,127 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   }
   if (p.top_p < 1.0) {
     u64 total = 0;
-    each([&](int idx, float z) {
-      const int b = bin_of(z);
-      if (b < NBIN - 1 && upto(z, idx)) { const u64 m = mass_of(weight(z)); total += m; atomicAdd(&s_mass[b], m); }
-    });
+    auto add = [&](float z) {
+      const float far = far_of(z);
+      if (far < (float)(NBIN - 1)) { const u64 m = mass_of(weight(z)); total += m; atomicAdd(&s_mass[(int)far], m); }
+    };
+    if (cut_k) each([&](int idx, float z) { if (upto(z, idx)) add(z); });
+    else each([&](int, float z) { add(z); });
     total = block_sum64(total, s_red, tid);
     const double goal = p.top_p * (double)total;
     const auto reached = [&](u64 s) { return (double)s >= goal; };
     find_bin([&](int b) { return s_mass[b]; }, reached);
     set_thr(resolve(upto, [&](float z) { return mass_of(weight(z)); }, reached));
     __syncthreads();
-    clear();
   }
 
-  auto kept = [&](float z, int idx) -> u64 {
-    if (idx >= V || !upto(z, idx)) return 0;
-    const double w = weight(z);
-    return w >= min_w ? mass_of(w) : 0;
-  };
-  // Kept mass of each segment of 256 consecutive tokens (one wave of one pass), segments in index order: [nj][16] <= 512.  The comparison runs over all
-  // tokens, the exponential only over those that passed it (a thread walks its own, eight passes at a time), the masses of one pass of a thread go to
-  // the segment at once.
-  u64* const seg = s_mass;
-#pragma unroll 1
-  for (int j0 = 0; j0 < nj; j0 += 8) {
-    uint32_t pass = 0;
-#pragma unroll 1
-    for (int j = j0; j < min(nj, j0 + 8); ++j) {
-      float z[4];
-      get(j, z);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { const int idx = j * STEP + tid * 4 + i; pass |= idx < V && upto(z[i], idx) ? 1u << ((j - j0) * 4 + i) : 0u; }
-    }
-    u64 own = 0;
-    while (pass) {
-      const int b = __builtin_ctz(pass), j = j0 + (b >> 2);
-      pass &= pass - 1;
-      const double w = weight(one(j * STEP + tid * 4 + (b & 3)));
-      own += w >= min_w ? mass_of(w) : 0;
-      if (!pass || j0 + (__builtin_ctz(pass) >> 2) != j) { atomicAdd(&seg[j * (NT / 64) + wave], own); own = 0; }
-    }
-  }
-  __syncthreads();
-  // the segment in which the running mass passes u * total (one wave: up to 512 segments, eight per lane), else the last one with any mass
-  const int nseg = nj * (NT / 64);
-  if (wave == 0) {
-    u64 own = 0;
-    for (int i = 0; i < 8; ++i) { const int sgi = lane * 8 + i; if (sgi < nseg) own += seg[sgi]; }
-    const u64 inc = wave_scan64(own, lane);
-    const u64 total = (u64)__shfl((long long)inc, 63, 64);
-    const double goal = u * (double)total;
-    u64 run = inc - own;
+  // a token that carries mass at all and is not behind the threshold
+  auto kept = [&](float z, int idx) { return far_of(z) < (float)(NBIN - 1) && upto(z, idx); };
+  auto mass_kept = [&](float z) -> u64 { const double w = weight(z); return w >= min_w ? mass_of(w) : 0; };
+  // of the masses m[] of eight consecutive tokens or segments of this lane with `pre` before them: the first one at which the running mass passes the
+  // goal, else (u = 1) the last one with any mass; one lane of the wave gets it
+  auto pick8 = [&](const u64 (&m)[8], u64 pre, double goal, int& at, u64& before) -> bool {
     int found = -1, last = -1;
-    u64 fpre = 0, lpre = 0;
+    u64 run = pre, fpre = 0, lpre = 0;
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int sgi = lane * 8 + i;
-      const u64 m = sgi < nseg ? seg[sgi] : 0;
-      if (m > 0) { last = sgi; lpre = run; }
-      if (found < 0 && m > 0 && (double)(run + m) > goal) { found = sgi; fpre = run; }
-      run += m;
-    }
-    const u64 any = __ballot(found >= 0), have = __ballot(last >= 0);
-    const int src = any ? __builtin_ctzll(any) : 63 - __builtin_clzll(have);
-    if (lane == src) { s_bin = any ? found : last; s_base = any ? fpre : lpre; s_thr = total; }
-  }
-  __syncthreads();
-  const int sg = s_bin, sj = sg / (NT / 64);
-  if (wave == sg % (NT / 64)) {
-    const u64 total = s_thr;
-    const double goal = u * (double)total;
-    float z[4];
-    get(sj, z);
-    u64 m[4], own = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { m[i] = kept(z[i], sj * STEP + tid * 4 + i); own += m[i]; }
-    u64 run = s_base + wave_scan64(own, lane) - own;
-    int found = -1, last = -1;
-    float fz = 0.f, lz = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (m[i] > 0) { last = sj * STEP + tid * 4 + i; lz = z[i]; }
-      if (found < 0 && m[i] > 0 && (double)(run + m[i]) > goal) { found = sj * STEP + tid * 4 + i; fz = z[i]; }
+      if (m[i] > 0) { last = i; lpre = run; }
+      if (found < 0 && m[i] > 0 && (double)(run + m[i]) > goal) { found = i; fpre = run; }
       run += m[i];
     }
     const u64 any = __ballot(found >= 0), have = __ballot(last >= 0);
-    const int src = any ? __builtin_ctzll(any) : 63 - __builtin_clzll(have);
-    if (lane == src) finish(any ? found : last, log_prob(any ? fz : lz, total));
+    at = any ? found : last;
+    before = any ? fpre : lpre;
+    return lane == (any ? __builtin_ctzll(any) : 63 - __builtin_clzll(have));
+  };
+  if constexpr (ROW) {
+    // mass of each thread's consecutive tokens: the comparison runs over all of them, the exponential only over those that passed it
+    uint32_t pass = 0;
+#pragma unroll 1
+    for (int j = 0; j < nj; ++j) {
+      float z[4];
+      get(j, z);
+      const int idx = group(j) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pass |= kept(z[i], idx + i) ? 1u << (j * 4 + i) : 0u;
+    }
+    auto logit = [&](int b) { return zs[place(group(b >> 2)) * 4 + (b & 3)]; };
+    u64 own = 0;
+    for (uint32_t m = pass; m; m &= m - 1) own += mass_kept(logit(__builtin_ctz(m)));
+    const u64 inc = wave_scan64(own, lane);
+    __syncthreads();
+    if (lane == 63) s_red[wave] = inc;
+    __syncthreads();
+    u64 pre = inc - own, total = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) { const u64 x = s_red[i]; pre += i < wave ? x : 0; total += x; }
+    const double goal = u * (double)total;
+    const bool here = own > 0 && ((double)(pre + own) > goal ? !((double)pre > goal) : pre + own == total && !((double)total > goal));
+    if (here) {                             // one thread of the block
+      u64 run = pre;
+      int tok = -1;
+      float zt = 0.f;
+      for (uint32_t m = pass; m; m &= m - 1) {
+        const int b = __builtin_ctz(m);
+        const float z = logit(b);
+        const u64 x = mass_kept(z);
+        if (x > 0) {
+          run += x;
+          tok = tid * cpt * 4 + b; zt = z;
+          if ((double)run > goal) break;
+        }
+      }
+      finish(tok, log_prob(zt, total));
+    }
+  } else {
+    // mass of each segment of 256 consecutive tokens (one wave of one step), segments in index order: [nj][16] <= 512; then within the drawn one
+    __syncthreads();
+    u64* const seg = s_mass;
+    auto masses = [&](int j, float (&z)[4], u64 (&m)[8]) {
+      get(j, z);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m[i] = i < 4 && kept(z[i & 3], group(j) * 4 + i) ? mass_kept(z[i & 3]) : 0;
+    };
+#pragma unroll 1
+    for (int j = 0; j < nj; ++j) {
+      float z[4];
+      u64 m[8];
+      masses(j, z, m);
+      const u64 own = wave_sum64(m[0] + m[1] + m[2] + m[3]);
+      if (lane == 0) seg[j * (NT / 64) + wave] = own;
+    }
+    __syncthreads();
+    int at;
+    u64 before;
+    if (wave == 0) {
+      u64 m[8], own = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { m[i] = lane * 8 + i < nj * (NT / 64) ? seg[lane * 8 + i] : 0; own += m[i]; }
+      const u64 inc = wave_scan64(own, lane), total = (u64)__shfl((long long)inc, 63, 64);
+      if (pick8(m, inc - own, u * (double)total, at, before)) { s_bin = lane * 8 + at; s_base = before; s_thr = total; }
+    }
+    __syncthreads();
+    const int sj = s_bin / (NT / 64);
+    if (wave == s_bin % (NT / 64)) {
+      const u64 total = s_thr;
+      float z[4];
+      u64 m[8];
+      masses(sj, z, m);
+      const u64 own = m[0] + m[1] + m[2] + m[3];
+      if (pick8(m, s_base + wave_scan64(own, lane) - own, u * (double)total, at, before))
+        finish(group(sj) * 4 + at, log_prob(at == 0 ? z[0] : (at == 1 ? z[1] : (at == 2 ? z[2] : z[3])), total));
+    }
   }
 }
 
 template <typename T> int sample_launch(SampleP& p, int rows, hipStream_t s) {
   const int nj = (p.V + STEP - 1) / STEP;
+  p.log_cpt = nj <= 1 ? 0 : (nj <= 2 ? 1 : (nj <= 4 ? 2 : 3)); p.cpt = 1 << p.log_cpt;
   p.vec = ((uintptr_t)p.logits % (4 * sizeof(T))) == 0 && p.ld % 4 == 0;
   if (nj <= ROW_MAX) {
     static bool attr = false;
     if (!attr) { (void)hipFuncSetAttribute((const void*)sample_kernel<T, true>, hipFuncAttributeMaxDynamicSharedMemorySize, ROW_MAX * STEP * 4); attr = true; }
-    hipLaunchKernelGGL((sample_kernel<T, true>), dim3(rows), dim3(NT), (size_t)nj * STEP * 4, s, p);
+    hipLaunchKernelGGL((sample_kernel<T, true>), dim3(rows), dim3(NT), (size_t)p.cpt * STEP * 4, s, p);
   } else {
     hipLaunchKernelGGL((sample_kernel<T, false>), dim3(rows), dim3(NT), 0, s, p);
   }
