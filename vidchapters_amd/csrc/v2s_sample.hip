@@ -63,16 +63,20 @@ __device__ __forceinline__ double exp2_mass(double t, const double* tab) {
 }
 // round to nearest: 2^46 w < 2^52, so the sum holds it in its low bits
 __device__ __forceinline__ u64 mass_of(double w46) { return (u64)__double_as_longlong(w46 + 4503599627370496.0) & 0xfffffffffffffull; }
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += (u64)__shfl_xor((long long)v, o, 64);
-  return v;
+// scan and sum of a wave by row shifts and row broadcasts of the vector unit (a shuffle through LDS costs five times the latency a step)
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t lane_step(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 lane_step(u64 v) {
+  return (u64)lane_step<CTRL, ROWS>((uint32_t)v) | ((u64)lane_step<CTRL, ROWS>((uint32_t)(v >> 32)) << 32);
 }
-__device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {      // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const u64 w = (u64)__shfl_up((long long)v, o, 64); if (lane >= o) v += w; }
-  return v;
+template <typename U> __device__ __forceinline__ U wave_scan(U v) {       // inclusive
+  v += lane_step<0x111, 0xf>(v); v += lane_step<0x112, 0xf>(v); v += lane_step<0x114, 0xf>(v); v += lane_step<0x118, 0xf>(v);      // row_shr 1, 2, 4, 8
+  v += lane_step<0x142, 0xa>(v);                                          // the last lane of row 0 to row 1, of row 2 to row 3
+  return v + lane_step<0x143, 0xc>(v);                                    // lane 31 to the rows 2 and 3
 }
+__device__ __forceinline__ u64 last_lane(u64 v) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63) | ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32);
+}
+__device__ __forceinline__ u64 wave_sum64(u64 v) { return last_lane(wave_scan(v)); }
 __device__ u64 block_sum64(u64 v, u64* red, int tid) {
   v = wave_sum64(v);
   __syncthreads();
@@ -236,8 +240,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
 
   // bin of the boundary: the first one at which the running sum (of counts or masses) reaches the goal; s_base = the sum before it
   auto find_bin = [&](auto value, auto reached) {
-    const u64 a = value(2 * tid), b = value(2 * tid + 1);
-    const u64 inc = wave_scan64(a + b, lane);
+    const auto a = value(2 * tid), b = value(2 * tid + 1);
+    const auto inc = wave_scan(a + b);
     __syncthreads();
     if (lane == 63) s_red[wave] = inc;
     if (tid == 0) { s_bin = NBIN - 1; s_n = 0; }
@@ -259,16 +263,23 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     if (b0 < NBIN - 1) atomicAdd(&s_cnt[b0], 1u);
     __syncthreads();
     const u64 k = (u64)p.top_k;
-    find_bin([&](int b) { return (u64)s_cnt[b]; }, [&](u64 s) { return s >= k; });
+    find_bin([&](int b) { return s_cnt[b]; }, [&](u64 s) { return s >= k; });
     const int bin = s_bin;
     if (bin < NBIN - 1) {
       const float limit = (float)(bin + 1);
-      each([&](int idx, float z) {
-        if (far_of(z) < limit) {
-          const int at = atomicAdd(&s_n, 1);
-          if (at < SMALL_N) s_key[at] = order_key(z, idx);
+#pragma unroll 2
+      for (int j = 0; j < nj; ++j) {
+        float z[4];
+        get(j, z);
+        if (far_of(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]))) < limit) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (far_of(z[i]) < limit) {
+              const int at = atomicAdd(&s_n, 1);
+              if (at < SMALL_N) s_key[at] = order_key(z[i], group(j) * 4 + i);
+            }
         }
-      });
+      }
       __syncthreads();
       const int n = s_n, n8 = (n + 7) & ~7;
       if (n >= p.top_k && n <= SMALL_N) {   // the same for the whole block
@@ -308,19 +319,33 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     clear();
   }
 
-  // the last kept token of the boundary's bin, as an order key: the first one at which the running sum of `value` over the bin's tokens in order
-  // reaches the goal.  `in` = tokens that take part at all
+  // The last kept token of the boundary's bin, as an order key: the first one at which the running sum of `value` over the bin's tokens in order reaches
+  // the goal; `in` = tokens that take part at all.  On the way the thread's tokens that take part are told apart (ROW, a bit each): those in the bins
+  // before the boundary's, and those in it.
+  uint32_t sure = 0, maybe = 0;
   auto resolve = [&](auto in, auto value, auto reached) -> u64 {
-    const int bin = s_bin;
     const u64 base = s_base;
-    const float lo = (float)bin, hi = (float)(bin + 1);
-    each([&](int idx, float z) {
-      const float far = far_of(z);
-      if (far >= lo && far < hi && in(z, idx)) {
-        const int at = atomicAdd(&s_n, 1);
-        if (at < CAP) { s_key[at] = order_key(z, idx); s_w[at] = value(z); }
+    const float lo = (float)s_bin, hi = (float)(s_bin + 1);
+    sure = maybe = 0;
+#pragma unroll 1
+    for (int j = 0; j < nj; ++j) {
+      float z[4];
+      get(j, z);
+      const int idx = group(j) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float far = far_of(z[i]);
+        if (far < hi && in(z[i], idx + i)) {
+          if (far < lo) {
+            if constexpr (ROW) sure |= 1u << (j * 4 + i);
+          } else {
+            if constexpr (ROW) maybe |= 1u << (j * 4 + i);
+            const int at = atomicAdd(&s_n, 1);
+            if (at < CAP) { s_key[at] = order_key(z[i], idx + i); s_w[at] = value(z[i]); }
+          }
+        }
       }
-    });
+    }
     __syncthreads();
     const int n = s_n, n8 = (n + 7) & ~7;
     if (n <= CAP) {
@@ -355,13 +380,16 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   int thr_i = V;
   auto upto = [&](float z, int idx) { return z > thr_z || (z == thr_z && idx <= thr_i); };
   auto set_thr = [&](u64 key) { thr_z = key_logit(key); thr_i = (int)(uint32_t)key; };
+  bool told = false;                        // sure and maybe describe the final cut
   if (cut_k) {
     each([&](int, float z) { const int b = bin_of(z); if (b < NBIN - 1) atomicAdd(&s_cnt[b], 1u); });
     __syncthreads();
     const u64 k = (u64)p.top_k;
-    find_bin([&](int b) { return (u64)s_cnt[b]; }, [&](u64 s) { return s >= k; });
-    if (s_bin < NBIN - 1)                   // otherwise every token with any mass is among the first k
+    find_bin([&](int b) { return s_cnt[b]; }, [&](u64 s) { return s >= k; });
+    if (s_bin < NBIN - 1) {                 // otherwise every token with any mass is among the first k
       set_thr(resolve([](float, int) { return true; }, [](float) { return (u64)1; }, [&](u64 s) { return s >= k; }));
+      told = true;
+    }
     __syncthreads();
     clear();
   }
@@ -377,7 +405,9 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     const double goal = p.top_p * (double)total;
     const auto reached = [&](u64 s) { return (double)s >= goal; };
     find_bin([&](int b) { return s_mass[b]; }, reached);
-    set_thr(resolve(upto, [&](float z) { return mass_of(weight(z)); }, reached));
+    if (cut_k) set_thr(resolve(upto, [&](float z) { return mass_of(weight(z)); }, reached));
+    else set_thr(resolve([](float, int) { return true; }, [&](float z) { return mass_of(weight(z)); }, reached));
+    told = true;
     __syncthreads();
   }
 
@@ -401,20 +431,30 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     return lane == (any ? __builtin_ctzll(any) : 63 - __builtin_clzll(have));
   };
   if constexpr (ROW) {
-    // mass of each thread's consecutive tokens: the comparison runs over all of them, the exponential only over those that passed it
-    uint32_t pass = 0;
-#pragma unroll 1
-    for (int j = 0; j < nj; ++j) {
-      float z[4];
-      get(j, z);
-      const int idx = group(j) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pass |= kept(z[i], idx + i) ? 1u << (j * 4 + i) : 0u;
-    }
+    // mass of each thread's consecutive tokens: only the kept ones are weighed, two at a time (a weight is one long chain)
     auto logit = [&](int b) { return zs[place(group(b >> 2)) * 4 + (b & 3)]; };
+    uint32_t pass = sure;
+    if (told) {
+      for (uint32_t m = maybe; m; m &= m - 1) { const int b = __builtin_ctz(m); pass |= upto(logit(b), tid * cpt * 4 + b) ? m & -m : 0u; }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < nj; ++j) {
+        float z[4];
+        get(j, z);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pass |= far_of(z[i]) < (float)(NBIN - 1) ? 1u << (j * 4 + i) : 0u;
+      }
+    }
     u64 own = 0;
-    for (uint32_t m = pass; m; m &= m - 1) own += mass_kept(logit(__builtin_ctz(m)));
-    const u64 inc = wave_scan64(own, lane);
+    for (uint32_t m = pass; m;) {
+      const int b0 = __builtin_ctz(m);
+      m &= m - 1;
+      const int b1 = m ? __builtin_ctz(m) : b0;
+      const u64 x0 = mass_kept(logit(b0)), x1 = mass_kept(logit(b1));
+      own += x0 + (m ? x1 : 0);
+      m &= m - 1;
+    }
+    const u64 inc = wave_scan(own);
     __syncthreads();
     if (lane == 63) s_red[wave] = inc;
     __syncthreads();
@@ -463,7 +503,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
       u64 m[8], own = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) { m[i] = lane * 8 + i < nj * (NT / 64) ? seg[lane * 8 + i] : 0; own += m[i]; }
-      const u64 inc = wave_scan64(own, lane), total = (u64)__shfl((long long)inc, 63, 64);
+      const u64 inc = wave_scan(own), total = last_lane(inc);
       if (pick8(m, inc - own, u * (double)total, at, before)) { s_bin = lane * 8 + at; s_base = before; s_thr = total; }
     }
     __syncthreads();
@@ -474,7 +514,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
       u64 m[8];
       masses(sj, z, m);
       const u64 own = m[0] + m[1] + m[2] + m[3];
-      if (pick8(m, s_base + wave_scan64(own, lane) - own, u * (double)total, at, before))
+      if (pick8(m, s_base + wave_scan(own) - own, u * (double)total, at, before))
         finish(group(sj) * 4 + at, log_prob(at == 0 ? z[0] : (at == 1 ? z[1] : (at == 2 ? z[2] : z[3])), total));
     }
   }
