@@ -69,7 +69,7 @@ const char* v2s_last_error(void);
  *   "gemm_a4_relu"  1 (default): the persistent form also takes forward GEMMs with a ReLU or ReLU + dropout epilogue (the FFN's wi: the
  *                   dropout mask of the library's counter-based generator is recomputed inside the kernel's MFMA gaps), 0: plain epilogues only
  *   "gemm_dbg"      profiling ablations of the tiled kernels (results invalid when non-zero): 1 = no global store, 2 = no epilogue, 3 = no hand-off
- *   "gemm_q8"       kernel of v2s_gemm_q8: 0 = by size (default), 1 = few rows, 2 / 3 / 4 = 64 x 64 / 128 x 128 / 128 x 256 tiles (results do not
+ *   "gemm_q8"       kernel of v2s_gemm_q8: 0 = by size (default), 1 = few rows, 2 / 3 / 4 = 64 x 64 / 128 x 128 / 256 x 256 tiles (results do not
  *                   depend on it: the sums are exact)
  *   "fp32_io"       DEBUG: 1 = v2s_*norm_fwd/bwd, v2s_ce_bwd and v2s_attn_fwd/bwd take and return FP32 activations (attention: fp32-arithmetic
  *                   reference kernels, dense layout only); parity work against fp32 references (<= 1e-4), never set by the product path

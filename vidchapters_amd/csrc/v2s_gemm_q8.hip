@@ -404,64 +404,53 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
-// Block = 16 MT rows x 16 NT columns; its waves split K (contiguous pieces: a wave uses whole cache lines of the weight) and load fragments straight
+// Block = 16 MT rows x 16 columns; its waves split K (contiguous pieces: a wave uses whole cache lines of the weight) and load fragments straight
 // from memory, every weight byte once per 16 MT rows; the partial sums meet in LDS as integers.
-template <int WAVES, int MT, int NT>
+template <int WAVES, int MT>
 __global__ __launch_bounds__(WAVES * 64) void gemm_q8_skinny_kernel(const GemmQ8 p) {
-  constexpr int F = MT * NT, U = 3;
-  __shared__ i32x4 red[WAVES][F][64];
+  constexpr int U = 3;                  // steps asked for together
+  static_assert(MT <= WAVES, "one wave writes 16 rows");
+  __shared__ i32x4 red[WAVES][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fg = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
   const int steps = (p.K + 63) >> 6, per = (steps + WAVES - 1) / WAVES;
   const int end = min(steps, (wave + 1) * per);
-  const i8 *pa[MT], *pb[NT];
+  const i8* pa[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) pa[i] = p.A + (long)min(m0 + i * 16 + fr, p.M - 1) * p.lda;
+  const i8* pb = p.B + (long)min(n0 + fr, p.N - 1) * p.ldb;
+  i32x4 acc[MT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) pb[j] = p.B + (long)min(n0 + j * 16 + fr, p.N - 1) * p.ldb;
-  i32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
   for (int s = wave * per; s < end; s += U) {
-    i32x4 a[U][MT], b[U][NT];
+    i32x4 a[U][MT], b[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = (s + u) * 64 + fg * 16;
       const bool ok = s + u < end && k < p.K;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) { b[u][j] = i32x4{0, 0, 0, 0}; if (ok) b[u][j] = *reinterpret_cast<const i32x4*>(pb[j] + k); }
+      b[u] = i32x4{0, 0, 0, 0};
+      if (ok) b[u] = *reinterpret_cast<const i32x4*>(pb + k);
 #pragma unroll
       for (int i = 0; i < MT; ++i) { a[u][i] = i32x4{0, 0, 0, 0}; if (ok) a[u][i] = *reinterpret_cast<const i32x4*>(pa[i] + k); }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[u][j], a[u][i], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[u], a[u][i], acc[i], 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) red[wave][i * NT + j][lane] = acc[i][j];
+  for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];
   __syncthreads();
+  if (wave >= MT) return;
+  i32x4 v = red[0][wave][lane];
 #pragma unroll
-  for (int q = 0; q < (F + WAVES - 1) / WAVES; ++q) {
-    const int f = q * WAVES + wave;
-    if (f >= F) break;
-    i32x4 v = red[0][f][lane];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += red[w][f][lane];
-    const int m = m0 + f / NT * 16 + fr, n = n0 + f % NT * 16 + fg * 4;
-    if (m < p.M && n < p.N) {
-      const float sa = p.alpha * p.sA[m];
-      float x[4] = {(float)v[0] * sa, (float)v[1] * sa, (float)v[2] * sa, (float)v[3] * sa};
-      finish4(p, x, cols<4>(p, n), m, n);
-    }
-  }
+  for (int w = 1; w < WAVES; ++w) v += red[w][wave][lane];
+  const int m = m0 + wave * 16 + fr, n = n0 + fg * 4;
+  if (m >= p.M || n >= p.N) return;
+  const float sa = p.alpha * p.sA[m];
+  float x[4] = {(float)v[0] * sa, (float)v[1] * sa, (float)v[2] * sa, (float)v[3] * sa};
+  finish4(p, x, cols<4>(p, n), m, n);
 }
 
 template <class G, int EPI> int tile_launch(GemmQ8& p, hipStream_t s) {
@@ -481,8 +470,8 @@ template <class G> int tile_any(GemmQ8& p, bool plain, hipStream_t s) {
   if (!plain) return tile_launch<G, EPI_ANY>(p, s);
   return p.residual ? tile_launch<G, EPI_RESIDUAL>(p, s) : tile_launch<G, EPI_PLAIN>(p, s);
 }
-template <int WAVES, int MT, int NT> int skinny_launch(const GemmQ8& p, hipStream_t s) {
-  hipLaunchKernelGGL((gemm_q8_skinny_kernel<WAVES, MT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, s, p);
+template <int WAVES, int MT> int skinny_launch(const GemmQ8& p, hipStream_t s) {
+  hipLaunchKernelGGL((gemm_q8_skinny_kernel<WAVES, MT>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, s, p);
   V2S_LAUNCH_CHECK();
   return V2S_OK;
 }
@@ -507,19 +496,23 @@ extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   // Rounds of the chip's blocks times the time of one (us, n = stages of 128): 256 x 256 tiles 6.5 + 1.5 n, 128 x 128 3.0 + 0.95 n, 64 x 64 1.9 + 0.66 n, fitted to
   // N = 2304, K = 16 .. 3200: at K = 768, M = 1000 / 2000 / 8000 / 27501 they take 14.4 / 14.5 / 32.1 / 64.9, 8.0 / 10.1 / 22.5 / 70.7 and 7.3 / 10.1 / 27.2 / 108 us.
-  // Up to 64 rows a launch is bound by the latency of its weights, and the few-row kernels ask for all of them at once (64 x 2304 x 768: 4.4 us, 64 x 64 tiles 5.2).
+  // Up to 64 rows a launch is bound by the latency of its weights, and the few-row kernels ask for all of them at once (64 x 2304 x 768: 4.3 us, 64 x 64 tiles
+  // 4.6; 16 x 6000 x 1024: 4.2 and 5.4), until the rows read again for every 16 columns outweigh that (64 x 5000 x 768: 6.1 and 5.1, 64 x 32228 x 768: 18.5 and 9.5).
   auto rounds = [&](int t, int slots) { return (double)(((int64_t)((p.M + t - 1) / t) * ((p.N + t - 1) / t) + slots - 1) / slots); };
   const double n = (p.K + 127) / 128;
   const double t4 = rounds(256, 256) * (6.5 + 1.5 * n), t3 = rounds(128, 512) * (3.0 + 0.95 * n), t2 = rounds(64, 1024) * (1.9 + 0.66 * n);
   int kind = v2s_opt_gemm_q8();
   const bool plain = !p.c_f32 && p.act != V2S_ACT_GELU;
-  if (kind == 0) kind = p.M <= 64 ? 1 : (plain && t4 <= t3 && t4 <= t2 ? 4 : (t3 <= t2 ? 3 : 2));
+  if (kind == 0) kind = p.M <= 64 && (int64_t)p.M * p.N <= 1 << 18 ? 1 : (plain && t4 <= t3 && t4 <= t2 ? 4 : (t3 <= t2 ? 3 : 2));
   if (kind == 4 && plain) return p.residual ? tile_launch<Tile256, EPI_RESIDUAL>(p, s) : tile_launch<Tile256, EPI_PLAIN>(p, s);
   if (kind >= 3) return tile_any<Tile128>(p, plain, s);
   if (kind == 2) return tile_any<Tile64>(p, plain, s);
-  const bool wide = p.N >= 8192, deep = p.K > 1024;
-  V2S_CHECK((p.M + 15) / 16 <= 65535, V2S_ERR_SHAPE, "v2s_gemm_q8: too many rows for the few-row kernels");
-  if (p.M <= 16) return deep ? skinny_launch<8, 1, 1>(p, s) : (wide ? skinny_launch<4, 1, 4>(p, s) : skinny_launch<4, 1, 1>(p, s));
-  if (p.M <= 32) return deep ? skinny_launch<8, 2, 1>(p, s) : (wide ? skinny_launch<4, 2, 4>(p, s) : skinny_launch<4, 2, 1>(p, s));
-  return deep ? skinny_launch<8, 4, 1>(p, s) : (wide ? skinny_launch<4, 4, 4>(p, s) : skinny_launch<4, 4, 1>(p, s));
+  const bool deep = p.K > 1024;
+  const int64_t mb = (p.M + 15) / 16, nb = (p.N + 15) / 16;
+  V2S_CHECK(mb <= 65535, V2S_ERR_SHAPE, "v2s_gemm_q8: too many rows for the few-row kernels");
+  // rows of one block: 16 as long as that leaves the chip under two blocks per CU (64 x 1024 x 4096: 6.2 us, 64 rows 11.7), as many as there are otherwise
+  // (64 x 4096 x 4096: 17 and 12 us)
+  if (mb == 1 || mb * nb < 512) return deep ? skinny_launch<8, 1>(p, s) : skinny_launch<4, 1>(p, s);
+  if (mb == 2) return deep ? skinny_launch<8, 2>(p, s) : skinny_launch<4, 2>(p, s);
+  return deep ? skinny_launch<8, 4>(p, s) : skinny_launch<4, 4>(p, s);
 }

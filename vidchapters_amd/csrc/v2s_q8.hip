@@ -35,6 +35,16 @@ __device__ __forceinline__ void q8_unpack4(uint32_t u, float* f) {
   f[0] = (float)(i8)(u & 255u); f[1] = (float)(i8)((u >> 8) & 255u); f[2] = (float)(i8)((u >> 16) & 255u); f[3] = (float)(i8)(u >> 24);
 }
 
+// eight values rounded to bf16 by v_cvt_pk_bf16_f32
+__device__ __forceinline__ uint4 round8(const float* f) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{f[2 * i], f[2 * i + 1]}), bf16x2));
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 // ---- rows -> codes ----------------------------------------------------------------------------------------------------------------------
 struct RowsQ8 {
   const void* x; long ldx;
@@ -84,7 +94,7 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
           ld8(p.delta + (long)row * p.ldd + c * 8, d);
 #pragma unroll
           for (int j = 0; j < 8; ++j) d[j] += v[i][j];
-          const uint4 s = pack8(d);           // the residual stream is bf16: the norm sees the value that the next layer will read
+          const uint4 s = round8(d);           // the residual stream is bf16: the norm sees the value that the next layer will read
           unpack8(s, v[i]);
           if (p.h) *reinterpret_cast<uint4*>(p.h + (long)row * p.ldh + c * 8) = s;
         }
@@ -138,7 +148,7 @@ __global__ __launch_bounds__(256) void dequant_q8_kernel(const i8* __restrict__ 
   q8_unpack4(u.x, f); q8_unpack4(u.y, f + 4);
 #pragma unroll
   for (int j = 0; j < 8; ++j) f[j] *= s;
-  *reinterpret_cast<uint4*>(y + (long)row * ldy + c * 8) = pack8(f);
+  *reinterpret_cast<uint4*>(y + (long)row * ldy + c * 8) = round8(f);
 }
 
 // ---- key / value cache --------------------------------------------------------------------------------------------------------------------
@@ -217,7 +227,7 @@ __global__ __launch_bounds__(256) void kv_read_q8_kernel(const KvQ8 p) {
     q8_unpack4(u.x, f); q8_unpack4(u.y, f + 4);
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] *= s;
-    *reinterpret_cast<uint4*>((w ? p.v : p.k) + dst) = pack8(f);
+    *reinterpret_cast<uint4*>((w ? p.v : p.k) + dst) = round8(f);
   }
 }
 
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
   const i8 *kq = p.kq + base * 64, *vq = p.vq + base * 64;
   const float *ks = p.ks + base, *vs = p.vs + base;
   const float* bias = nullptr;
-  if (p.bias) bias = p.bias + (long)h * p.bias_ld + k0 + (p.pos_dev ? p.bias_maxlen - 1 - *p.pos_dev : 0);
+  if (p.bias) bias = p.bias + (long)h * p.bias_ld + k0 + (p.pos_dev ? p.bias_maxlen - 1 - min(*p.pos_dev, p.bias_maxlen - 1) : 0);
 
   if (tid == 0) s_any = 0;
   __syncthreads();
@@ -390,12 +400,12 @@ __global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
         w[i] = x * sv[i];
       }
       uint4 hi, lo;
-      hi = pack8(w);
+      hi = round8(w);
       float hf[8];
       unpack8(hi, hf);
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] -= hf[i];
-      lo = pack8(w);
+      lo = round8(w);
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
         typedef __attribute__((ext_vector_type(2))) int i32x2;
@@ -465,7 +475,7 @@ __global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {
   const i8 *kq = p.kq + base * 64, *vq = p.vq + base * 64;
   const float *ks = p.ks + base, *vs = p.vs + base;
   const float* bias = nullptr;
-  if (p.bias) bias = p.bias + (long)h * p.bias_ld + k0 + (p.pos_dev ? p.bias_maxlen - 1 - *p.pos_dev : 0);
+  if (p.bias) bias = p.bias + (long)h * p.bias_ld + k0 + (p.pos_dev ? p.bias_maxlen - 1 - min(*p.pos_dev, p.bias_maxlen - 1) : 0);
   float qv[16];
   const long qr = (long)e * p.q_bs + h * 64 + c * 16;
   ld8(p.q + qr, qv); ld8(p.q + qr + 8, qv + 8);

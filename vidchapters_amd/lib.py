@@ -795,6 +795,11 @@ def _strided(t, dtype, dev: int, what: str, need: int):
     return t.data_ptr()
 
 
+def _view(t, dtype, dev: int, what: str):
+    """Address of an operand whose shape and strides the caller has looked at: its view covers what is read or written."""
+    return t.data_ptr() if t.dtype is dtype and t.get_device() == dev else _strided(t, dtype, dev, what, 0)
+
+
 def quant_rows_q8(x, q, scale, rows, cols, *, ldx=None, ldq=None):
     """int8 codes ``q`` [rows, ldq] and one fp32 scale per row of the rows of ``x`` (bf16 or fp32): weights once, activations per token."""
     ldx, ldq, dev, f32 = ldx or cols, ldq or cols, _device(x), x.dtype is _F32
@@ -850,18 +855,19 @@ def _kv_q8(kq, ks, vq, vs, dev: int, what: str) -> KvQ8:
     if one != 1 or vs.stride() != strides or kq.stride() != (e * 64, h * 64, 64, 1) or vq.stride() != (e * 64, h * 64, 64, 1):
         raise ValueError(f"{what}: codes and scales of a cache share their row strides, the rows of a head are contiguous")
     c.entries, c.heads, c.maxlen, c.e_rows, c.h_rows = shape[0], shape[1], shape[2], e, h
-    c.k, c.ks = _operand(kq, _I8, dev, what + " k"), _operand(ks, _F32, dev, what + " ks")
-    c.v, c.vs = _operand(vq, _I8, dev, what + " v"), _operand(vs, _F32, dev, what + " vs")
+    c.k, c.ks, c.v, c.vs = _view(kq, _I8, dev, what), _view(ks, _F32, dev, what), _view(vq, _I8, dev, what), _view(vs, _F32, dev, what)
     return c
 
 
 def _kv_move(fn, name: str, k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count):
     dev = _device(kq)
     c = _kv_q8(kq, ks, vq, vs, dev, name)
-    shape, (bs, rs, _) = k.shape, k.stride()
-    if v.shape != shape or shape[0] != c.entries or shape[1] < T or shape[2] < c.heads * 64 or v.stride() != k.stride():
+    shape, (bs, rs, one) = k.shape, k.stride()
+    if v.shape != shape or shape[0] != c.entries or shape[1] < T or shape[2] < c.heads * 64 or v.stride() != (bs, rs, 1):
         raise ValueError(f"{name}: k and v are [{c.entries}, >= {T}, >= {c.heads * 64}] with the same strides, got {tuple(shape)} and {tuple(v.shape)}")
-    _check(fn(C.byref(c), _operand(k, _BF16, dev, name + " k"), _operand(v, _BF16, dev, name + " v"), bs, rs, T, pos0,
+    if one != 1:
+        raise ValueError(f"{name}: the last dimension of k and v must be contiguous")
+    _check(fn(C.byref(c), _view(k, _BF16, dev, name), _view(v, _BF16, dev, name), bs, rs, T, pos0,
               _operand(pos, _I32, dev, name + " pos", c.entries), _operand(pos_dev, _I32, dev, name + " pos_dev", 1),
               _operand(count, _I32, dev, name + " count", c.entries), _raw_stream(dev)), "v2s_" + name)
 
