@@ -144,7 +144,7 @@ def test_gemm_q8(M, N, K, out):
         assert (C[:M, N:] == 7).all() and (C[M:] == 7).all()      # nothing outside the product is written
 
 
-@pytest.mark.parametrize("kind", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("kind", [1, 2, 3, 4], ids=["few_rows", "64x64", "128x128", "256x256"])
 @pytest.mark.parametrize("M,N,K", [(1, 8, 16), (70, 300, 48), (130, 257, 112), (300, 520, 64), (257, 513, 1040), (128, 512, 4096), (513, 769, 784)])
 def test_gemm_q8_every_kernel_gives_the_same_bits(M, N, K, kind):
     A, sa = codes(M, K, 3)
@@ -161,6 +161,25 @@ def test_gemm_q8_every_kernel_gives_the_same_bits(M, N, K, kind):
         L.set_option("gemm_q8", 0)
     assert torch.equal(C, auto) and (C[M:] == 0).all()
     assert ((C[:M, :N].double() - want).abs() <= mag * 7 * U32 + want.abs() * UBF).all()
+
+
+@pytest.mark.parametrize("kind", [2, 3, 4], ids=["64x64", "128x128", "256x256"])
+@pytest.mark.parametrize("out,act,res", [(BF, L.ACT_RELU, False), (BF, L.ACT_NONE, True), (BF, L.ACT_GELU, True), (torch.float32, L.ACT_NONE, False)])
+def test_gemm_q8_more_tiles_than_blocks(kind, out, act, res):
+    """A block that takes several tiles, with every form of the write-out and rows and columns left over."""
+    M, N, K = 5100, 4104, 144
+    A, sa = codes(M, K, 13)
+    B, sb = codes(N, K, 14)
+    bias, r = rnd(N, seed=5, dtype=torch.float32), rnd(M, N, seed=6) if res else None
+    C = torch.full((M + 1, N), 7.0, dtype=out, device=DEV)
+    L.set_option("gemm_q8", kind)
+    try:
+        L.gemm_q8(A, B, sa, sb, C, M, N, K, bias=bias, act=act, residual=r)
+    finally:
+        L.set_option("gemm_q8", 0)
+    want, mag = product_ref(A, B, sa, sb, 1.0, bias, act, r)
+    tol = mag * (7 if act != L.ACT_GELU else 16) * U32 + want.abs() * (UBF if out == BF else 0)
+    assert ((C[:M].double() - want).abs() <= tol).all() and (C[M:] == 7).all()
 
 
 def test_gemm_q8_codes_are_summed_exactly():
@@ -381,6 +400,23 @@ def test_decode_attn_q8_counter_bias_and_batch_independence():
         assert torch.equal(alone, o[2:3])
 
 
+def test_decode_attn_q8_counter_behind_the_range():
+    """A counter that ran past the keys: all of them, and the last position's bias row at most; a negative one: no keys."""
+    E, G, H, n, top = 3, 2, 2, 90, 100
+    cache = make_cache(E, H, n, 6)
+    diag = rnd(H, 2 * top - 1, seed=7, dtype=torch.float32)
+    for G in (1, 2):
+        q = rnd(E * G, H * 64, seed=5)
+        for t in (95, 99, 100, 5000, 2**31 - 2, -1, -7):
+            o = attend(q, cache, n, group=G, pos_dev=torch.tensor([t], dtype=torch.int32, device=DEV), bias_row=diag, bias_maxlen=top)
+            if t < 0:
+                assert (o == 0).all()
+                continue
+            row = diag[:, top - 1 - min(t, top - 1):][:, :n].contiguous()
+            want, tol = attn_ref(q, *cache, 1.0, G, None, None, row)
+            assert ((o.double() - want).abs() <= tol).all()
+
+
 def test_decode_attn_q8_cache_views_behind_2_31_bytes():
     """A long cache whose later entries start behind 2^31 codes, as views of a larger one."""
     E, H, n = 3, 1, 12_000_000
@@ -510,3 +546,141 @@ def test_sample_step_frequencies():
     p = torch.softmax(z[0].double() / 0.7, 0)
     f = torch.bincount(tok, minlength=V).double() / n
     assert ((f - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all()
+
+
+# --------------------------------------------------------------------------------------------- the operators together
+class Block:
+    """One decoder layer and a head over an int8 cache, as a serving loop strings the operators together; every intermediate stays readable."""
+
+    def __init__(self, B, H, ffn, V, maxlen, steps):
+        d = self.d = H * 64
+        self.B, self.H, self.ffn, self.V, self.n = B, H, ffn, V, maxlen
+        self.w = {}
+        for i, (name, rows, cols) in enumerate((("qkv", 3 * d, d), ("out", d, d), ("up", ffn, d), ("down", d, ffn), ("head", V, d))):
+            wq, ws = torch.empty(rows, cols, dtype=torch.int8, device=DEV), torch.empty(rows, device=DEV)
+            L.quant_rows_q8(rnd(rows, cols, seed=20 + i, scale=cols ** -0.5, dtype=torch.float32), wq, ws, rows, cols)
+            self.w[name] = (wq, ws)
+        self.emb, self.g = rnd(V, d, seed=30), [1 + 0.1 * rnd(d, seed=31 + i, dtype=torch.float32) for i in range(3)]
+        self.bias = rnd(H, 2 * maxlen - 1, seed=40, dtype=torch.float32)
+        self.kv = new_cache(B, H, maxlen)
+        new = lambda *s, t=BF: torch.zeros(*s, dtype=t, device=DEV)  # noqa: E731
+        self.x, self.h1, self.h2, self.h3, self.qkv, self.o, self.up, self.logits = (new(B, d), new(B, d), new(B, d), new(B, d), new(B, 3 * d), new(B, d), new(B, ffn),
+                                                                                   new(B, (V + 7) // 8 * 8, t=torch.float32))
+        self.a, self.f = new(B, d), new(B, d)
+        self.codes = [(new(B, c, t=torch.int8), new(B, t=torch.float32)) for c in (d, d, d, ffn, d)]
+        self.tok, self.lp, self.un = new(B, t=torch.long), new(B, t=torch.float32), torch.ones(B, dtype=torch.int32, device=DEV)
+        self.seq, self.pos = new(B, maxlen + 1, t=torch.long), new(1, t=torch.int32)
+        self.u = torch.rand(steps, B, generator=torch.Generator().manual_seed(3)).to(DEV)
+        self.ws = L.decode_attn_q8_workspace(B, H, maxlen, DEV)
+        self.ctr = new(1, t=torch.int32)
+
+    def product(self, i, name, out, N, K, **kw):
+        L.gemm_q8(self.codes[i][0], self.w[name][0], self.codes[i][1], self.w[name][1], out, self.B, N, K, **kw)
+
+    def prefill(self, T):
+        kv = rnd(self.B, T, 2 * self.d, seed=50)
+        L.kv_append_q8(kv[:, :, :self.d], kv[:, :, self.d:], *self.kv, T)
+        self.pos.fill_(T)
+        self.ctr.zero_()
+        self.tok.copy_(torch.arange(self.B, device=DEV))
+
+    def step(self):
+        B, d, c = self.B, self.d, self.codes
+        self.x.copy_(self.emb[self.tok])
+        L.rmsnorm_q8(self.x, self.g[0], *c[0], B, d, 1e-6, h=None)
+        self.product(0, "qkv", self.qkv, 3 * d, d)
+        q, k, v = self.qkv[:, :d], self.qkv[:, None, d:2 * d], self.qkv[:, None, 2 * d:]
+        L.kv_append_q8(k, v, *self.kv, 1, pos_dev=self.pos)
+        L.decode_attn_q8(q, *self.kv, self.o, self.n, pos_dev=self.pos, bias_row=self.bias, bias_maxlen=self.n, workspace=self.ws)
+        L.quant_rows_q8(self.o, *c[1], B, d)
+        self.product(1, "out", self.a, d, d)
+        L.rmsnorm_q8(self.x, self.g[1], *c[2], B, d, 1e-6, delta=self.a, h=self.h1)
+        self.product(2, "up", self.up, self.ffn, d, act=L.ACT_RELU)
+        L.quant_rows_q8(self.up, *c[3], B, self.ffn)
+        self.product(3, "down", self.h2, d, self.ffn, residual=self.h1)
+        L.rmsnorm_q8(self.h2, self.g[2], *c[4], B, d, 1e-6)
+        self.product(4, "head", self.logits, self.V, d, ldc=self.logits.shape[1])
+        L.sample_step(self.logits, B, self.V, self.u, self.tok, ld=self.logits.shape[1], temperature=0.8, top_k=40, top_p=0.95, logp=self.lp, unfinished=self.un,
+                      seq_out=self.seq, seq_ld=self.n + 1, pos_dev=self.ctr)
+        self.pos.add_(1)
+        self.ctr.add_(1)
+
+    def state(self):
+        return [t.clone() for t in (*self.kv, self.o, self.h1, self.h2, self.logits, self.tok, self.lp, self.seq)]
+
+
+def test_operators_together_match_their_formulas():
+    """Every value of two steps from the values in front of it; the second step reads what the first wrote into the cache."""
+    b = Block(3, 2, 200 // 8 * 16, 500, 1500, 2)
+    b.prefill(1395)
+    for _ in range(2):
+        pos = int(b.pos)
+        b.step()
+        norm = lambda x, g: x.double() * torch.rsqrt((x.double() ** 2).mean(1, keepdim=True) + 1e-6) * g.double()  # noqa: E731
+        d, slack = b.d, (b.d / 64 + 14) * U32
+        check_codes(*b.codes[0], norm(b.x, b.g[0]), slack)
+        for i, name, got, r in ((0, "qkv", b.qkv, None), (1, "out", b.a, None), (3, "down", b.h2, b.h1), (4, "head", b.logits[:, :b.V], None)):
+            want, mag = product_ref(b.codes[i][0], b.w[name][0], b.codes[i][1], b.w[name][1], 1.0, None, L.ACT_NONE, r)
+            assert ((got.double() - want).abs() <= mag * 7 * U32 + want.abs() * (UBF if name != "head" else 0)).all(), name
+        k = b.qkv[:, d:2 * d].double().reshape(-1, 64)
+        check_codes(b.kv[0][:, :, pos].reshape(-1, 64), b.kv[1][:, :, pos].reshape(-1), k, 0.0)
+        row = b.bias[:, b.n - 1 - pos:2 * b.n - 1 - pos].contiguous()
+        want, tol = attn_ref(b.qkv[:, :d], *b.kv, 1.0, 1, torch.full((b.B,), pos + 1), None, row)
+        assert ((b.o.double() - want).abs() <= tol).all()
+        check_codes(*b.codes[1], b.o.double(), 0.0)
+        s = b.x.double() + b.a.double()
+        assert ((b.h1.double() - s).abs() <= s.abs() * (UBF + U32)).all()
+        check_codes(*b.codes[2], norm(b.h1, b.g[1]), slack)
+        check_codes(*b.codes[4], norm(b.h2, b.g[2]), slack)
+        for r in range(b.B):
+            tok, lp, near = sample_ref(b.logits[r, :b.V].cpu(), float(b.u[int(b.ctr) - 1, r]), 0.8, 40, 0.95, 0.0)
+            if near > b.V * 2.0 ** -46:
+                assert int(b.tok[r]) == tok == int(b.seq[r, int(b.ctr)]) and abs(float(b.lp[r]) - lp) <= 4 * U32 * max(1.0, abs(lp)) + b.V * 2.0 ** -46
+
+
+def test_operators_together_captured_and_replayed():
+    """Two loops, each captured once and replayed in turn with eager work between the replays, give the bits of the eager loop."""
+    steps = 6
+    eager = Block(3, 2, 416, 500, 1500, steps)
+    eager.prefill(1390)
+    eager.step()                                                      # loads every kernel before the capture
+    blocks = [Block(3, 2, 416, 500, 1500, steps) for _ in range(2)]
+    graphs = []
+    for b in blocks:
+        b.prefill(1390)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            b.step()
+        graphs.append(graph)
+        b.prefill(1390)
+    for i in range(steps):
+        if i:
+            eager.step()
+        for graph, b in zip(graphs, blocks):
+            graph.replay()
+            torch.cuda.synchronize()
+            scratch = torch.randn(1000, device=DEV).sum().item()      # eager work between the replays
+            assert math.isfinite(scratch)
+            for x, y in zip(b.state(), eager.state()):
+                assert torch.equal(x, y), i
+
+
+def test_operators_on_a_side_stream():
+    """The launches go to the current stream: a loop on a stream of its own, behind that stream's work, gives the same bits."""
+    a, b = Block(2, 2, 128, 300, 1400, 2), Block(2, 2, 128, 300, 1400, 2)
+    a.prefill(1380)
+    a.step()
+    a.step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        big = torch.randn(2048, 2048, device=DEV)
+        for _ in range(20):
+            big = big @ big * 0.01                                    # the stream is busy when the loop is enqueued
+        b.prefill(1380)
+        b.step()
+        b.step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for x, y in zip(b.state(), a.state()):
+        assert torch.equal(x, y)

@@ -267,8 +267,10 @@ __device__ __forceinline__ float rescale(float m, float M) { return m == M ? 1.f
 __device__ float attn_q8_mean(const i8* vq, const float* vs, int n, float* lds) {
   const int d = threadIdx.x & 63, part = threadIdx.x >> 6;
   float s = 0.f;
-  if (part < 4)
-    for (int k = part; k < n; k += 4) s += vs[k] * (float)vq[(long)k * 64 + d];
+  if (part < 4) {
+#pragma unroll 16
+    for (int k = part; k < n; k += 4) s = fmaf(vs[k], (float)vq[(long)k * 64 + d], s);
+  }
   __syncthreads();
   if (part < 4) lds[threadIdx.x] = s;
   __syncthreads();

@@ -827,17 +827,13 @@ def dequant_q8(q, scale, y, rows, cols, *, ldq=None, ldy=None):
 
 def gemm_q8(A, B, sA, sB, C_out, M, N, K, *, lda=None, ldb=None, ldc=None, alpha=1.0, bias=None, act=ACT_NONE, residual=None, ldr=None):
     """C[M, N] = act(alpha * sA[m] * sB[n] * A(m, :) . B(n, :) + bias) + residual with int8 A (token codes) and B (weight codes [out, in])."""
-    a, dev, f32, last = GemmQ8Args(), _device(A), C_out.dtype is _F32, M - 1
+    dev, f32, last = _device(A), C_out.dtype is _F32, M - 1
     lda, ldb, ldc, ldr = lda or K, ldb or K, ldc or N, ldr or N
-    a.M, a.N, a.K, a.lda, a.ldb, a.ldc, a.ldr = M, N, K, lda, ldb, ldc, ldr
-    a.A, a.B = _operand(A, _I8, dev, "gemm_q8 A", last * lda + K), _operand(B, _I8, dev, "gemm_q8 B", (N - 1) * ldb + K)
-    a.sA, a.sB = _operand(sA, _F32, dev, "gemm_q8 sA", M), _operand(sB, _F32, dev, "gemm_q8 sB", N)
-    a.C, a.c_dtype = _operand(C_out, _F32 if f32 else _BF16, dev, "gemm_q8 C", last * ldc + N), V2S_F32 if f32 else V2S_BF16
-    a.alpha, a.act = alpha, act
-    if bias is not None:
-        a.bias = _operand(bias, _F32, dev, "gemm_q8 bias", N)
-    if residual is not None:
-        a.residual = _operand(residual, _BF16, dev, "gemm_q8 residual", last * ldr + N)
+    a = GemmQ8Args(M, N, K, _operand(A, _I8, dev, "gemm_q8 A", last * lda + K), _operand(B, _I8, dev, "gemm_q8 B", (N - 1) * ldb + K), lda, ldb,
+                   _operand(sA, _F32, dev, "gemm_q8 sA", M), _operand(sB, _F32, dev, "gemm_q8 sB", N),
+                   _operand(C_out, _F32 if f32 else _BF16, dev, "gemm_q8 C", last * ldc + N), ldc, V2S_F32 if f32 else V2S_BF16, alpha,
+                   None if bias is None else _operand(bias, _F32, dev, "gemm_q8 bias", N), act,
+                   None if residual is None else _operand(residual, _BF16, dev, "gemm_q8 residual", last * ldr + N), ldr)
     kt = KernelTimer.active
     if kt is not None:
         e0 = kt.begin()
@@ -848,28 +844,28 @@ def gemm_q8(A, B, sA, sB, C_out, M, N, K, *, lda=None, ldb=None, ldc=None, alpha
 
 def _kv_q8(kq, ks, vq, vs, dev: int, what: str) -> KvQ8:
     """The cache as four tensors: codes [entries, heads, maxlen, 64] int8 and scales [entries, heads, maxlen] fp32."""
-    c, shape = KvQ8(), kq.shape
-    if len(shape) != 4 or shape[3] != 64 or vq.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
+    rows = ks.shape
+    if len(rows) != 3 or vs.shape != rows or kq.shape != (*rows, 64) or vq.shape != (*rows, 64):
         raise ValueError(f"{what}: a cache is codes [entries, heads, maxlen, 64] and scales [entries, heads, maxlen] for keys and for values")
     e, h, one = strides = ks.stride()
-    if one != 1 or vs.stride() != strides or kq.stride() != (e * 64, h * 64, 64, 1) or vq.stride() != (e * 64, h * 64, 64, 1):
+    codes = (e * 64, h * 64, 64, 1)
+    if one != 1 or vs.stride() != strides or kq.stride() != codes or vq.stride() != codes:
         raise ValueError(f"{what}: codes and scales of a cache share their row strides, the rows of a head are contiguous")
-    c.entries, c.heads, c.maxlen, c.e_rows, c.h_rows = shape[0], shape[1], shape[2], e, h
-    c.k, c.ks, c.v, c.vs = _view(kq, _I8, dev, what), _view(ks, _F32, dev, what), _view(vq, _I8, dev, what), _view(vs, _F32, dev, what)
-    return c
+    return KvQ8(_view(kq, _I8, dev, what), _view(ks, _F32, dev, what), _view(vq, _I8, dev, what), _view(vs, _F32, dev, what), e, h, *rows)
 
 
 def _kv_move(fn, name: str, k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count):
     dev = _device(kq)
     c = _kv_q8(kq, ks, vq, vs, dev, name)
-    shape, (bs, rs, one) = k.shape, k.stride()
-    if v.shape != shape or shape[0] != c.entries or shape[1] < T or shape[2] < c.heads * 64 or v.stride() != (bs, rs, 1):
-        raise ValueError(f"{name}: k and v are [{c.entries}, >= {T}, >= {c.heads * 64}] with the same strides, got {tuple(shape)} and {tuple(v.shape)}")
+    shape, strides, E, cols = k.shape, k.stride(), c.entries, c.heads * 64
+    if len(shape) != 3 or v.shape != shape or shape[0] != E or shape[1] < T or shape[2] < cols or v.stride() != strides:
+        raise ValueError(f"{name}: k and v are [{E}, >= {T}, >= {cols}] with the same strides, got {tuple(shape)} and {tuple(v.shape)}")
+    bs, rs, one = strides
     if one != 1:
         raise ValueError(f"{name}: the last dimension of k and v must be contiguous")
     _check(fn(C.byref(c), _view(k, _BF16, dev, name), _view(v, _BF16, dev, name), bs, rs, T, pos0,
-              _operand(pos, _I32, dev, name + " pos", c.entries), _operand(pos_dev, _I32, dev, name + " pos_dev", 1),
-              _operand(count, _I32, dev, name + " count", c.entries), _raw_stream(dev)), "v2s_" + name)
+              pos if pos is None else _operand(pos, _I32, dev, name, E), pos_dev if pos_dev is None else _operand(pos_dev, _I32, dev, name, 1),
+              count if count is None else _operand(count, _I32, dev, name, E), _raw_stream(dev)), "v2s_" + name)
 
 
 def kv_append_q8(k, v, kq, ks, vq, vs, T, *, pos0=0, pos=None, pos_dev=None, count=None):
