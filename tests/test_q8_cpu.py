@@ -20,7 +20,7 @@ def test_rows_refusals():
     l = L.lib()
     ok = dict(x=P, dt=0, ldx=64, q=P, ldq=64, s=P, rows=4, cols=64)
     for change, word in ((dict(x=None), "NULL"), (dict(s=None), "NULL"), (dict(dt=7), "bf16 or fp32"), (dict(cols=60), "multiple of 8"), (dict(cols=8200, ldx=8200, ldq=8200), "8192"),
-                         (dict(rows=0), "rows=0"), (dict(ldx=56), "shorter"), (dict(ldq=63), "shorter"), (dict(ldx=68), "multiples of 8"), (dict(x=P + 2), "aligned"),
+                         (dict(rows=0), "rows=0"), (dict(rows=1 << 22, ld=100), "2^22"), (dict(ldx=56), "shorter"), (dict(ldq=63), "shorter"), (dict(ldx=68), "multiples of 8"), (dict(x=P + 2), "aligned"),
                          (dict(q=P + 4), "aligned")):
         a = {**ok, **change}
         refused(l.v2s_quant_rows_q8(a["x"], a["dt"], a["ldx"], a["q"], a["ldq"], a["s"], a["rows"], a["cols"], None), word)
@@ -59,7 +59,7 @@ def test_cache_refusals():
         def call(c=None, k=P, bs=256, rs=128, T=2):
             return fn(ctypes.byref(c if c is not None else cache()), k, P, bs, rs, T, 0, None, None, None, None)
         for kw, word in ((dict(c=cache(ks=None)), "NULL"), (dict(k=None), "NULL"), (dict(T=0), "positive"), (dict(c=cache(maxlen=0)), "positive"), (dict(c=cache(h_rows=39)), "row strides"),
-                         (dict(k=P + 8), "aligned"), (dict(rs=130), "multiples of 8"), (dict(c=cache(k=P + 8)), "aligned"), (dict(c=cache(entries=1 << 20, heads=1024), T=64), "too large")):
+                         (dict(k=P + 8), "aligned"), (dict(rs=130), "multiples of 8"), (dict(c=cache(k=P + 8)), "aligned"), (dict(c=cache(entries=1 << 20, heads=1024), T=64), "too large"), (dict(c=cache(entries=1 << 16, heads=1024), T=8), "too large")):
             refused(call(**kw), word)
         assert fn(None, P, P, 8, 8, 1, 0, None, None, None, None) < 0
 
@@ -73,7 +73,7 @@ def test_attention_refusals():
     for kw, word in ((dict(q=None), "NULL"), (dict(cache=cache(v=None)), "NULL"), (dict(B=4), "query rows"), (dict(B=3, group=2), "query rows"), (dict(Nk=41), "maxlen"), (dict(Nk=0), "positive"),
                      (dict(klen=P, pos_dev=P), "exclude"), (dict(bias_row=P, bias_ld=39), "bias"), (dict(bias_row=P, bias_ld=78, pos_dev=P, bias_maxlen=40), "bias"),
                      (dict(bias_row=P, bias_ld=200, pos_dev=P, bias_maxlen=39), "bias"), (dict(key_mask=P, mask_ld=39), "mask_ld"), (dict(q_bs=120), "shorter"), (dict(q_bs=132), "multiple of 8"),
-                     (dict(q=P + 8), "aligned")):
+                     (dict(q=P + 8), "aligned"), (dict(B=1 << 24, cache=cache(entries=1 << 24)), "too many")):
         refused(call(**kw), word)
     long = dict(cache=cache(e_rows=4000, h_rows=2000, maxlen=2000), Nk=2000)
     need = L.lib().v2s_decode_attn_q8_workspace_floats(3, 2, 2000)
@@ -87,7 +87,7 @@ def test_sample_refusals():
     nan = float("nan")
     for change, word in ((dict(z=None), "NULL"), (dict(u=None), "NULL"), (dict(dt=3), "fp32 or bf16"), (dict(V=0), "V=0"), (dict(V=200), "ld >= V"), (dict(V=131073, ld=140000), "131072"),
                          (dict(T=0.0), "temperature"), (dict(T=nan), "temperature"), (dict(k=-1), "top_k"), (dict(p=0.0), "top_p"), (dict(p=1.5), "top_p"), (dict(p=nan), "top_p"),
-                         (dict(m=-0.1), "min_p"), (dict(m=1.1), "min_p"), (dict(seq=P), "pos_dev"), (dict(pos=P), "u_steps"), (dict(pos=P, u_ld=1, us=4), "u_ld"), (dict(rows=0), "rows=0")):
+                         (dict(m=-0.1), "min_p"), (dict(m=1.1), "min_p"), (dict(seq=P), "pos_dev"), (dict(pos=P), "u_steps"), (dict(pos=P, u_ld=1, us=4), "u_ld"), (dict(rows=0), "rows=0"), (dict(rows=1 << 22, ld=100), "2^22")):
         a = {**ok, **change}
         refused(L.lib().v2s_sample_step(a["z"], a["dt"], a["ld"], a["rows"], a["V"], a["T"], a["k"], a["p"], a["m"], a["u"], a["u_ld"], a["us"], a["tok"], None, None, -1, 0,
                                         a["seq"], 5, a["pos"], 0, None), word)

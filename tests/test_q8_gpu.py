@@ -214,6 +214,30 @@ def test_gemm_q8_strides_in_place_residual_and_nan_scales():
     assert torch.equal(C[:, N:], old[:, N:])
 
 
+def test_gemm_q8_row_strides_behind_2_31_bytes():
+    """Rows of one tile that start further apart than 2^31 bytes, at the largest stride."""
+    M, N, K, ld = 256, 200, 272, 1 << 24
+    A, sa = codes(M, K, 1)
+    B, sb = codes(N, K, 2)
+    far = torch.empty((M - 1) * ld + K, dtype=torch.int8, device=DEV)
+    a = far.as_strided((M, K), (ld, 1))
+    a.copy_(A)
+    want, C = torch.empty(M, N, dtype=BF, device=DEV), torch.empty(M, N, dtype=BF, device=DEV)
+    L.gemm_q8(A, B, sa, sb, want, M, N, K)
+    for kind in (1, 2, 3, 4):
+        C.zero_()
+        L.set_option("gemm_q8", kind)
+        try:
+            L.gemm_q8(a, B, sa, sb, C, M, N, K, lda=ld)
+        finally:
+            L.set_option("gemm_q8", 0)
+        assert torch.equal(C, want), kind
+    b = far.as_strided((N, K), (ld, 1))
+    b.copy_(B)
+    L.gemm_q8(A, b, sa, sb, C, M, N, K, ldb=ld)
+    assert torch.equal(C, want)
+
+
 def test_gemm_q8_rows_do_not_depend_on_their_batch():
     """Sums are exact and the epilogue is per value: a row's result is the same bits in any call, whatever kernel the size chose."""
     M, N, K = 700, 776, 768
@@ -368,6 +392,23 @@ def test_decode_attn_q8_rows_without_keys_and_hidden_garbage():
         o = attend(q, fresh, n, group=G, bias_row=everywhere)
         want, tol = attn_ref(q, *fresh, 1.0, G, None, None, everywhere)
         assert ((o.double() - want).abs() <= tol).all()
+
+
+def test_operands_whose_storage_is_too_small_are_refused():
+    cache = make_cache(2, 1, 1300, 1)
+    q = rnd(2, 64, seed=1)
+    o = torch.empty_like(q)
+    with pytest.raises(ValueError, match="storage"):                  # 264 elements over 66 of storage
+        L.decode_attn_q8(q, *cache, o, 1300, workspace=torch.empty(1, 66, device=DEV).expand(4, 66))
+    with pytest.raises(ValueError, match="contiguous"):
+        L.decode_attn_q8(q, *cache, o, 1200, klen=torch.tensor([5], dtype=torch.int32, device=DEV).expand(2))
+    with pytest.raises(ValueError, match="storage"):
+        L.kv_append_q8(q[:, None], q[:, None], *cache, 1, pos=torch.zeros(1, dtype=torch.int32, device=DEV))
+    a, s = codes(4, 64, 1)
+    with pytest.raises(ValueError, match="storage"):
+        L.gemm_q8(a, a, s, s, torch.empty(4, 6, dtype=BF, device=DEV), 4, 4, 64, ldc=8)      # 3 * 8 + 4 = 28 over 24
+    with pytest.raises(RuntimeError, match="dtype"):
+        L.dequant_q8(a.view(torch.uint8), s, torch.empty(4, 64, dtype=BF, device=DEV), 4, 64)
 
 
 def test_decode_attn_q8_large_and_lowest_scores():

@@ -480,8 +480,8 @@ template <int WAVES, int MT> int skinny_launch(const GemmQ8& p, hipStream_t s) {
 
 extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   V2S_CHECK(a && a->A && a->B && a->sA && a->sB && a->C, V2S_ERR_ARG, "v2s_gemm_q8: NULL pointer");
-  V2S_CHECK(a->M > 0 && a->N > 0 && a->K > 0 && a->K % 16 == 0 && a->K <= 131056, V2S_ERR_SHAPE,
-            "v2s_gemm_q8: unsupported shape M=%d N=%d K=%d (K a multiple of 16, <= 131056)", a->M, a->N, a->K);
+  V2S_CHECK(a->M > 0 && a->N > 0 && a->M <= 0x7fffff00 && a->N <= 0x7fffff00 && a->K > 0 && a->K % 16 == 0 && a->K <= 131056, V2S_ERR_SHAPE,
+            "v2s_gemm_q8: unsupported shape M=%d N=%d K=%d (M, N <= 2^31 - 256, K a multiple of 16, <= 131056)", a->M, a->N, a->K);
   V2S_CHECK(a->lda >= a->K && a->ldb >= a->K && a->ldc >= a->N && (!a->residual || a->ldr >= a->N), V2S_ERR_SHAPE, "v2s_gemm_q8: a row stride is shorter than the row");
   V2S_CHECK(a->lda <= (1 << 24) && a->ldb <= (1 << 24), V2S_ERR_SHAPE, "v2s_gemm_q8: lda and ldb must be at most 2^24");
   V2S_CHECK(a->c_dtype == V2S_BF16 || a->c_dtype == V2S_F32, V2S_ERR_DTYPE, "v2s_gemm_q8: C must be bf16 or fp32");

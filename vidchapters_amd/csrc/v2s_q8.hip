@@ -1,6 +1,7 @@
 // 8-bit decoding for gfx950: rows of activations to int8 codes with one fp32 scale per row (with the residual addition and the RMSNorm in
 // front of it), the int8 key / value cache, and the single-query attention that reads it.
-//   code q and scale s of a row y:  s = max(amax|y|, 127 * 2^-126) / 127,  q = round_to_even(y / s),  so that |y - s q| <= s / 2 (1 + 2^-23)
+//   code q and scale s of a row y:  s = max(amax|y|, 127 * 2^-126) / 127,  q = round_to_even(y * (127 / amax)).  That factor and s carry four fp32 roundings
+//   in all, 127 codes times 2^-22, so that |y - s q| <= s / 2 (1 + 2^-14)
 // The floor of s keeps 1 / s finite: rows below it (1.5e-36) keep the smallest normal scale and fewer codes.  A row that holds a NaN or an
 // infinity gets s = NaN and zero codes: every value that is read back is NaN, none of them is a plausible number.
 //   RMSNorm: model/modeling_t5.py:263-277 (T5LayerNorm.forward); the cache it replaces: model/modeling_t5.py:555-556
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(256) void attn_q8_join_kernel(const AttnQ8 p) {
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 template <typename T, bool NORM> int rows_q8_launch(const RowsQ8& p, hipStream_t s) {
-  const dim3 grid((unsigned)((p.rows + 3) / 4)), block(256);
+  const dim3 grid((unsigned)((p.rows + 3) / 4)), block(256);      // rows < 2^26
   if (p.cols <= 512) hipLaunchKernelGGL((rows_q8_kernel<T, 1, NORM>), grid, block, 0, s, p);
   else if (p.cols <= 1024) hipLaunchKernelGGL((rows_q8_kernel<T, 2, NORM>), grid, block, 0, s, p);
   else if (p.cols <= 2048) hipLaunchKernelGGL((rows_q8_kernel<T, 4, NORM>), grid, block, 0, s, p);
@@ -626,7 +627,7 @@ int kv_check(const char* who, const v2s_kv_q8* c, const void* k, const void* v, 
   V2S_CHECK(aligned(c->k, 16) && aligned(c->v, 16) && aligned(k, 16) && aligned(v, 16) && aligned(c->ks, 4) && aligned(c->vs, 4) && bs % 8 == 0 && rs % 8 == 0,
             V2S_ERR_ALIGN, "%s: pointers must be 16-byte aligned and strides multiples of 8 elements", who);
   const int64_t units = (int64_t)c->entries * ((c->heads + 7) & ~7) * (((int64_t)T + 7) & ~7);
-  V2S_CHECK(units < (int64_t)0xffffff00u, V2S_ERR_SHAPE, "%s: entries x heads x T too large for one launch", who);
+  V2S_CHECK(units < 1 << 29, V2S_ERR_SHAPE, "%s: entries x heads x T too large for one launch", who);      // 2^32 threads
   return V2S_OK;
 }
 
@@ -649,7 +650,8 @@ unsigned kv_blocks(const KvQ8& p, bool tokens) {
 extern "C" int v2s_quant_rows_q8(const void* x, int32_t x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int32_t rows, int32_t cols, void* stream) {
   V2S_CHECK(x && q && scale, V2S_ERR_ARG, "v2s_quant_rows_q8: NULL pointer");
   V2S_CHECK(x_dtype == V2S_BF16 || x_dtype == V2S_F32, V2S_ERR_DTYPE, "v2s_quant_rows_q8: x must be bf16 or fp32");
-  V2S_CHECK(rows > 0 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE, "v2s_quant_rows_q8: unsupported shape rows=%d cols=%d (cols a multiple of 8, <= 8192)", rows, cols);
+  V2S_CHECK(rows > 0 && rows < 1 << 26 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE,
+            "v2s_quant_rows_q8: unsupported shape rows=%d cols=%d (rows below 2^26, cols a multiple of 8, <= 8192)", rows, cols);
   V2S_CHECK(ldx >= cols && ldq >= cols, V2S_ERR_SHAPE, "v2s_quant_rows_q8: a row stride is shorter than the row");
   V2S_CHECK(aligned(x, 16) && aligned(q, 8) && aligned(scale, 4) && ldx % 8 == 0 && ldq % 8 == 0, V2S_ERR_ALIGN,
             "v2s_quant_rows_q8: x must be 16-byte and q 8-byte aligned, strides multiples of 8");
@@ -663,7 +665,8 @@ extern "C" int v2s_rmsnorm_q8(const void* x, int64_t ldx, const void* delta, int
   V2S_CHECK(x && w && q && scale, V2S_ERR_ARG, "v2s_rmsnorm_q8: NULL pointer");
   V2S_CHECK(!h || delta, V2S_ERR_ARG, "v2s_rmsnorm_q8: h is the sum x + delta, it needs delta");
   V2S_CHECK(eps >= 0.f, V2S_ERR_ARG, "v2s_rmsnorm_q8: eps must not be negative");
-  V2S_CHECK(rows > 0 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE, "v2s_rmsnorm_q8: unsupported shape rows=%d cols=%d (cols a multiple of 8, <= 8192)", rows, cols);
+  V2S_CHECK(rows > 0 && rows < 1 << 26 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE,
+            "v2s_rmsnorm_q8: unsupported shape rows=%d cols=%d (rows below 2^26, cols a multiple of 8, <= 8192)", rows, cols);
   V2S_CHECK(ldx >= cols && ldq >= cols && (!delta || ldd >= cols) && (!h || ldh >= cols), V2S_ERR_SHAPE, "v2s_rmsnorm_q8: a row stride is shorter than the row");
   V2S_CHECK(aligned(x, 16) && aligned(delta, 16) && aligned(h, 16) && aligned(w, 16) && aligned(q, 8) && aligned(scale, 4) && ldx % 8 == 0 && ldq % 8 == 0 &&
                 (!delta || ldd % 8 == 0) && (!h || ldh % 8 == 0),
@@ -681,7 +684,7 @@ extern "C" int v2s_dequant_q8(const int8_t* q, int64_t ldq, const float* scale, 
   V2S_CHECK(aligned(q, 8) && aligned(y, 16) && aligned(scale, 4) && ldq % 8 == 0 && ldy % 8 == 0, V2S_ERR_ALIGN,
             "v2s_dequant_q8: q must be 8-byte and y 16-byte aligned, strides multiples of 8");
   const int64_t blocks = ((int64_t)rows * (cols / 8) + 255) / 256;
-  V2S_CHECK(blocks <= 0x7fffffff, V2S_ERR_SHAPE, "v2s_dequant_q8: too many elements for one launch");
+  V2S_CHECK(blocks < 1 << 24, V2S_ERR_SHAPE, "v2s_dequant_q8: too many elements for one launch");
   hipLaunchKernelGGL(dequant_q8_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const i8*)q, (long)ldq, scale, (bf16_t*)y, (long)ldy, rows, cols / 8);
   V2S_LAUNCH_CHECK();
   return V2S_OK;
@@ -736,7 +739,7 @@ extern "C" int v2s_decode_attn_q8(const v2s_decode_attn_q8_args* a, void* stream
   V2S_CHECK(need == 0 || (a->workspace && a->workspace_bytes >= need && aligned(a->workspace, 4)), V2S_ERR_ARG,
             "v2s_decode_attn_q8: %lld bytes of workspace needed for %d keys, got %lld", (long long)need, a->Nk, (long long)(a->workspace ? a->workspace_bytes : 0));
   p.gchunks = (G + 15) / 16;
-  V2S_CHECK((int64_t)c.entries * c.heads * p.gchunks <= 0x7fffffff && p.np <= 65535, V2S_ERR_SHAPE, "v2s_decode_attn_q8: too many rows or keys for one launch");
+  V2S_CHECK((int64_t)a->B * c.heads < 1 << 24 && p.np <= 65535, V2S_ERR_SHAPE, "v2s_decode_attn_q8: too many rows or keys for one launch");
   const dim3 grid((unsigned)(c.entries * c.heads * p.gchunks), (unsigned)p.np);
   hipStream_t s = (hipStream_t)stream;
   if (G == 1) hipLaunchKernelGGL(attn_q8_one_kernel, grid, dim3(W1 * 64), 0, s, p);

@@ -542,7 +542,7 @@ extern "C" int v2s_sample_step(const void* logits, int32_t logits_dtype, int64_t
                                int32_t pad_id, int64_t* seq_out, int64_t seq_ld, const int32_t* pos_dev, int32_t min_length, void* stream) {
   V2S_CHECK(logits && u && next_tok, V2S_ERR_ARG, "v2s_sample_step: NULL pointer");
   V2S_CHECK(logits_dtype == V2S_F32 || logits_dtype == V2S_BF16, V2S_ERR_DTYPE, "v2s_sample_step: logits must be fp32 or bf16");
-  V2S_CHECK(rows > 0 && V > 0 && V <= 131072 && ld >= V, V2S_ERR_SHAPE, "v2s_sample_step: unsupported shape rows=%d V=%d ld=%lld (V <= 131072, ld >= V)", rows, V, (long long)ld);
+  V2S_CHECK(rows > 0 && rows < 1 << 22 && V > 0 && V <= 131072 && ld >= V, V2S_ERR_SHAPE, "v2s_sample_step: unsupported shape rows=%d V=%d ld=%lld (rows below 2^22, V <= 131072, ld >= V)", rows, V, (long long)ld);
   V2S_CHECK(temperature >= 1e-6 && temperature <= 1e6, V2S_ERR_ARG, "v2s_sample_step: temperature must be in [1e-6, 1e6]");
   V2S_CHECK(top_k >= 0 && top_p > 0.0 && top_p <= 1.0 && min_p >= 0.0 && min_p <= 1.0, V2S_ERR_ARG, "v2s_sample_step: top_k >= 0, top_p in (0, 1], min_p in [0, 1]");
   V2S_CHECK(!seq_out || pos_dev, V2S_ERR_ARG, "v2s_sample_step: seq_out needs pos_dev");

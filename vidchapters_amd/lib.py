@@ -911,7 +911,8 @@ def decode_attn_q8(q, kq, ks, vq, vs, o, Nk, *, group=1, klen=None, pos_dev=None
     if klen is not None:
         a.klen = _operand(klen, _I32, dev, n + " klen", E)
     if workspace is not None:
-        a.workspace, a.workspace_bytes = _operand(workspace, _F32, dev, n + " workspace"), workspace.numel() * 4
+        a.workspace_bytes = workspace.numel() * 4
+        a.workspace = _operand(workspace, _F32, dev, n + " workspace", workspace.numel())
     _check(lib().v2s_decode_attn_q8(C.byref(a), _raw_stream(dev)), "v2s_decode_attn_q8")
 
 
