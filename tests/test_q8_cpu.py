@@ -10,6 +10,10 @@ from vidchapters_amd import lib as L
 P = 1 << 20              # a plausible, 16-byte aligned address
 
 
+# the addresses below stand for nothing: a call that is not refused must not find a device to be launched on
+pytestmark = pytest.mark.skipif(torch.cuda.device_count() > 0, reason="refusals are checked where nothing can be launched")
+
+
 def refused(rc, word):
     assert rc < 0
     msg = L.lib().v2s_last_error().decode()
@@ -20,7 +24,7 @@ def test_rows_refusals():
     l = L.lib()
     ok = dict(x=P, dt=0, ldx=64, q=P, ldq=64, s=P, rows=4, cols=64)
     for change, word in ((dict(x=None), "NULL"), (dict(s=None), "NULL"), (dict(dt=7), "bf16 or fp32"), (dict(cols=60), "multiple of 8"), (dict(cols=8200, ldx=8200, ldq=8200), "8192"),
-                         (dict(rows=0), "rows=0"), (dict(rows=1 << 22, ld=100), "2^22"), (dict(ldx=56), "shorter"), (dict(ldq=63), "shorter"), (dict(ldx=68), "multiples of 8"), (dict(x=P + 2), "aligned"),
+                         (dict(rows=0), "rows=0"), (dict(rows=1 << 26), "2^26"), (dict(ldx=56), "shorter"), (dict(ldq=63), "shorter"), (dict(ldx=68), "multiples of 8"), (dict(x=P + 2), "aligned"),
                          (dict(q=P + 4), "aligned")):
         a = {**ok, **change}
         refused(l.v2s_quant_rows_q8(a["x"], a["dt"], a["ldx"], a["q"], a["ldq"], a["s"], a["rows"], a["cols"], None), word)
