@@ -102,6 +102,28 @@ def test_struct_sizes_match_the_binding():
         assert L.lib().v2s_sizeof(name.encode()) == ctypes.sizeof(t)
 
 
+def test_wrappers_refuse_what_is_no_tensor_and_numbers_that_do_not_fit():
+    q, s = torch.empty(4, 64, dtype=torch.int8), torch.empty(4)
+    with pytest.raises(TypeError, match="tensor"):
+        L.dequant_q8(q.numpy(), s, q, 4, 64)
+    with pytest.raises(TypeError, match="tensor"):
+        L.gemm_q8(q, q, s, s, None, 4, 4, 64)
+    with pytest.raises(ValueError, match="32 bits"):
+        L.dequant_q8(q, s, q, 1 << 40, 64)
+    with pytest.raises(ValueError, match="32 bits"):
+        L.dequant_q8(q, s, q, 4, 64, ldq=1 << 62)
+    with pytest.raises(TypeError):
+        L.quant_rows_q8(s, q, s, 4.0, 64)
+    with pytest.raises(TypeError, match="arguments"):
+        L._bind().gemm_q8(q)
+    kq, ks = torch.empty(2, 3, 10, 64, dtype=torch.int8), torch.empty(2, 3, 10)
+    for bad in (torch.empty(2, 10, 192), torch.empty(2, 1, 191), torch.empty(1, 2, 192), torch.empty(2, 192)):
+        with pytest.raises(ValueError, match="k and v are"):
+            L.kv_append_q8(bad, torch.empty(2, 2, 192), kq, ks, kq, ks, 2)
+    with pytest.raises(ValueError, match="q and o are"):
+        L.decode_attn_q8(torch.empty(2, 190), kq, ks, kq, ks, torch.empty(2, 190), 10)
+
+
 def test_wrappers_refuse_tensors_that_are_not_on_the_gpu_and_wrong_shapes():
     q, s = torch.empty(4, 64, dtype=torch.int8), torch.empty(4)
     with pytest.raises(RuntimeError, match="GPU"):

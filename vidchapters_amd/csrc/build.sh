@@ -69,3 +69,11 @@ fi
 OBJS=""; for s in $SRCS; do OBJS="$OBJS build/$s.o"; done
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o ../libvid2seq_hip.so $OBJS
 echo "built $(realpath ../libvid2seq_hip.so)"
+# the Python module that takes tensors apart for the 8-bit decoding calls (host code only; torch's libraries are loaded when it is imported)
+if [ ! -f ../_bind.so ] || [ ! -f build/bind.done ] || [ v2s_bind.cpp -nt build/bind.done ] || [ ../../include/vid2seq_hip.h -nt build/bind.done ]; then
+  TORCH=$(python3 -c 'import importlib.util as u, os; print(os.path.dirname(u.find_spec("torch").origin))')
+  PYINC=$(python3 -c 'import sysconfig; print(sysconfig.get_paths()["include"])')
+  g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -Wall -I"$TORCH/include" -I"$PYINC" v2s_bind.cpp -o ../_bind.so -L"$TORCH/lib" -ltorch_python -ltorch_cpu -lc10
+  touch build/bind.done
+  echo "built $(realpath ../_bind.so)"
+fi

@@ -8,6 +8,7 @@ import of :func:`lib` fails loudly (product path never routes through the CPU or
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 from typing import Optional
 
@@ -763,120 +764,64 @@ def beam_sample_cand(logits, ld, rows, V, K, beam_scores, top_p, temperature, to
 
 
 # --------------------------------------------------------------------------------------------- 8-bit decoding
-# A decode step is a chain of launches of a few microseconds, so the wrappers below keep their own cost low: an operand that is contiguous and large
-# enough passes in four comparisons, everything else goes through _strided, which words the refusals.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
-_F32, _BF16, _I8, _I32, _I64 = torch.float32, torch.bfloat16, torch.int8, torch.int32, torch.int64
+# A decode step is a chain of launches of a few microseconds, so these calls look at their operands in native code (csrc/v2s_bind.cpp).  Every operand
+# lives on the current device, and the launch goes to its current stream; wrong types and devices raise RuntimeError, shapes, strides and tensors whose
+# storage is too small ValueError.
+_BIND = None
 
 
-def _device(t) -> int:
-    """Index of the current device, which every operand has to live on: the launch goes to its current stream."""
-    return torch.cuda.current_device() if t.is_cuda else -2
-
-
-def _operand(t, dtype, dev: int, what: str, need: int = 0):
-    """Address of an operand of this type on device ``dev`` with at least ``need`` elements of storage behind its first one (None for None)."""
-    if t is None:
-        return None
-    if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= need:
-        return t.data_ptr()
-    return _strided(t, dtype, dev, what, need)
-
-
-def _strided(t, dtype, dev: int, what: str, need: int):
-    _need(t, dtype, what)
-    if t.get_device() != dev:
-        raise RuntimeError(f"{what}: tensor lives on {t.device}, the launch goes to cuda:{dev}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}: the last dimension must be contiguous")
-    have = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
-    if have < need:
-        raise ValueError(f"{what}: {need} elements are read or written, the tensor's storage holds {have}")
-    return t.data_ptr()
-
-
-def _view(t, dtype, dev: int, what: str):
-    """Address of an operand whose shape and strides the caller has looked at: its view covers what is read or written."""
-    return t.data_ptr() if t.dtype is dtype and t.get_device() == dev else _strided(t, dtype, dev, what, 0)
+def _bind():
+    global _BIND
+    if _BIND is None:
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_bind.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} not found: build it with vidchapters_amd/csrc/build.sh (or __graft_entry__.build()).")
+        spec = importlib.util.spec_from_file_location("vidchapters_amd._bind", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        address = lambda name: C.cast(getattr(lib(), "v2s_" + name), _vp).value  # noqa: E731
+        m.attach(getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+                 getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream),
+                 *(address(n) for n in ("quant_rows_q8", "rmsnorm_q8", "dequant_q8", "gemm_q8", "kv_append_q8", "kv_read_q8", "decode_attn_q8", "sample_step")))
+        _BIND = m
+    return _BIND
 
 
 def quant_rows_q8(x, q, scale, rows, cols, *, ldx=None, ldq=None):
     """int8 codes ``q`` [rows, ldq] and one fp32 scale per row of the rows of ``x`` (bf16 or fp32): weights once, activations per token."""
-    ldx, ldq, dev, f32 = ldx or cols, ldq or cols, _device(x), x.dtype is _F32
-    xp = _operand(x, _F32 if f32 else _BF16, dev, "quant_rows_q8 x", (rows - 1) * ldx + cols)
-    qp, sp = _operand(q, _I8, dev, "quant_rows_q8 q", (rows - 1) * ldq + cols), _operand(scale, _F32, dev, "quant_rows_q8 scale", rows)
-    _check(lib().v2s_quant_rows_q8(xp, V2S_F32 if f32 else V2S_BF16, ldx, qp, ldq, sp, rows, cols, _raw_stream(dev)), "v2s_quant_rows_q8")
+    _check(_bind().quant_rows_q8(x, q, scale, rows, cols, ldx, ldq), "v2s_quant_rows_q8")
 
 
 def rmsnorm_q8(x, w, q, scale, rows, cols, eps, *, delta=None, h=None, ldx=None, ldd=None, ldh=None, ldq=None):
     """s = bf16(x + delta) (to ``h`` if given), then T5 RMSNorm and int8 codes ``q`` with one ``scale`` per row, in one pass."""
-    ldx, ldd, ldh, ldq, dev, last = ldx or cols, ldd or cols, ldh or cols, ldq or cols, _device(x), rows - 1
-    xp, wp = _operand(x, _BF16, dev, "rmsnorm_q8 x", last * ldx + cols), _operand(w, _F32, dev, "rmsnorm_q8 w", cols)
-    dp, hp = _operand(delta, _BF16, dev, "rmsnorm_q8 delta", last * ldd + cols), _operand(h, _BF16, dev, "rmsnorm_q8 h", last * ldh + cols)
-    qp, sp = _operand(q, _I8, dev, "rmsnorm_q8 q", last * ldq + cols), _operand(scale, _F32, dev, "rmsnorm_q8 scale", rows)
-    _check(lib().v2s_rmsnorm_q8(xp, ldx, dp, ldd, wp, hp, ldh, qp, ldq, sp, rows, cols, eps, _raw_stream(dev)), "v2s_rmsnorm_q8")
+    _check(_bind().rmsnorm_q8(x, w, q, scale, rows, cols, eps, delta, h, ldx, ldd, ldh, ldq), "v2s_rmsnorm_q8")
 
 
 def dequant_q8(q, scale, y, rows, cols, *, ldq=None, ldy=None):
     """y[rows, ldy] (bf16) = scale[row] * q[row]: the values that codes stand for."""
-    ldq, ldy, dev = ldq or cols, ldy or cols, _device(q)
-    qp, sp = _operand(q, _I8, dev, "dequant_q8 q", (rows - 1) * ldq + cols), _operand(scale, _F32, dev, "dequant_q8 scale", rows)
-    yp = _operand(y, _BF16, dev, "dequant_q8 y", (rows - 1) * ldy + cols)
-    _check(lib().v2s_dequant_q8(qp, ldq, sp, yp, ldy, rows, cols, _raw_stream(dev)), "v2s_dequant_q8")
+    _check(_bind().dequant_q8(q, scale, y, rows, cols, ldq, ldy), "v2s_dequant_q8")
 
 
 def gemm_q8(A, B, sA, sB, C_out, M, N, K, *, lda=None, ldb=None, ldc=None, alpha=1.0, bias=None, act=ACT_NONE, residual=None, ldr=None):
     """C[M, N] = act(alpha * sA[m] * sB[n] * A(m, :) . B(n, :) + bias) + residual with int8 A (token codes) and B (weight codes [out, in])."""
-    dev, f32, last = _device(A), C_out.dtype is _F32, M - 1
-    lda, ldb, ldc, ldr = lda or K, ldb or K, ldc or N, ldr or N
-    a = GemmQ8Args(M, N, K, _operand(A, _I8, dev, "gemm_q8 A", last * lda + K), _operand(B, _I8, dev, "gemm_q8 B", (N - 1) * ldb + K), lda, ldb,
-                   _operand(sA, _F32, dev, "gemm_q8 sA", M), _operand(sB, _F32, dev, "gemm_q8 sB", N),
-                   _operand(C_out, _F32 if f32 else _BF16, dev, "gemm_q8 C", last * ldc + N), ldc, V2S_F32 if f32 else V2S_BF16, alpha,
-                   None if bias is None else _operand(bias, _F32, dev, "gemm_q8 bias", N), act,
-                   None if residual is None else _operand(residual, _BF16, dev, "gemm_q8 residual", last * ldr + N), ldr)
     kt = KernelTimer.active
     if kt is not None:
         e0 = kt.begin()
-    _check(lib().v2s_gemm_q8(C.byref(a), _raw_stream(dev)), "v2s_gemm_q8")
+    _check(_bind().gemm_q8(A, B, sA, sB, C_out, M, N, K, lda, ldb, ldc, alpha, bias, act, residual, ldr), "v2s_gemm_q8")
     if kt is not None:
         kt.end("gemm_q8" + (f":{M}x{N}x{K}" if kt.detail else ""), 2.0 * M * N * K, e0)
 
 
-def _kv_q8(kq, ks, vq, vs, dev: int, what: str) -> KvQ8:
-    """The cache as four tensors: codes [entries, heads, maxlen, 64] int8 and scales [entries, heads, maxlen] fp32."""
-    rows = ks.shape
-    if len(rows) != 3 or vs.shape != rows or kq.shape != (*rows, 64) or vq.shape != (*rows, 64):
-        raise ValueError(f"{what}: a cache is codes [entries, heads, maxlen, 64] and scales [entries, heads, maxlen] for keys and for values")
-    e, h, one = strides = ks.stride()
-    codes = (e * 64, h * 64, 64, 1)
-    if one != 1 or vs.stride() != strides or kq.stride() != codes or vq.stride() != codes:
-        raise ValueError(f"{what}: codes and scales of a cache share their row strides, the rows of a head are contiguous")
-    return KvQ8(_view(kq, _I8, dev, what), _view(ks, _F32, dev, what), _view(vq, _I8, dev, what), _view(vs, _F32, dev, what), e, h, *rows)
-
-
-def _kv_move(fn, name: str, k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count):
-    dev = _device(kq)
-    c = _kv_q8(kq, ks, vq, vs, dev, name)
-    shape, strides, E, cols = k.shape, k.stride(), c.entries, c.heads * 64
-    if len(shape) != 3 or v.shape != shape or shape[0] != E or shape[1] < T or shape[2] < cols or v.stride() != strides:
-        raise ValueError(f"{name}: k and v are [{E}, >= {T}, >= {cols}] with the same strides, got {tuple(shape)} and {tuple(v.shape)}")
-    bs, rs, one = strides
-    if one != 1:
-        raise ValueError(f"{name}: the last dimension of k and v must be contiguous")
-    _check(fn(C.byref(c), _view(k, _BF16, dev, name), _view(v, _BF16, dev, name), bs, rs, T, pos0,
-              pos if pos is None else _operand(pos, _I32, dev, name, E), pos_dev if pos_dev is None else _operand(pos_dev, _I32, dev, name, 1),
-              count if count is None else _operand(count, _I32, dev, name, E), _raw_stream(dev)), "v2s_" + name)
-
-
 def kv_append_q8(k, v, kq, ks, vq, vs, T, *, pos0=0, pos=None, pos_dev=None, count=None):
-    """Quantises T new tokens per entry (k, v: bf16 [entries, T, heads * 64]) as they enter the int8 cache, at ``pos`` (int32 [entries]) or ``pos0``,
-    plus ``*pos_dev``; ``count`` (int32 [entries]) limits an entry to its first tokens.  Tokens outside the cache are dropped."""
-    _kv_move(lib().v2s_kv_append_q8, "kv_append_q8", k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count)
+    """Quantises T new tokens per entry (k, v: bf16 [entries, T, heads * 64]) as they enter the int8 cache (codes [entries, heads, maxlen, 64] int8 and
+    scales [entries, heads, maxlen] fp32 for keys and for values), at ``pos`` (int32 [entries]) or ``pos0``, plus ``*pos_dev``; ``count`` (int32 [entries])
+    limits an entry to its first tokens.  Tokens outside the cache are dropped."""
+    _check(_bind().kv_append_q8(k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count), "v2s_kv_append_q8")
 
 
 def kv_read_q8(kq, ks, vq, vs, k, v, T, *, pos0=0, pos=None, pos_dev=None, count=None):
     """Reads T tokens per entry back as bf16 rows of the attention's layout; rows that take no part stay as they are."""
-    _kv_move(lib().v2s_kv_read_q8, "kv_read_q8", k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count)
+    _check(_bind().kv_read_q8(k, v, kq, ks, vq, vs, T, pos0, pos, pos_dev, count), "v2s_kv_read_q8")
 
 
 def decode_attn_q8_workspace(B, H, Nk, device):
@@ -888,46 +833,12 @@ def decode_attn_q8_workspace(B, H, Nk, device):
 def decode_attn_q8(q, kq, ks, vq, vs, o, Nk, *, group=1, klen=None, pos_dev=None, bias_maxlen=0, bias_row=None, key_mask=None, scale=1.0, workspace=None):
     """o[B, heads * 64] = attention of one query row per (row, head) over the first ``Nk`` (or ``klen[entry]``, or ``*pos_dev + 1``) keys of the int8
     cache; ``group`` consecutive rows of q share an entry.  See include/vid2seq_hip.h for masks and empty rows."""
-    a, dev, n = DecodeAttnQ8Args(), _device(q), "decode_attn_q8"
-    c = a.cache = _kv_q8(kq, ks, vq, vs, dev, n)
-    E, H = c.entries, c.heads
-    B = E * group
-    if q.shape != (B, H * 64) or o.shape != (B, H * 64):
-        raise ValueError(f"{n}: q and o are [{B}, {H * 64}], got {tuple(q.shape)} and {tuple(o.shape)}")
-    a.B, a.Nk, a.group, a.scale = B, Nk, group, scale
-    a.q, a.q_bs, a.o, a.o_bs = _operand(q, _BF16, dev, n + " q"), q.stride(0), _operand(o, _BF16, dev, n + " o"), o.stride(0)
-    if bias_row is not None:
-        if bias_row.dim() != 2 or bias_row.shape[0] != H:
-            raise ValueError(f"{n}: bias_row is [heads, keys], got {tuple(bias_row.shape)}")
-        a.bias_ld = bias_row.stride(0) if H > 1 else bias_row.shape[1]
-        a.bias_row = _operand(bias_row, _F32, dev, n + " bias_row", (H - 1) * a.bias_ld + (2 * bias_maxlen - 1 if pos_dev is not None else Nk))
-    if key_mask is not None:
-        if key_mask.dim() != 2 or key_mask.shape[0] != E:
-            raise ValueError(f"{n}: key_mask is [entries, keys], got {tuple(key_mask.shape)}")
-        a.mask_ld = key_mask.stride(0) if E > 1 else key_mask.shape[1]
-        a.key_mask = _operand(key_mask, torch.uint8, dev, n + " key_mask", (E - 1) * a.mask_ld + Nk)
-    if pos_dev is not None:
-        a.pos_dev, a.bias_maxlen = _operand(pos_dev, _I32, dev, n + " pos_dev", 1), bias_maxlen
-    if klen is not None:
-        a.klen = _operand(klen, _I32, dev, n + " klen", E)
-    if workspace is not None:
-        a.workspace_bytes = workspace.numel() * 4
-        a.workspace = _operand(workspace, _F32, dev, n + " workspace", workspace.numel())
-    _check(lib().v2s_decode_attn_q8(C.byref(a), _raw_stream(dev)), "v2s_decode_attn_q8")
+    _check(_bind().decode_attn_q8(q, kq, ks, vq, vs, o, Nk, group, klen, pos_dev, bias_maxlen, bias_row, key_mask, scale, workspace), "v2s_decode_attn_q8")
 
 
 def sample_step(logits, rows, V, u, next_tok, *, ld=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logp=None, unfinished=None, eos_id=-1, pad_id=0,
                 seq_out=None, seq_ld=0, pos_dev=None, min_length=0):
     """One token per row of ``logits`` (fp32 or bf16 [rows, ld]) from temperature, top-k, top-p, min-p and the given numbers ``u`` (fp32 [rows] in
     [0, 1), or [steps, rows] with ``pos_dev``): every draw is a function of its arguments.  ``logp``: log-probability of the token among the kept ones."""
-    n, dev, f32 = "sample_step", _device(logits), logits.dtype is _F32
-    ld = ld or (logits.stride(0) if logits.dim() == 2 and rows > 1 else V)
-    if u.dim() != (1 if pos_dev is None else 2) or u.shape[-1] < rows:
-        raise ValueError(f"sample_step: u is [rows], or [steps, rows] with pos_dev, got {tuple(u.shape)} for {rows} rows")
-    steps, u_ld = (0, 0) if pos_dev is None else (u.shape[0], u.stride(0) if u.shape[0] > 1 else u.shape[1])
-    zp = _operand(logits, _F32 if f32 else _BF16, dev, n + " logits", (rows - 1) * ld + V)
-    up, tp, pp = _operand(u, _F32, dev, n + " u", rows), _operand(next_tok, _I64, dev, n + " next_tok", rows), _operand(logp, _F32, dev, n + " logp", rows)
-    fp, sp = _operand(unfinished, _I32, dev, n + " unfinished", rows), _operand(seq_out, _I64, dev, n + " seq_out", rows * seq_ld)
-    dp = _operand(pos_dev, _I32, dev, n + " pos_dev", 1)
-    _check(lib().v2s_sample_step(zp, V2S_F32 if f32 else V2S_BF16, ld, rows, V, temperature, top_k, top_p, min_p, up, u_ld, steps, tp, pp, fp, eos_id, pad_id, sp,
-                                 seq_ld, dp, min_length, _raw_stream(dev)), "v2s_sample_step")
+    _check(_bind().sample_step(logits, rows, V, u, next_tok, ld, temperature, top_k, top_p, min_p, logp, unfinished, eos_id, pad_id, seq_out, seq_ld, pos_dev,
+                               min_length), "v2s_sample_step")
