@@ -12,6 +12,7 @@ namespace {
 
 typedef signed char i8;
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
 constexpr float Q8_TINY = 127.0f * 1.17549435e-38f;
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -280,6 +281,14 @@ __device__ float attn_q8_mean(const i8* vq, const float* vs, int n, float* lds) 
   return n > 0 ? s / (float)n : 0.f;
 }
 
+// reduction over the lanes with the same lane & 15, by the swaps of half waves and of odd and even rows (a shuffle through LDS has five times the latency)
+template <class F> __device__ __forceinline__ float rows_reduce(float v, F f) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // eight codes as bf16, exactly
 __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
   float f[8];
@@ -293,20 +302,24 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
 }
 
 // Block = 4 waves = up to PIECE keys of one (entry, head) against up to 16 of its queries, on the matrix pipe; a wave takes 64 keys at a time.
+//   loads    16 whole keys (1 KiB in a row) per instruction.  Keys loaded straight into the fragments' lanes (16 rows of 16 bytes per instruction) asked the
+//            cache for every line four times: 348 MB in 94 us, through LDS in 66.
 //   scores   S^T[key][query] = K[key][d] . Q^T[d][query] by v_mfma_f32_16x16x32_bf16: codes are exact in bf16, so the products are exact and the sums
-//            fp32.  A lane loads 16 contiguous codes of a key (one load of the wave: 16 whole keys); tile t of a group of 32 keys holds the keys
-//            8 (row >> 2) + 4 t + (row & 3), so that the eight scores a lane gets of its query are those of the consecutive keys 8 g .. 8 g + 7
-//            (g = lane >> 4), which is the B operand of the second product without any movement.
-//   output   O^T[d][query] += V^T[d][key] . P^T[key][query]: the value codes pass through LDS, the transposing read (ds_read_b64_tr_b8) returns the
-//            codes of eight keys for one d.  The weights carry the values' scales and are split into bf16 high and low parts (16 bits, two products).
-// The running maximum of a query is shared by its four lanes (two exchanges per 64 keys); scales and bias of the piece wait in LDS, where a key
-// without a part has bias -infinity and scales of zero.
-// A value-per-lane form without the matrix pipe was bound by VALU issue at four queries (127 us at 4 x 4 queries x 16 heads x 40000 keys).
-constexpr int VPITCH = 80;            // bytes per key of the value tile: the 16-byte rows of a transposing read fall into different banks
-__global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
+//            fp32.  Tile t of a group of 32 keys holds the keys 8 (row >> 2) + 4 t + (row & 3), so that the eight scores a lane gets of its query are
+//            those of the consecutive keys 8 g .. 8 g + 7 (g = lane >> 4), which is the B operand of the second product without any movement.
+//   output   O^T[d][query] += V^T[d][key] . P^T[key][query]: the value codes follow the keys in the wave's LDS tile, the transposing read
+//            (ds_read_b64_tr_b8) returns the codes of eight keys for one d.  The weights carry the values' scales and are split into bf16 high and low
+//            parts (16 bits, two products).
+// The running maximum of a query is shared by its four lanes; scales and bias of the piece wait in LDS, where a key without a part has bias -infinity
+// and scales of zero.  4 x 4 queries x 16 heads x 40000 keys: 66 us, 5.3 TB/s, the rate of a large copy.  A value-per-lane form without the matrix pipe was
+// bound by VALU issue (127 us); eight waves per block or five blocks per CU were slower on large caches, requesting the next chunk ahead did not pay.
+constexpr int WG = 4;                 // waves per block
+// byte of the 16-byte chunk c of key k in a wave's tile: the rows of a fragment read and those of a transposing read fall into different banks
+__device__ __forceinline__ int tile_at(int k, int c) { return k * 64 + (c ^ ((k >> 3) & 3) ^ ((k >> 2) & 1)) * 16; }
+__global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
   __shared__ __attribute__((aligned(16))) float s_ks[PIECE], s_vs[PIECE], s_b[PIECE];
-  __shared__ __attribute__((aligned(16))) char s_v[4][64 * VPITCH];       // value tiles, then the waves' sums
-  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ __attribute__((aligned(16))) char s_v[WG][64 * 64];       // value tiles, then the waves' sums
+  __shared__ float s_m[WG][16], s_l[WG][16];
   __shared__ uint32_t s_any;           // chunks of 64 keys that hold a visible one
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 15, g = lane >> 4;
   const int gc = blockIdx.x % p.gchunks, eh = blockIdx.x / p.gchunks;
@@ -333,17 +346,25 @@ __global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
     }
     qf[0] = __builtin_bit_cast(bf16x8, a); qf[1] = __builtin_bit_cast(bf16x8, b);
   }
-  for (int r = 0; r < nch; r += 4) {
-    const int k = r * 64 + tid;
-    bool see = k < end;
-    if (see && p.mask) see = p.mask[(long)e * p.mask_ld + k0 + k] != 0;
-    float b = -INFINITY;
-    if (see) b = bias ? bias[k] : 0.f;
-    see = !(b == -INFINITY);
-    const float sk = see ? ks[k] * p.scale : 0.f, sv = see ? vs[k] : 0.f;
-    if (k < PIECE) { s_ks[k] = sk; s_vs[k] = sv; s_b[k] = b; }
-    const unsigned long long any = __ballot(see);
-    if (lane == 0 && any != 0) atomicOr(&s_any, 1u << (r + wave));
+  if (nch > 0) {                        // every load in flight before the first is used
+    constexpr int R = (PIECE + WG * 64 - 1) / (WG * 64);
+    float sk[R], sv[R], b[R];
+    uint8_t mk[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = min(r * (WG * 64) + tid, end - 1);
+      sk[r] = ks[k]; sv[r] = vs[k];
+      b[r] = bias ? bias[k] : 0.f;
+      mk[r] = p.mask ? p.mask[(long)e * p.mask_ld + k0 + k] : 1;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = r * (WG * 64) + tid;
+      const bool see = k < end && mk[r] != 0 && !(b[r] == -INFINITY);
+      if (k < PIECE) { s_ks[k] = see ? sk[r] * p.scale : 0.f; s_vs[k] = see ? sv[r] : 0.f; s_b[k] = see ? b[r] : -INFINITY; }
+      const unsigned long long any = __ballot(see);
+      if (lane == 0 && any != 0) atomicOr(&s_any, 1u << (r * WG + wave));
+    }
   }
   __syncthreads();
 
@@ -352,38 +373,55 @@ __global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
   for (int i = 0; i < 4; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   char* const vt = s_v[wave];
-  // (requesting the next chunk's codes ahead was slower: it costs a quarter of the waves, and these hide the loads of each other)
+  u32x4 kr[4], vr[4];
+  auto load = [&](int ch) {             // codes of a chunk; keys behind the end load the last one: their scales are zero
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = (uint32_t)(min(ch * 64 + i * 16 + (lane >> 2), end - 1) * 64 + (lane & 3) * 16);
+      kr[i] = *reinterpret_cast<const u32x4*>(kq + at);
+      vr[i] = *reinterpret_cast<const u32x4*>(vq + at);
+    }
+  };
   for (uint32_t rest = __builtin_amdgcn_readfirstlane(s_any) & (0x11111111u << wave); rest; rest &= rest - 1) {
     const int ch = __builtin_ctz(rest);
-    u32x4 kr[4], vr[4];
+    load(ch);
+    // all of the chunk's LDS traffic but the values' scales in one go (a wave's LDS operations keep their order, so the values may follow the keys in place)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {       // keys behind the end load the last one: their scales are zero
-      const int kk = ch * 64 + (i >> 1) * 32 + 8 * (qi >> 2) + 4 * (i & 1) + (qi & 3), kv = ch * 64 + i * 16 + (lane >> 2);
-      kr[i] = *reinterpret_cast<const u32x4*>(kq + (uint32_t)(min(kk, end - 1) * 64 + g * 16));
-      vr[i] = *reinterpret_cast<const u32x4*>(vq + (uint32_t)(min(kv, end - 1) * 64 + (lane & 3) * 16));
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(vt + tile_at(i * 16 + (lane >> 2), lane & 3)) = kr[i];
+    u32x4 kf[4];
+    float4 sk[4], sb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      kf[i] = *reinterpret_cast<const u32x4*>(vt + tile_at((i >> 1) * 32 + 8 * (qi >> 2) + 4 * (i & 1) + (qi & 3), g));
+      const int at = ch * 64 + (i >> 1) * 32 + 8 * g + 4 * (i & 1);
+      sk[i] = *reinterpret_cast<const float4*>(s_ks + at); sb[i] = *reinterpret_cast<const float4*>(s_b + at);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(vt + tile_at(i * 16 + (lane >> 2), lane & 3)) = vr[i];
+    i32x2 vc[2][4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+        vc[kb][dt] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((V2S_LDS i32x2*)(vt + tile_at(kb * 32 + 8 * g + (qi >> 1), dt) + (qi & 1) * 8));
+    __builtin_amdgcn_sched_barrier(0);
     float sc[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f32x4 d = {0.f, 0.f, 0.f, 0.f};
-      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(kr[i][0], kr[i][1]), qf[0], d, 0, 0, 0);
-      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(kr[i][2], kr[i][3]), qf[1], d, 0, 0, 0);
-      const int at = ch * 64 + (i >> 1) * 32 + 8 * g + 4 * (i & 1);
-      const float4 sk = *reinterpret_cast<const float4*>(s_ks + at), b = *reinterpret_cast<const float4*>(s_b + at);
-      const float z0 = fmaf(d[0], sk.x, b.x);
-      const float z1 = fmaf(d[1], sk.y, b.y);
-      const float z2 = fmaf(d[2], sk.z, b.z);
-      const float z3 = fmaf(d[3], sk.w, b.w);
-      sc[4 * i + 0] = b.x == -INFINITY ? b.x : z0; sc[4 * i + 1] = b.y == -INFINITY ? b.y : z1;       // whatever a query holds
-      sc[4 * i + 2] = b.z == -INFINITY ? b.z : z2; sc[4 * i + 3] = b.w == -INFINITY ? b.w : z3;
-    }
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(kf[i][0], kf[i][1]), qf[0], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(kf[i][2], kf[i][3]), qf[1], d, 0, 0, 0);
+      const float ks4[4] = {sk[i].x, sk[i].y, sk[i].z, sk[i].w}, b4[4] = {sb[i].x, sb[i].y, sb[i].z, sb[i].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(vt + (i * 16 + (lane >> 2)) * VPITCH + (lane & 3) * 16) = vr[i];
+      for (int r = 0; r < 4; ++r) {
+        const float z = fmaf(d[r], ks4[r], b4[r]);
+        sc[4 * i + r] = b4[r] == -INFINITY ? b4[r] : z;      // whatever a query holds
+      }
+    }
     float mn = sc[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mn = fmaxf(mn, sc[i]);
-    mn = fmaxf(mn, __shfl_xor(mn, 16, 64));
-    mn = fmaxf(mn, __shfl_xor(mn, 32, 64));
+    mn = rows_reduce(mn, [](float a, float b) { return fmaxf(a, b); });
     mn = fmaxf(mn, m);
     const float a = rescale(m, mn);
     m = mn;
@@ -411,39 +449,42 @@ __global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
       lo = round8(w);
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
-        typedef __attribute__((ext_vector_type(2))) int i32x2;
-        const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((V2S_LDS i32x2*)(vt + (kb * 32 + 8 * g + (qi >> 1)) * VPITCH + dt * 16 + (qi & 1) * 8));
-        const bf16x8 vf = codes_bf16((uint32_t)c[0], (uint32_t)c[1]);
+        const bf16x8 vf = codes_bf16((uint32_t)vc[kb][dt][0], (uint32_t)vc[kb][dt][1]);
         acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, hi), acc[dt], 0, 0, 0);
         acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, lo), acc[dt], 0, 0, 0);
       }
     }
   }
   // join the waves: [query][64] sums per wave in the wave's own tile
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  l = rows_reduce(l, [](float a, float b) { return a + b; });
   float* const so = reinterpret_cast<float*>(vt);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<f32x4*>(so + qi * 64 + dt * 16 + g * 4) = acc[dt];
   if (g == 0) { s_m[wave][qi] = m; s_l[wave][qi] = l; }
   __syncthreads();
+  const auto seen = [&](int q) {        // sum of a query's weights: zero if it sees no key
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WG; ++w) l += s_l[w][q];
+    return l != 0.f;
+  };
   if (p.np == 1) {
     bool none = false;                  // a query of this block without a visible key
-    for (int q = 0; q < ng; ++q) none |= s_l[0][q] + s_l[1][q] + s_l[2][q] + s_l[3][q] == 0.f;
+    for (int q = 0; q < ng; ++q) none |= !seen(q);
     if (none) {                         // the same for every thread of the block
       const float mean = attn_q8_mean(vq, vs, n, s_b);
-      for (int t = tid; t < ng * 64; t += 256) {
-        const int q = t >> 6;
-        if (s_l[0][q] + s_l[1][q] + s_l[2][q] + s_l[3][q] == 0.f) p.o[((long)e * p.G + g0 + q) * p.o_bs + h * 64 + (t & 63)] = f2bf(mean);
-      }
+      for (int t = tid; t < ng * 64; t += WG * 64)
+        if (!seen(t >> 6)) p.o[((long)e * p.G + g0 + (t >> 6)) * p.o_bs + h * 64 + (t & 63)] = f2bf(mean);
     }
   }
-  for (int t = tid; t < ng * 64; t += 256) {
+  for (int t = tid; t < ng * 64; t += WG * 64) {
     const int q = t >> 6, d = t & 63;
-    const float M = fmaxf(fmaxf(s_m[0][q], s_m[1][q]), fmaxf(s_m[2][q], s_m[3][q]));
+    float M = s_m[0][q];
+#pragma unroll
+    for (int w = 1; w < WG; ++w) M = fmaxf(M, s_m[w][q]);
     float L = 0.f, O = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WG; ++w) {
       const float a = rescale(s_m[w][q], M);
       L += s_l[w][q] * a; O += reinterpret_cast<const float*>(s_v[w])[q * 64 + d] * a;
     }
@@ -461,6 +502,8 @@ __global__ __launch_bounds__(256, 4) void attn_q8_kernel(const AttnQ8 p) {
 // One query per entry: block = 4 waves = up to PIECE keys of one (entry, head).  lane = (key slot lane >> 2, 16 dimensions lane & 3): a load of the wave is
 // 16 whole keys (1 KiB).  On the matrix pipe fifteen of the sixteen query columns would be empty while every lane still converts the codes and
 // computes a softmax, so the fp32 pipe needs a third fewer instructions here.
+// 32 x 16 heads x 5000 keys: 68 us with the join, 5.1 TB/s; twice the waves per block: 8 x 12 heads x 1200 keys 7.7 instead of 8.7 us, but 64 x 12 x 300
+// keys 11.1 instead of 9.6.
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
@@ -548,16 +591,18 @@ __global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {
   // the 16 key slots of the wave, then the waves
   float M = m;
 #pragma unroll
-  for (int o = 4; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  for (int o = 4; o < 16; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  M = rows_reduce(M, [](float x, float y) { return fmaxf(x, y); });
   const float a = rescale(m, M);
   float L = l * a;
   L = dpp_add<0x128>(L); L = dpp_add<0x124>(L);      // row_ror 8 and 4 keep lane & 3
-  L += __shfl_xor(L, 16, 64); L += __shfl_xor(L, 32, 64);
+  const auto add = [](float x, float y) { return x + y; };
+  L = rows_reduce(L, add);
 #pragma unroll
   for (int d = 0; d < 16; ++d) {
     float x = acc[d] * a;
     x = dpp_add<0x128>(x); x = dpp_add<0x124>(x);
-    x += __shfl_xor(x, 16, 64); x += __shfl_xor(x, 32, 64);
+    x = rows_reduce(x, add);
     if (slot == 0) s_o[wave][c * 16 + d] = x;
   }
   if (lane == 0) { s_m[wave] = M; s_l[wave] = L; }
@@ -581,24 +626,36 @@ __global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {
 
 // joins the pieces of one (query, head): 4 waves take the pieces in turn
 __global__ __launch_bounds__(256) void attn_q8_join_kernel(const AttnQ8 p) {
-  __shared__ float s_l[4], s_o[4][64], s_red[256];
+  __shared__ float s_m[4], s_l[4], s_o[4][64], s_red[256];
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H, e = b / p.G;
   const int d = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = attn_q8_keys(p, e), np = (n + PIECE - 1) / PIECE;
   const float* w = p.ws + (long)blockIdx.x * p.np * 66;
-  float M = -INFINITY, L = 0.f, O = 0.f;              // the maximum first: the pieces' sums can then be read without waiting for each other
-  for (int i = d; i < np; i += 64) M = fmaxf(M, w[i * 66 + 64]);
-  M = wave_max(M);
-#pragma unroll 8
-  for (int i = wave; i < np; i += 4) {
-    const float a = rescale(w[i * 66 + 64], M);
-    L += w[i * 66 + 65] * a; O += w[i * 66 + d] * a;
+  float M = -INFINITY, L = 0.f, O = 0.f;
+  for (int i0 = wave; i0 < p.np; i0 += 32) {         // eight pieces of the wave in flight, before the length is known: those behind it have no part
+    float m[8], l[8], o[8], mn = M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float* v = w + min(i0 + j * 4, p.np - 1) * 66;
+      m[j] = v[64]; l[j] = v[65]; o[j] = v[d];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i0 + j * 4 >= np) { m[j] = -INFINITY; l[j] = 0.f; o[j] = 0.f; }
+      mn = fmaxf(mn, m[j]);
+    }
+    const float a = rescale(M, mn);
+    L *= a; O *= a; M = mn;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { const float x = rescale(m[j], mn); L += l[j] * x; O += o[j] * x; }
   }
   s_o[wave][d] = O;
-  if (d == 0) s_l[wave] = L;
+  if (d == 0) { s_m[wave] = M; s_l[wave] = L; }
   __syncthreads();
-  L = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-  O = s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d];
+  M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  L = O = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float x = rescale(s_m[i], M); L += s_l[i] * x; O += s_o[i][d] * x; }
   float r = O / L;
   if (L == 0.f) {                                    // the same for every thread of the block
     const long base = (long)e * p.e_rows + (long)h * p.h_rows;
@@ -743,7 +800,7 @@ extern "C" int v2s_decode_attn_q8(const v2s_decode_attn_q8_args* a, void* stream
   const dim3 grid((unsigned)(c.entries * c.heads * p.gchunks), (unsigned)p.np);
   hipStream_t s = (hipStream_t)stream;
   if (G == 1) hipLaunchKernelGGL(attn_q8_one_kernel, grid, dim3(W1 * 64), 0, s, p);
-  else hipLaunchKernelGGL(attn_q8_kernel, grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL(attn_q8_kernel, grid, dim3(WG * 64), 0, s, p);
   V2S_LAUNCH_CHECK();
   if (p.np > 1) {
     hipLaunchKernelGGL(attn_q8_join_kernel, dim3((unsigned)(a->B * c.heads)), dim3(256), 0, s, p);
