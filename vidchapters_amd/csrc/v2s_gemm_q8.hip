@@ -47,14 +47,14 @@ template <int W> __device__ __forceinline__ typename Raw<W>::T residual_of(const
   if (m < p.M && n + W <= p.N) z = *reinterpret_cast<const typename Raw<W>::T*>(p.residual + (long)m * p.ldr + n);
   return z;
 }
-// exact-erf GELU without branches: v Phi(v) with erfc(|v| / sqrt 2) = (a1 t + ... + a5 t^5) exp(-v^2 / 2), t = 1 / (1 + p |v| / sqrt 2) (Abramowitz and
-// Stegun 7.1.26, absolute error below 1.5e-7, that is 1.3 fp32 roundings of v); the library's erf is three times as long
+// exact-erf GELU: v Phi(v) with Phi(v) = 1 / (1 + exp(-L(v))), L(v) = log(Phi(v) / Phi(-v)) = v P(v^2).  P is the weighted minimax polynomial of degree six
+// on v^2 <= 36 (error of v Phi below 7e-8, with the fp32 evaluation below 3 roundings of v), held at its last value beyond, where Phi is 0 or 1 to fp32; its
+// coefficients carry the factor -log2 e.  19 cycles' worth of instructions a value, a quarter less than a form with the two tails of erfc apart.
 __device__ __forceinline__ float gelu_q8(float v) {
-  const float x = fabsf(v) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
-  const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float tail = 0.5f * v * q * __builtin_amdgcn_exp2f(x * x * -1.44269504088896340736f);      // v (1 - Phi(|v|))
-  return v < 0.f ? tail : v - tail;
+  const float s = fminf(v * v, 36.0f);
+  float t = fmaf(-5.209905840e-9f, s, 3.850448422e-7f);
+  t = fmaf(t, s, -1.145242732e-5f); t = fmaf(t, s, 1.593893976e-4f); t = fmaf(t, s, 9.559299360e-5f); t = fmaf(t, s, -0.1048385799f); t = fmaf(t, s, -2.302207232f);
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * t));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   typedef __attribute__((ext_vector_type(2))) float f32x2;
@@ -496,14 +496,15 @@ extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   // Rounds of the chip's blocks times the time of one (us, n = stages of 128): 256 x 256 tiles 6.5 + 1.5 n, 128 x 128 3.0 + 0.95 n, 64 x 64 1.9 + 0.66 n, fitted to
   // N = 2304, K = 16 .. 3200: at K = 768, M = 1000 / 2000 / 8000 / 27501 they take 14.4 / 14.5 / 32.1 / 64.9, 8.0 / 10.1 / 22.5 / 70.7 and 7.3 / 10.1 / 27.2 / 108 us.
-  // Up to 64 rows a launch is bound by the latency of its weights, and the few-row kernels ask for all of them at once (64 x 2304 x 768: 4.3 us, 64 x 64 tiles
-  // 4.6; 16 x 6000 x 1024: 4.2 and 5.4), until the rows read again for every 16 columns outweigh that (64 x 5000 x 768: 6.1 and 5.1, 64 x 32228 x 768: 18.5 and 9.5).
+  // Few rows: a launch is bound by the latency of its operands, and the few-row kernels ask for all of them at once (64 x 2304 x 768: 4.3 us, 64 x 64 tiles 4.6;
+  // 16 x 6000 x 1024: 4.2 and 5.4), until the rows read again for every 16 columns outweigh that (64 x 5000 x 768: 6.1 and 5.1, 64 x 32228 x 768: 18.5 and 9.5).
+  // With more rows that comes earlier (400 x 300 x 4096: 10.2 and 12.8, 1000 x 128 x 768: 4.6 and 5.2; 300 x 1000 x 2000: 9.3 and 8.4, 7581 x 64 x 3488: 23 and 11).
   auto rounds = [&](int t, int slots) { return (double)(((int64_t)((p.M + t - 1) / t) * ((p.N + t - 1) / t) + slots - 1) / slots); };
   const double n = (p.K + 127) / 128;
   const double t4 = rounds(256, 256) * (6.5 + 1.5 * n), t3 = rounds(128, 512) * (3.0 + 0.95 * n), t2 = rounds(64, 1024) * (1.9 + 0.66 * n);
   int kind = v2s_opt_gemm_q8();
   const bool plain = !p.c_f32 && p.act != V2S_ACT_GELU;
-  if (kind == 0) kind = p.M <= 64 && (int64_t)p.M * p.N <= 1 << 18 ? 1 : (plain && t4 <= t3 && t4 <= t2 ? 4 : (t3 <= t2 ? 3 : 2));
+  if (kind == 0) kind = (int64_t)p.M * p.N <= (p.M <= 64 ? 1 << 18 : 1 << 17) ? 1 : (plain && t4 <= t3 && t4 <= t2 ? 4 : (t3 <= t2 ? 3 : 2));
   if (kind == 4 && plain) return p.residual ? tile_launch<Tile256, EPI_RESIDUAL>(p, s) : tile_launch<Tile256, EPI_PLAIN>(p, s);
   if (kind >= 3) return tile_any<Tile128>(p, plain, s);
   if (kind == 2) return tile_any<Tile64>(p, plain, s);
