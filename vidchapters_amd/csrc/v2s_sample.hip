@@ -321,29 +321,38 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
 
   // The last kept token of the boundary's bin, as an order key: the first one at which the running sum of `value` over the bin's tokens in order reaches
   // the goal; `in` = tokens that take part at all.  On the way the thread's tokens that take part are told apart (ROW, a bit each): those in the bins
-  // before the boundary's, and those in it.
-  uint32_t sure = 0, maybe = 0;
+  // before the boundary's, and those in it.  After a cut `pass` has the thread's tokens that it left, and the next passes visit only these.
+  uint32_t sure = 0, maybe = 0, pass = 0;
+  bool told = false, few = false;           // pass describes the cut; it left so few tokens that visiting them one by one is faster than all in order
+  auto logit = [&](int b) { return zs[place(group(b >> 2)) * 4 + (b & 3)]; };
+  auto visit = [&](uint32_t m, auto f) {    // f(bit, index, logit)
+    for (; m; m &= m - 1) { const int b = __builtin_ctz(m); f(b, tid * cpt * 4 + b, logit(b)); }
+  };
   auto resolve = [&](auto in, auto value, auto reached) -> u64 {
     const u64 base = s_base;
     const float lo = (float)s_bin, hi = (float)(s_bin + 1);
     sure = maybe = 0;
-#pragma unroll 1
-    for (int j = 0; j < nj; ++j) {
-      float z[4];
-      get(j, z);
-      const int idx = group(j) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float far = far_of(z[i]);
-        if (far < hi && in(z[i], idx + i)) {
-          if (far < lo) {
-            if constexpr (ROW) sure |= 1u << (j * 4 + i);
-          } else {
-            if constexpr (ROW) maybe |= 1u << (j * 4 + i);
-            const int at = atomicAdd(&s_n, 1);
-            if (at < CAP) { s_key[at] = order_key(z[i], idx + i); s_w[at] = value(z[i]); }
-          }
+    auto sort = [&](int b, int idx, float z) {
+      const float far = far_of(z);
+      if (far < hi && in(z, idx)) {
+        if (far < lo) {
+          if constexpr (ROW) sure |= 1u << b;
+        } else {
+          if constexpr (ROW) maybe |= 1u << b;
+          const int at = atomicAdd(&s_n, 1);
+          if (at < CAP) { s_key[at] = order_key(z, idx); s_w[at] = value(z); }
         }
+      }
+    };
+    if (ROW && few) {
+      visit(pass, sort);
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < nj; ++j) {
+        float z[4];
+        get(j, z);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sort(j * 4 + i, group(j) * 4 + i, z[i]);
       }
     }
     __syncthreads();
@@ -379,8 +388,14 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   float thr_z = -INFINITY;
   int thr_i = V;
   auto upto = [&](float z, int idx) { return z > thr_z || (z == thr_z && idx <= thr_i); };
-  auto set_thr = [&](u64 key) { thr_z = key_logit(key); thr_i = (int)(uint32_t)key; };
-  bool told = false;                        // sure and maybe describe the final cut
+  auto set_thr = [&](u64 key) {
+    thr_z = key_logit(key); thr_i = (int)(uint32_t)key;
+    if constexpr (ROW) {
+      pass = sure;
+      visit(maybe, [&](int b, int idx, float z) { pass |= upto(z, idx) ? 1u << b : 0u; });
+      told = true;
+    }
+  };
   if (cut_k) {
     each([&](int, float z) { const int b = bin_of(z); if (b < NBIN - 1) atomicAdd(&s_cnt[b], 1u); });
     __syncthreads();
@@ -388,7 +403,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     find_bin([&](int b) { return s_cnt[b]; }, [&](u64 s) { return s >= k; });
     if (s_bin < NBIN - 1) {                 // otherwise every token with any mass is among the first k
       set_thr(resolve([](float, int) { return true; }, [](float) { return (u64)1; }, [&](u64 s) { return s >= k; }));
-      told = true;
+      few = told && p.top_k < V / 4;
     }
     __syncthreads();
     clear();
@@ -399,7 +414,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
       const float far = far_of(z);
       if (far < (float)(NBIN - 1)) { const u64 m = mass_of(weight(z)); total += m; atomicAdd(&s_mass[(int)far], m); }
     };
-    if (cut_k) each([&](int idx, float z) { if (upto(z, idx)) add(z); });
+    if (ROW && few) visit(pass, [&](int, int, float z) { add(z); });
+    else if (cut_k) each([&](int idx, float z) { if (upto(z, idx)) add(z); });
     else each([&](int, float z) { add(z); });
     total = block_sum64(total, s_red, tid);
     const double goal = p.top_p * (double)total;
@@ -407,7 +423,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     find_bin([&](int b) { return s_mass[b]; }, reached);
     if (cut_k) set_thr(resolve(upto, [&](float z) { return mass_of(weight(z)); }, reached));
     else set_thr(resolve([](float, int) { return true; }, [&](float z) { return mass_of(weight(z)); }, reached));
-    told = true;
     __syncthreads();
   }
 
@@ -432,11 +447,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   };
   if constexpr (ROW) {
     // mass of each thread's consecutive tokens: only the kept ones are weighed, two at a time (a weight is one long chain)
-    auto logit = [&](int b) { return zs[place(group(b >> 2)) * 4 + (b & 3)]; };
-    uint32_t pass = sure;
-    if (told) {
-      for (uint32_t m = maybe; m; m &= m - 1) { const int b = __builtin_ctz(m); pass |= upto(logit(b), tid * cpt * 4 + b) ? m & -m : 0u; }
-    } else {
+    if (!told) {
 #pragma unroll 1
       for (int j = 0; j < nj; ++j) {
         float z[4];
