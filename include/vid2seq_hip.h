@@ -500,9 +500,9 @@ int v2s_sample_step(const void* logits, int32_t logits_dtype, int64_t ld, int32_
 
 /* ------------------------------------------------------------------------------------------------
  * 8-bit decoding: int8 codes with fp32 scales (the values they stand for are scale * code)
- *   a row y gets  scale = max(amax|y|, 127 * 2^-126) / 127,  code = round_to_even(y / scale) (the quotient to four fp32 roundings, so that a value is off by
- *   at most scale / 2 (1 + 2^-14));  a row that holds a NaN or an infinity gets scale NaN and
- *   zero codes, so that every value of it is read back as NaN.
+ *   a row y gets  scale = max(amax|y|, 127 * 2^-126) / 127,  code = round_to_even(y / scale) (as y * (127 / amax), both rounded to fp32, so that a value
+ *   is off by at most scale / 2 (1 + 2^-14));  a row that holds a NaN or an infinity gets scale NaN and zero codes, so that every value of it is read back
+ *   as NaN.
  * ---------------------------------------------------------------------------------------------- */
 /* codes q[rows][ldq] and scale[rows] of the rows of x (bf16 or fp32 [rows][ldx]): weights once (a scale per output channel), activations per token.
  * cols a multiple of 8, <= 8192; x 16-byte, q 8-byte aligned, strides multiples of 8. */

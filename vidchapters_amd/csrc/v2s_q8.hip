@@ -1,7 +1,7 @@
 // 8-bit decoding for gfx950: rows of activations to int8 codes with one fp32 scale per row (with the residual addition and the RMSNorm in
 // front of it), the int8 key / value cache, and the single-query attention that reads it.
-//   code q and scale s of a row y:  s = max(amax|y|, 127 * 2^-126) / 127,  q = round_to_even(y * (127 / amax)).  That factor and s carry four fp32 roundings
-//   in all, 127 codes times 2^-22, so that |y - s q| <= s / 2 (1 + 2^-14)
+//   code q and scale s of a row y:  s = max(amax|y|, 127 * 2^-126) / 127,  q = round_to_even(y * (127 / amax)).  s, that factor and the product are rounded
+//   once each to fp32, so that |y - s q| <= s / 2 (1 + 2^-14)
 // The floor of s keeps 1 / s finite: rows below it (1.5e-36) keep the smallest normal scale and fewer codes.  A row that holds a NaN or an
 // infinity gets s = NaN and zero codes: every value that is read back is NaN, none of them is a plausible number.
 //   RMSNorm: model/modeling_t5.py:263-277 (T5LayerNorm.forward); the cache it replaces: model/modeling_t5.py:555-556
@@ -21,11 +21,13 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   for (int o = 32; o > 0; o >>= 1) { const uint32_t w = (uint32_t)__shfl_xor((int)v, o, 64); v = v > w ? v : w; }
   return v;
 }
-// scale of a row whose largest magnitude has these bits (the maximum is taken on the bits: infinities and NaN are the largest), and 1 / scale
+// scale of a row whose largest magnitude has these bits (the maximum is taken on the bits: infinities and NaN are the largest), and 1 / scale; the quotient by
+// 127 is the correctly rounded one (product with 1 / 127, corrected by its remainder)
 __device__ __forceinline__ void q8_scale(uint32_t amax, float& scale, float& inv) {
   const float a = fmaxf(__uint_as_float(amax), Q8_TINY);
   const bool ok = amax < 0x7f800000u;
-  scale = ok ? a * (1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
+  const float s = a * (1.0f / 127.0f);
+  scale = ok ? fmaf(fmaf(-127.0f, s, a), 1.0f / 127.0f, s) : __uint_as_float(0x7fc00000u);
   inv = ok ? 127.0f / a : 0.f;
 }
 __device__ __forceinline__ uint32_t q8_pack4(const float* y, float inv, bool ok) {
