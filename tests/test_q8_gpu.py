@@ -41,7 +41,7 @@ def check_codes(q, scale, y, slack):
     assert int(q.abs().amax()) <= 127
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 8), (3, 64), (5, 72), (64, 768), (37, 1024), (9, 1032), (7, 2048), (6, 4096), (3, 8192), (1025, 520)])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (3, 64), (5, 72), (131, 128), (67, 136), (35, 256), (9, 264), (64, 768), (37, 1024), (9, 1032), (7, 2048), (6, 4096), (3, 8192), (1025, 520)])
 @pytest.mark.parametrize("dtype", [BF, torch.float32])
 def test_quant_rows(rows, cols, dtype):
     x = rnd(rows, cols, seed=rows, dtype=dtype) * torch.logspace(-3, 3, rows, device=DEV)[:, None].to(dtype)
@@ -54,7 +54,7 @@ def test_quant_rows(rows, cols, dtype):
     assert ((y.double() - want).abs() <= want.abs() * (UBF + 2 * U32)).all()
 
 
-@pytest.mark.parametrize("rows,cols,add,store", [(1, 8, True, True), (64, 768, True, True), (65, 768, True, False), (33, 1024, False, False), (5, 2040, True, True),
+@pytest.mark.parametrize("rows,cols,add,store", [(1, 8, True, True), (77, 48, True, True), (50, 128, False, False), (33, 248, True, True), (64, 768, True, True), (65, 768, True, False), (33, 1024, False, False), (5, 2040, True, True),
                                                  (4, 4096, True, True), (2, 8192, False, False), (4099, 768, True, True)])
 def test_rmsnorm_q8(rows, cols, add, store):
     x, d = rnd(rows, cols, seed=1, scale=2.0), rnd(rows, cols, seed=2)

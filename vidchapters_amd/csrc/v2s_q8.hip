@@ -16,11 +16,33 @@ typedef __attribute__((ext_vector_type(2))) int i32x2;
 constexpr float Q8_TINY = 127.0f * 1.17549435e-38f;
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { const uint32_t w = (uint32_t)__shfl_xor((int)v, o, 64); v = v > w ? v : w; }
-  return v;
+// Reductions on the vector unit: rotations and mirrors within rows of 16 lanes, swaps of half waves and of odd and even rows across them (a shuffle through
+// LDS has over ten times the latency, which is what a call of a few rows consists of).  Every lane gets the result.
+template <int CTRL, class T> __device__ __forceinline__ T dpp(T v) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
+template <class T, class F> __device__ __forceinline__ T half_reduce(T v, F f) {      // lane and lane ^ 32
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return f(__builtin_bit_cast(T, (uint32_t)a[0]), __builtin_bit_cast(T, (uint32_t)a[1]));
+}
+template <class T, class F> __device__ __forceinline__ T pair_reduce(T v, F f) {      // lane and lane ^ 16
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return f(__builtin_bit_cast(T, (uint32_t)a[0]), __builtin_bit_cast(T, (uint32_t)a[1]));
+}
+template <class T, class F> __device__ __forceinline__ T rows_reduce(T v, F f) { return pair_reduce(half_reduce(v, f), f); }      // the lanes with the same lane & 15
+// over groups of LPR lanes
+template <int LPR, class T, class F> __device__ __forceinline__ T group_reduce(T v, F f) {
+  v = f(v, dpp<0x128>(v)); v = f(v, dpp<0x124>(v)); v = f(v, dpp<0x122>(v)); v = f(v, dpp<0x121>(v));      // row_ror 8, 4, 2, 1
+  if (LPR >= 32) v = pair_reduce(v, f);
+  return LPR == 64 ? half_reduce(v, f) : v;
+}
+struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
+};
 // scale of a row whose largest magnitude has these bits (the maximum is taken on the bits: infinities and NaN are the largest), and 1 / scale; the quotient by
 // 127 is the correctly rounded one (product with 1 / 127, corrected by its remainder)
 __device__ __forceinline__ void q8_scale(uint32_t amax, float& scale, float& inv) {
@@ -67,11 +89,12 @@ __device__ __forceinline__ void ld8(const float* p, float* f) {
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
-// one wave per row, NCH chunks of 512 columns held in registers: every byte is read once and written once
-template <typename T, int NCH, bool NORM>
+// LPR lanes per row (a wave, unless the row is shorter than half of one), NCH chunks of 8 LPR columns held in registers: every byte is read once and written
+// once.  32000 x 768 with the residual: 28 us, 5.3 TB/s; 64 x 768: 3.6 us, of which a row's chain of loads and reductions is one.
+template <typename T, int NCH, int LPR, bool NORM>
 __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & (LPR - 1);
+  const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   if (row >= p.rows) return;
   const int nch = p.cols >> 3;
   const T* x = (const T*)p.x + (long)row * p.ldx;
@@ -80,7 +103,7 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
   uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = lane + i * 64;
+    const int c = lane + i * LPR;
     if (c < nch) {
       ld8(x + c * 8, v[i]);
     } else {
@@ -88,11 +111,17 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
     }
   }
+  constexpr bool EARLY = NCH <= 4;      // weights of the norm under the row's reduction, as far as registers go
+  float w[EARLY ? NCH : 1][8];
   if (NORM) {
+    if (EARLY) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) if (lane + i * LPR < nch) ld8(p.w + (lane + i * LPR) * 8, w[i]);
+    }
     if (p.delta) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const int c = lane + i * 64;
+        const int c = lane + i * LPR;
         if (c < nch) {
           float d[8];
           ld8(p.delta + (long)row * p.ldd + c * 8, d);
@@ -108,15 +137,14 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
-    const float rstd = rsqrtf(wave_sum(ss) / p.cols + p.eps);
+    const float rstd = rsqrtf(group_reduce<LPR>(ss, Add()) / p.cols + p.eps);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = lane + i * 64;
+      const int c = lane + i * LPR;
       if (c < nch) {
-        float w[8];
-        ld8(p.w + c * 8, w);
+        if (!EARLY) ld8(p.w + c * 8, w[0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = w[j] * (v[i][j] * rstd);
+        for (int j = 0; j < 8; ++j) v[i][j] = w[EARLY ? i : 0][j] * (v[i][j] * rstd);
       }
     }
   }
@@ -124,14 +152,14 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(v[i][j]); amax = amax > b ? amax : b; }
-  amax = wave_umax(amax);
+  amax = group_reduce<LPR>(amax, Max());
   float scale, inv;
   q8_scale(amax, scale, inv);
   const bool ok = amax < 0x7f800000u;
   if (lane == 0) p.scale[row] = scale;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int c = lane + i * 64;
+    const int c = lane + i * LPR;
     if (c < nch) {
       uint2 o;
       o.x = q8_pack4(v[i], inv, ok); o.y = q8_pack4(v[i] + 4, inv, ok);
@@ -171,7 +199,7 @@ struct KvQ8 {
 
 // eight lanes per (entry, head, token); TOKENS: eight tokens of one head per wave (512 contiguous bytes of codes), else eight heads of one token
 template <bool TOKENS>
-__device__ __forceinline__ bool kv_unit(const KvQ8& p, int& e, int& h, int& t, int& at) {
+__device__ __forceinline__ bool kv_unit(const KvQ8& p, int& e, int& h, int& t) {
   const uint32_t u = blockIdx.x * 32u + (threadIdx.x >> 3);
   if (TOKENS) {
     const uint32_t tp = (uint32_t)(p.T + 7) & ~7u;
@@ -182,21 +210,25 @@ __device__ __forceinline__ bool kv_unit(const KvQ8& p, int& e, int& h, int& t, i
     const uint32_t et = u / hp;
     h = (int)(u - et * hp); t = (int)(et % (uint32_t)p.T); e = (int)(et / (uint32_t)p.T);
   }
-  if (e >= p.E || h >= p.H || t >= p.T) return false;
-  if (p.count && t >= p.count[e]) return false;
-  const long a = (long)(p.pos ? p.pos[e] : p.pos0) + (p.pos_dev ? *p.pos_dev : 0) + t;
-  at = (int)a;
-  return a >= 0 && a < p.maxlen;     // a token behind the cache's end has no row
+  return e < p.E && h < p.H && t < p.T;
+}
+// cache row of a unit; false if it takes no part, or has no row: a token behind the cache's end
+__device__ __forceinline__ bool kv_row(const KvQ8& p, int e, int h, int t, long& row) {
+  const long at = (long)(p.pos ? p.pos[e] : p.pos0) + (p.pos_dev ? *p.pos_dev : 0) + t;
+  row = (long)e * p.e_rows + (long)h * p.h_rows + at;
+  return !(p.count && t >= p.count[e]) && at >= 0 && at < p.maxlen;
 }
 
 template <bool TOKENS>
 __global__ __launch_bounds__(256) void kv_append_q8_kernel(const KvQ8 p) {
-  int e = 0, h = 0, t = 0, at = 0;
-  if (!kv_unit<TOKENS>(p, e, h, t, at)) return;      // whole groups of eight lanes
+  int e = 0, h = 0, t = 0;
+  long row;
+  if (!kv_unit<TOKENS>(p, e, h, t)) return;          // whole groups of eight lanes
+  if (TOKENS && !kv_row(p, e, h, t, row)) return;
   const int c = threadIdx.x & 7;
   const long src = (long)e * p.bs + (long)t * p.rs + h * 64 + c * 8;
   const uint4 kr = *reinterpret_cast<const uint4*>(p.k + src), vr = *reinterpret_cast<const uint4*>(p.v + src);
-  const long row = (long)e * p.e_rows + (long)h * p.h_rows + at;
+  if (!TOKENS && !kv_row(p, e, h, t, row)) return;   // few tokens: the position arrives together with them, not in front of them
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     float f[8];
@@ -204,8 +236,7 @@ __global__ __launch_bounds__(256) void kv_append_q8_kernel(const KvQ8 p) {
     uint32_t amax = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(f[j]); amax = amax > b ? amax : b; }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) { const uint32_t b = (uint32_t)__shfl_xor((int)amax, o, 64); amax = amax > b ? amax : b; }
+    amax = Max()(amax, dpp<0xB1>(amax)); amax = Max()(amax, dpp<0x4E>(amax)); amax = Max()(amax, dpp<0x141>(amax));      // quad permutes, half mirror: eight lanes
     float scale, inv;
     q8_scale(amax, scale, inv);
     const bool ok = amax < 0x7f800000u;
@@ -218,11 +249,11 @@ __global__ __launch_bounds__(256) void kv_append_q8_kernel(const KvQ8 p) {
 
 template <bool TOKENS>
 __global__ __launch_bounds__(256) void kv_read_q8_kernel(const KvQ8 p) {
-  int e = 0, h = 0, t = 0, at = 0;
-  if (!kv_unit<TOKENS>(p, e, h, t, at)) return;
+  int e = 0, h = 0, t = 0;
+  long row;
+  if (!kv_unit<TOKENS>(p, e, h, t) || !kv_row(p, e, h, t, row)) return;
   const int c = threadIdx.x & 7;
   const long dst = (long)e * p.bs + (long)t * p.rs + h * 64 + c * 8;
-  const long row = (long)e * p.e_rows + (long)h * p.h_rows + at;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const uint2 u = *reinterpret_cast<const uint2*>((w ? p.vq : p.kq) + row * 64 + c * 8);
@@ -281,14 +312,6 @@ __device__ float attn_q8_mean(const i8* vq, const float* vs, int n, float* lds) 
   s = lds[d] + lds[64 + d] + lds[128 + d] + lds[192 + d];
   __syncthreads();
   return n > 0 ? s / (float)n : 0.f;
-}
-
-// reduction over the lanes with the same lane & 15, by the swaps of half waves and of odd and even rows (a shuffle through LDS has five times the latency)
-template <class F> __device__ __forceinline__ float rows_reduce(float v, F f) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // eight codes as bf16, exactly
@@ -423,7 +446,7 @@ __global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
     float mn = sc[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mn = fmaxf(mn, sc[i]);
-    mn = rows_reduce(mn, [](float a, float b) { return fmaxf(a, b); });
+    mn = rows_reduce(mn, Max());
     mn = fmaxf(mn, m);
     const float a = rescale(m, mn);
     m = mn;
@@ -458,7 +481,7 @@ __global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
     }
   }
   // join the waves: [query][64] sums per wave in the wave's own tile
-  l = rows_reduce(l, [](float a, float b) { return a + b; });
+  l = rows_reduce(l, Add());
   float* const so = reinterpret_cast<float*>(vt);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<f32x4*>(so + qi * 64 + dt * 16 + g * 4) = acc[dt];
@@ -506,9 +529,6 @@ __global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
 // computes a softmax, so the fp32 pipe needs a third fewer instructions here.
 // 32 x 16 heads x 5000 keys: 68 us with the join, 5.1 TB/s; twice the waves per block: 8 x 12 heads x 1200 keys 7.7 instead of 8.7 us, but 64 x 12 x 300
 // keys 11.1 instead of 9.6.
-template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
 constexpr int W1 = 4;
 __global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {
   __shared__ float s_m[W1], s_l[W1], s_o[W1][64], s_red[256];
@@ -563,8 +583,8 @@ __global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) d = fmaf(qv[4 * i + t], f[t], d);
       }
-      d = dpp_add<0xB1>(d);                          // the four lanes of a key: quad permutes [1,0,3,2] and [2,3,0,1]
-      d = dpp_add<0x4E>(d);
+      d += dpp<0xB1>(d);                             // the four lanes of a key: quad permutes [1,0,3,2] and [2,3,0,1]
+      d += dpp<0x4E>(d);
       const bool see = (bits >> (j * 16 + slot)) & 1ull && !(bz[j] == -INFINITY);
       const float z = fmaf(d, sk[j] * p.scale, bz[j]);
       sc[j] = see ? z : -INFINITY;
@@ -592,19 +612,17 @@ __global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {
   }
   // the 16 key slots of the wave, then the waves
   float M = m;
-#pragma unroll
-  for (int o = 4; o < 16; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  M = rows_reduce(M, [](float x, float y) { return fmaxf(x, y); });
+  M = fmaxf(M, dpp<0x128>(M)); M = fmaxf(M, dpp<0x124>(M));
+  M = rows_reduce(M, Max());
   const float a = rescale(m, M);
   float L = l * a;
-  L = dpp_add<0x128>(L); L = dpp_add<0x124>(L);      // row_ror 8 and 4 keep lane & 3
-  const auto add = [](float x, float y) { return x + y; };
-  L = rows_reduce(L, add);
+  L += dpp<0x128>(L); L += dpp<0x124>(L);      // row_ror 8 and 4 keep lane & 3
+  L = rows_reduce(L, Add());
 #pragma unroll
   for (int d = 0; d < 16; ++d) {
     float x = acc[d] * a;
-    x = dpp_add<0x128>(x); x = dpp_add<0x124>(x);
-    x = rows_reduce(x, add);
+    x += dpp<0x128>(x); x += dpp<0x124>(x);
+    x = rows_reduce(x, Add());
     if (slot == 0) s_o[wave][c * 16 + d] = x;
   }
   if (lane == 0) { s_m[wave] = M; s_l[wave] = L; }
@@ -668,15 +686,19 @@ __global__ __launch_bounds__(256) void attn_q8_join_kernel(const AttnQ8 p) {
 
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-template <typename T, bool NORM> int rows_q8_launch(const RowsQ8& p, hipStream_t s) {
-  const dim3 grid((unsigned)((p.rows + 3) / 4)), block(256);      // rows < 2^26
-  if (p.cols <= 512) hipLaunchKernelGGL((rows_q8_kernel<T, 1, NORM>), grid, block, 0, s, p);
-  else if (p.cols <= 1024) hipLaunchKernelGGL((rows_q8_kernel<T, 2, NORM>), grid, block, 0, s, p);
-  else if (p.cols <= 2048) hipLaunchKernelGGL((rows_q8_kernel<T, 4, NORM>), grid, block, 0, s, p);
-  else if (p.cols <= 4096) hipLaunchKernelGGL((rows_q8_kernel<T, 8, NORM>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((rows_q8_kernel<T, 16, NORM>), grid, block, 0, s, p);
+template <typename T, int NCH, int LPR, bool NORM> int rows_q8_launch(const RowsQ8& p, hipStream_t s) {
+  hipLaunchKernelGGL((rows_q8_kernel<T, NCH, LPR, NORM>), dim3((unsigned)((p.rows + 256 / LPR - 1) / (256 / LPR))), dim3(256), 0, s, p);      // rows < 2^26
   V2S_LAUNCH_CHECK();
   return V2S_OK;
+}
+template <typename T, bool NORM> int rows_q8_any(const RowsQ8& p, hipStream_t s) {
+  if (p.cols <= 128) return rows_q8_launch<T, 1, 16, NORM>(p, s);
+  if (p.cols <= 256) return rows_q8_launch<T, 1, 32, NORM>(p, s);
+  if (p.cols <= 512) return rows_q8_launch<T, 1, 64, NORM>(p, s);
+  if (p.cols <= 1024) return rows_q8_launch<T, 2, 64, NORM>(p, s);
+  if (p.cols <= 2048) return rows_q8_launch<T, 4, 64, NORM>(p, s);
+  if (p.cols <= 4096) return rows_q8_launch<T, 8, 64, NORM>(p, s);
+  return rows_q8_launch<T, 16, 64, NORM>(p, s);
 }
 
 int kv_check(const char* who, const v2s_kv_q8* c, const void* k, const void* v, int64_t bs, int64_t rs, int32_t T) {
@@ -716,7 +738,7 @@ extern "C" int v2s_quant_rows_q8(const void* x, int32_t x_dtype, int64_t ldx, in
             "v2s_quant_rows_q8: x must be 16-byte and q 8-byte aligned, strides multiples of 8");
   RowsQ8 p = {};
   p.x = x; p.ldx = ldx; p.q = (i8*)q; p.ldq = ldq; p.scale = scale; p.rows = rows; p.cols = cols;
-  return x_dtype == V2S_F32 ? rows_q8_launch<float, false>(p, (hipStream_t)stream) : rows_q8_launch<bf16_t, false>(p, (hipStream_t)stream);
+  return x_dtype == V2S_F32 ? rows_q8_any<float, false>(p, (hipStream_t)stream) : rows_q8_any<bf16_t, false>(p, (hipStream_t)stream);
 }
 
 extern "C" int v2s_rmsnorm_q8(const void* x, int64_t ldx, const void* delta, int64_t ldd, const float* w, void* h, int64_t ldh, int8_t* q, int64_t ldq,
@@ -733,7 +755,7 @@ extern "C" int v2s_rmsnorm_q8(const void* x, int64_t ldx, const void* delta, int
   RowsQ8 p = {};
   p.x = x; p.ldx = ldx; p.delta = (const bf16_t*)delta; p.ldd = ldd; p.w = w; p.h = (bf16_t*)h; p.ldh = ldh; p.q = (i8*)q; p.ldq = ldq; p.scale = scale;
   p.rows = rows; p.cols = cols; p.eps = eps;
-  return rows_q8_launch<bf16_t, true>(p, (hipStream_t)stream);
+  return rows_q8_any<bf16_t, true>(p, (hipStream_t)stream);
 }
 
 extern "C" int v2s_dequant_q8(const int8_t* q, int64_t ldq, const float* scale, void* y, int64_t ldy, int32_t rows, int32_t cols, void* stream) {
