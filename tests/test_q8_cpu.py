@@ -24,7 +24,7 @@ def test_rows_refusals():
     l = L.lib()
     ok = dict(x=P, dt=0, ldx=64, q=P, ldq=64, s=P, rows=4, cols=64)
     for change, word in ((dict(x=None), "NULL"), (dict(s=None), "NULL"), (dict(dt=7), "bf16 or fp32"), (dict(cols=60), "multiple of 8"), (dict(cols=8200, ldx=8200, ldq=8200), "8192"),
-                         (dict(rows=0), "rows=0"), (dict(rows=1 << 26), "2^26"), (dict(ldx=56), "shorter"), (dict(ldq=63), "shorter"), (dict(ldx=68), "multiples of 8"), (dict(x=P + 2), "aligned"),
+                         (dict(rows=0), "rows=0"), (dict(rows=1 << 24), "2^24"), (dict(ldx=56), "shorter"), (dict(ldq=63), "shorter"), (dict(ldx=68), "multiples of 8"), (dict(x=P + 2), "aligned"),
                          (dict(q=P + 4), "aligned")):
         a = {**ok, **change}
         refused(l.v2s_quant_rows_q8(a["x"], a["dt"], a["ldx"], a["q"], a["ldq"], a["s"], a["rows"], a["cols"], None), word)

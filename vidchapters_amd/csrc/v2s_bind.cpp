@@ -229,7 +229,7 @@ PyObject* sample_step(PyObject* const* a) {
   const at::Tensor &z = c.tensor(a[0], "logits"), &u = c.tensor(a[3], "u");
   const bool f32 = z.scalar_type() == at::kFloat, table = a[16] != Py_None;
   const int32_t rows = small(a[1], "rows"), V = small(a[2], "V");
-  const int64_t ld = or_default(a[5], z.dim() == 2 && rows > 1 ? z.stride(0) : V), seq_ld = integer(a[15]);
+  const int64_t ld = or_default(a[5], z.dim() == 2 && rows > 1 ? z.stride(0) : V), seq_ld = or_default(a[15], 0);
   if (u.dim() != (table ? 2 : 1) || u.size(-1) < rows)
     raise(PyExc_ValueError, "sample_step: u is [rows], or [steps, rows] with pos_dev, for " + std::to_string(rows) + " rows");
   const int64_t steps = table ? u.size(0) : 0, u_ld = !table ? 0 : (steps > 1 ? u.stride(0) : u.size(1));

@@ -32,11 +32,17 @@ template <class T, class F> __device__ __forceinline__ T pair_reduce(T v, F f) {
   return f(__builtin_bit_cast(T, (uint32_t)a[0]), __builtin_bit_cast(T, (uint32_t)a[1]));
 }
 template <class T, class F> __device__ __forceinline__ T rows_reduce(T v, F f) { return pair_reduce(half_reduce(v, f), f); }      // the lanes with the same lane & 15
-// over groups of LPR lanes
-template <int LPR, class T, class F> __device__ __forceinline__ T group_reduce(T v, F f) {
+// over groups of LPR lanes; 256: a block, through red[4]
+template <int LPR, class T, class F> __device__ __forceinline__ T group_reduce(T v, F f, T* red) {
   v = f(v, dpp<0x128>(v)); v = f(v, dpp<0x124>(v)); v = f(v, dpp<0x122>(v)); v = f(v, dpp<0x121>(v));      // row_ror 8, 4, 2, 1
   if (LPR >= 32) v = pair_reduce(v, f);
-  return LPR == 64 ? half_reduce(v, f) : v;
+  if (LPR >= 64) v = half_reduce(v, f);
+  if (LPR == 256) {
+    red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = f(f(red[0], red[1]), f(red[2], red[3]));
+  }
+  return v;
 }
 struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
 struct Max {
@@ -89,10 +95,13 @@ __device__ __forceinline__ void ld8(const float* p, float* f) {
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
-// LPR lanes per row (a wave, unless the row is shorter than half of one), NCH chunks of 8 LPR columns held in registers: every byte is read once and written
-// once.  32000 x 768 with the residual: 28 us, 5.3 TB/s; 64 x 768: 3.6 us, of which a row's chain of loads and reductions is one.
+// LPR lanes per row (a wave; fewer for a row shorter than half of one, a block for one longer than two), NCH chunks of 8 LPR columns held in registers: every byte is read once and written
+// once.  32000 x 768 with the residual: 28 us, 5.3 TB/s; 64 x 768: 3.5 us, a launch and one chain of loads and reductions.  A wave per row took 10.3 instead of
+// 4.3 us for 24017 x 48, 7.3 instead of 3.6 for 64 x 4096 and 46 instead of 36 for 4000 x 8192.
 template <typename T, int NCH, int LPR, bool NORM>
 __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
+  __shared__ float s_sum[4];
+  __shared__ uint32_t s_max[4];
   const int lane = threadIdx.x & (LPR - 1);
   const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   if (row >= p.rows) return;
@@ -111,13 +120,10 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
     }
   }
-  constexpr bool EARLY = NCH <= 4;      // weights of the norm under the row's reduction, as far as registers go
-  float w[EARLY ? NCH : 1][8];
+  float w[NCH][8];
   if (NORM) {
-    if (EARLY) {
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) if (lane + i * LPR < nch) ld8(p.w + (lane + i * LPR) * 8, w[i]);
-    }
+    for (int i = 0; i < NCH; ++i) if (lane + i * LPR < nch) ld8(p.w + (lane + i * LPR) * 8, w[i]);      // under the row's reduction
     if (p.delta) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
@@ -137,14 +143,13 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
-    const float rstd = rsqrtf(group_reduce<LPR>(ss, Add()) / p.cols + p.eps);
+    const float rstd = rsqrtf(group_reduce<LPR>(ss, Add(), s_sum) / p.cols + p.eps);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int c = lane + i * LPR;
       if (c < nch) {
-        if (!EARLY) ld8(p.w + c * 8, w[0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = w[EARLY ? i : 0][j] * (v[i][j] * rstd);
+        for (int j = 0; j < 8; ++j) v[i][j] = w[i][j] * (v[i][j] * rstd);
       }
     }
   }
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(v[i][j]); amax = amax > b ? amax : b; }
-  amax = group_reduce<LPR>(amax, Max());
+  amax = group_reduce<LPR>(amax, Max(), s_max);
   float scale, inv;
   q8_scale(amax, scale, inv);
   const bool ok = amax < 0x7f800000u;
@@ -687,7 +692,7 @@ __global__ __launch_bounds__(256) void attn_q8_join_kernel(const AttnQ8 p) {
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 template <typename T, int NCH, int LPR, bool NORM> int rows_q8_launch(const RowsQ8& p, hipStream_t s) {
-  hipLaunchKernelGGL((rows_q8_kernel<T, NCH, LPR, NORM>), dim3((unsigned)((p.rows + 256 / LPR - 1) / (256 / LPR))), dim3(256), 0, s, p);      // rows < 2^26
+  hipLaunchKernelGGL((rows_q8_kernel<T, NCH, LPR, NORM>), dim3((unsigned)((p.rows + 256 / LPR - 1) / (256 / LPR))), dim3(256), 0, s, p);      // rows < 2^24
   V2S_LAUNCH_CHECK();
   return V2S_OK;
 }
@@ -696,9 +701,9 @@ template <typename T, bool NORM> int rows_q8_any(const RowsQ8& p, hipStream_t s)
   if (p.cols <= 256) return rows_q8_launch<T, 1, 32, NORM>(p, s);
   if (p.cols <= 512) return rows_q8_launch<T, 1, 64, NORM>(p, s);
   if (p.cols <= 1024) return rows_q8_launch<T, 2, 64, NORM>(p, s);
-  if (p.cols <= 2048) return rows_q8_launch<T, 4, 64, NORM>(p, s);
-  if (p.cols <= 4096) return rows_q8_launch<T, 8, 64, NORM>(p, s);
-  return rows_q8_launch<T, 16, 64, NORM>(p, s);
+  if (p.cols <= 2048) return rows_q8_launch<T, 1, 256, NORM>(p, s);
+  if (p.cols <= 4096) return rows_q8_launch<T, 2, 256, NORM>(p, s);
+  return rows_q8_launch<T, 4, 256, NORM>(p, s);
 }
 
 int kv_check(const char* who, const v2s_kv_q8* c, const void* k, const void* v, int64_t bs, int64_t rs, int32_t T) {
@@ -731,8 +736,8 @@ unsigned kv_blocks(const KvQ8& p, bool tokens) {
 extern "C" int v2s_quant_rows_q8(const void* x, int32_t x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int32_t rows, int32_t cols, void* stream) {
   V2S_CHECK(x && q && scale, V2S_ERR_ARG, "v2s_quant_rows_q8: NULL pointer");
   V2S_CHECK(x_dtype == V2S_BF16 || x_dtype == V2S_F32, V2S_ERR_DTYPE, "v2s_quant_rows_q8: x must be bf16 or fp32");
-  V2S_CHECK(rows > 0 && rows < 1 << 26 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE,
-            "v2s_quant_rows_q8: unsupported shape rows=%d cols=%d (rows below 2^26, cols a multiple of 8, <= 8192)", rows, cols);
+  V2S_CHECK(rows > 0 && rows < 1 << 24 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE,
+            "v2s_quant_rows_q8: unsupported shape rows=%d cols=%d (rows below 2^24, cols a multiple of 8, <= 8192)", rows, cols);
   V2S_CHECK(ldx >= cols && ldq >= cols, V2S_ERR_SHAPE, "v2s_quant_rows_q8: a row stride is shorter than the row");
   V2S_CHECK(aligned(x, 16) && aligned(q, 8) && aligned(scale, 4) && ldx % 8 == 0 && ldq % 8 == 0, V2S_ERR_ALIGN,
             "v2s_quant_rows_q8: x must be 16-byte and q 8-byte aligned, strides multiples of 8");
@@ -746,8 +751,8 @@ extern "C" int v2s_rmsnorm_q8(const void* x, int64_t ldx, const void* delta, int
   V2S_CHECK(x && w && q && scale, V2S_ERR_ARG, "v2s_rmsnorm_q8: NULL pointer");
   V2S_CHECK(!h || delta, V2S_ERR_ARG, "v2s_rmsnorm_q8: h is the sum x + delta, it needs delta");
   V2S_CHECK(eps >= 0.f, V2S_ERR_ARG, "v2s_rmsnorm_q8: eps must not be negative");
-  V2S_CHECK(rows > 0 && rows < 1 << 26 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE,
-            "v2s_rmsnorm_q8: unsupported shape rows=%d cols=%d (rows below 2^26, cols a multiple of 8, <= 8192)", rows, cols);
+  V2S_CHECK(rows > 0 && rows < 1 << 24 && cols > 0 && cols % 8 == 0 && cols <= 8192, V2S_ERR_SHAPE,
+            "v2s_rmsnorm_q8: unsupported shape rows=%d cols=%d (rows below 2^24, cols a multiple of 8, <= 8192)", rows, cols);
   V2S_CHECK(ldx >= cols && ldq >= cols && (!delta || ldd >= cols) && (!h || ldh >= cols), V2S_ERR_SHAPE, "v2s_rmsnorm_q8: a row stride is shorter than the row");
   V2S_CHECK(aligned(x, 16) && aligned(delta, 16) && aligned(h, 16) && aligned(w, 16) && aligned(q, 8) && aligned(scale, 4) && ldx % 8 == 0 && ldq % 8 == 0 &&
                 (!delta || ldd % 8 == 0) && (!h || ldh % 8 == 0),
