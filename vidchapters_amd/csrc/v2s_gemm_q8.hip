@@ -84,12 +84,12 @@ template <int W> __device__ __forceinline__ typename Raw<W>::T pack(const float 
   for (int r = 0; r < W / 2; ++r) o[r] = pack_bf16(v[2 * r], v[2 * r + 1]);
   return o;
 }
-// the rest of the epilogue of four columns n .. n + 3 of row m, cut by N
-__device__ __forceinline__ void finish4(const GemmQ8& p, float (&v)[4], const Cols<4>& c, int m, int n) {
+// the rest of the epilogue of four columns n .. n + 3 of row m, cut by N; res: their residual where N does not cut them
+__device__ __forceinline__ void finish4(const GemmQ8& p, float (&v)[4], const Cols<4>& c, u32x2 res, int m, int n) {
   activate<4, true>(p, v, c);
   const long at = (long)m * p.ldc + n;
   if (n + 4 <= p.N) {
-    if (p.residual) add_residual<4>(v, residual_of<4>(p, m, n));
+    if (p.residual) add_residual<4>(v, res);
     if (p.c_f32) *reinterpret_cast<float4*>((float*)p.C + at) = make_float4(v[0], v[1], v[2], v[3]);
     else *reinterpret_cast<u32x2*>((bf16_t*)p.C + at) = pack<4>(v);
   } else {
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
           Cols<4> c;
 #pragma unroll
           for (int y = 0; y < 4; ++y) { c.s[y] = s_b[ch * 4 + y]; c.b[y] = s_b[BN + ch * 4 + y]; }
-          finish4(p, v, c, m, n);
+          finish4(p, v, c, p.residual ? residual_of<4>(p, m, n) : u32x2{}, m, n);
         }
       }
       __syncthreads();
@@ -416,6 +416,16 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_q8_skinny_kernel(const GemmQ8
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
   const int steps = (p.K + 63) >> 6, per = (steps + WAVES - 1) / WAVES;
   const int end = min(steps, (wave + 1) * per);
+  // what wave w < MT needs to finish 16 rows, asked for in front of the operands
+  const int m = m0 + wave * 16 + fr, n = n0 + fg * 4;
+  float sa = 0.f;
+  Cols<4> c = {};
+  u32x2 res = {};
+  if (wave < MT) {
+    sa = p.sA[min(m, p.M - 1)];
+    c = cols<4>(p, n);
+    if (p.residual) res = residual_of<4>(p, m, n);
+  }
   const i8* pa[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) pa[i] = p.A + (long)min(m0 + i * 16 + fr, p.M - 1) * p.lda;
@@ -446,11 +456,10 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_q8_skinny_kernel(const GemmQ8
   i32x4 v = red[0][wave][lane];
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) v += red[w][wave][lane];
-  const int m = m0 + wave * 16 + fr, n = n0 + fg * 4;
   if (m >= p.M || n >= p.N) return;
-  const float sa = p.alpha * p.sA[m];
+  sa *= p.alpha;
   float x[4] = {(float)v[0] * sa, (float)v[1] * sa, (float)v[2] * sa, (float)v[3] * sa};
-  finish4(p, x, cols<4>(p, n), m, n);
+  finish4(p, x, c, res, m, n);
 }
 
 template <class G, int EPI> int tile_launch(GemmQ8& p, hipStream_t s) {
