@@ -9,7 +9,7 @@
 // A row of up to 32768 logits is read from memory once and stays in LDS as fp32 (larger ones are read again for every pass, mostly from L2).  The
 // passes over it are bound by VALU issue, not by memory: one instruction per logit costs a block 0.2 us at V = 32228.  Hence: the weights' exponential
 // is a table and five terms of its own, small top-k never touches most logits, and the last pass compares all tokens but weighs only those it keeps.
-// 64 rows of 32228 logits, top-k 50 and top-p 0.95: 13 us; 256 rows, top-p 0.92 and min-p: 31 us, a third of it the exact masses.
+// 64 rows of 32228 logits, top-k 50 and top-p 0.95: 13 us; 256 rows, top-p 0.92 and min-p: 28 us, a third of it the exact masses.
 #include <math.h>
 #include "v2s_common.h"
 
@@ -24,7 +24,7 @@ constexpr float BIN_RANGE = 33.0f;          // exp(-33) < 2^-47: what lies furth
 constexpr double ONE = 70368744177664.0;    // 2^46: 131072 tokens of weight one sum to 2^63
 
 struct SampleP {
-  const void* logits; long ld; int V, vec, cpt, log_cpt;
+  const void* logits; long ld; int V, cpt, log_cpt;
   double inv_temp, exp2_scale; float bin_scale;   // 1 / T, log2(e) / T, bins per unit of logit
   int top_k; double top_p, min_p;
   const float* u; long u_ld; int u_steps;
@@ -42,16 +42,19 @@ __device__ __forceinline__ float key_logit(u64 key) {
   const uint32_t asc = ~(uint32_t)(key >> 32);
   return __uint_as_float((asc >> 31) ? asc ^ 0x80000000u : ~asc);
 }
-// 2^r for |r| <= 1 by the series of exp(r ln 2), 2^46 * 2^t for t <= 0 by a table of 2^(i / 64) and the first terms of the same series: t = n / 64 + r,
-// |r| <= 1 / 128 (remainder below 2^-54).  Sixteen instructions in 64 bits; the series alone took 25, the library's exp over 40.
+// 2^46 * 2^t for t <= 0 by a table of 2^(i / 64), which the compiler sums from the series of exp(i / 64 ln 2), and the first terms of the same series: t = n / 64
+// + r, |r| <= 1 / 128 (remainder below 2^-54).  Sixteen instructions in 64 bits; the series alone took 25, the library's exp over 40.
 constexpr double LN2 = 0.69314718055994530942;
-__device__ double exp2_series(double r) {
-  const double x = r * LN2;
-  double s = 1.0;
-#pragma unroll 1
-  for (int i = 19; i > 0; --i) s = fma(s * (1.0 / i), x, 1.0);
-  return s;
-}
+struct Powers {
+  double v[64];
+  constexpr Powers() : v() {
+    for (int i = 0; i < 64; ++i) {
+      v[i] = 1.0;
+      for (int k = 19; k > 0; --k) v[i] = v[i] * (i / 64.0 * LN2) / k + 1.0;
+    }
+  }
+};
+__device__ constexpr Powers POWERS;
 __device__ __forceinline__ double exp2_mass(double t, const double* tab) {
   constexpr double MAGIC = 105553116266496.0;      // 1.5 * 2^46: adding it leaves multiples of 1 / 64
   constexpr double C1 = LN2, C2 = C1 * LN2 / 2, C3 = C2 * LN2 / 3, C4 = C3 * LN2 / 4, C5 = C4 * LN2 / 5;
@@ -77,15 +80,18 @@ __device__ __forceinline__ u64 last_lane(u64 v) {
   return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63) | ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32);
 }
 __device__ __forceinline__ u64 wave_sum64(u64 v) { return last_lane(wave_scan(v)); }
+// sum of the first n of 16 numbers, by every wave for itself: a row of lanes reads and adds them (a loop over all of them costs a block 1000 cycles)
+__device__ __forceinline__ u64 first_sum(const u64* red, int n, int lane) {
+  u64 v = (lane & 15) < n ? red[lane & 15] : 0;
+  v += lane_step<0x128, 0xf>(v); v += lane_step<0x124, 0xf>(v); v += lane_step<0x122, 0xf>(v);      // row_ror 8, 4, 2, 1
+  return v + lane_step<0x121, 0xf>(v);
+}
 __device__ u64 block_sum64(u64 v, u64* red, int tid) {
   v = wave_sum64(v);
   __syncthreads();
   if ((tid & 63) == 0) red[tid >> 6] = v;
   __syncthreads();
-  u64 s = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) s += red[i];
-  return s;
+  return first_sum(red, NT / 64, tid & 63);
 }
 // u64 sums of a loop of independent LDS reads, eight in flight
 template <class F> __device__ __forceinline__ void list_loop(int n8, F f) {
@@ -95,19 +101,22 @@ template <class F> __device__ __forceinline__ void list_loop(int n8, F f) {
     for (int j = 0; j < 8; ++j) f(i + j);
   }
 }
-__device__ __forceinline__ void load4(const float* z, int i0, int V, int vec, float (&o)[4]) {
-  if (vec && i0 + 4 <= V) {
-    const float4 v = *reinterpret_cast<const float4*>(z + i0);
-    o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+// four consecutive logits in one load, whatever the row's alignment (one element at a time: 20000 instead of 8000 cycles for a row of 30113)
+__device__ __forceinline__ void load4(const float* z, int i0, int V, float (&o)[4]) {
+  typedef __attribute__((ext_vector_type(4), aligned(4))) float F4;
+  if (i0 + 4 <= V) {
+    const F4 v = *reinterpret_cast<const F4*>(z + i0);
+    o[0] = v[0]; o[1] = v[1]; o[2] = v[2]; o[3] = v[3];
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = i0 + i < V ? z[i0 + i] : -INFINITY;
   }
 }
-__device__ __forceinline__ void load4(const bf16_t* z, int i0, int V, int vec, float (&o)[4]) {
-  if (vec && i0 + 4 <= V) {
-    const uint2 v = *reinterpret_cast<const uint2*>(z + i0);
-    o[0] = __uint_as_float(v.x << 16); o[1] = __uint_as_float(v.x & 0xffff0000u); o[2] = __uint_as_float(v.y << 16); o[3] = __uint_as_float(v.y & 0xffff0000u);
+__device__ __forceinline__ void load4(const bf16_t* z, int i0, int V, float (&o)[4]) {
+  typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t U2;
+  if (i0 + 4 <= V) {
+    const U2 v = *reinterpret_cast<const U2*>(z + i0);
+    o[0] = __uint_as_float(v[0] << 16); o[1] = __uint_as_float(v[0] & 0xffff0000u); o[2] = __uint_as_float(v[1] << 16); o[3] = __uint_as_float(v[1] & 0xffff0000u);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = i0 + i < V ? bf2f(z[i0 + i]) : -INFINITY;
@@ -122,7 +131,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   __shared__ u64 s_mass[NBIN];
   __shared__ u64 s_key[CAP + 8], s_w[CAP + 8];
   __shared__ double s_tab[64];
-  __shared__ u64 s_red[NT / 64], s_thr, s_base;
+  __shared__ u64 s_red[NT / 64], s_scan[NT / 64], s_thr, s_base;
   __shared__ float s_max[NT / 64];
   __shared__ int s_n, s_bin, s_nan;
   uint32_t* const s_cnt = reinterpret_cast<uint32_t*>(s_mass);      // the counts of top-k, before the masses of top-p
@@ -135,7 +144,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   int edge = 0;                             // 1: the maximum is +infinity, its tokens share everything; -1: every token is -infinity, all are equal
 
   auto fetch = [&](int g, float (&z)[4]) {  // group g of four tokens as the caller's rules leave them; -0 becomes +0, behind the row -infinity
-    load4(z0, g * 4, V, p.vec, z);
+    load4(z0, g * 4, V, z);
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = g * 4 + i == ban ? -INFINITY : z[i] + 0.0f;
   };
@@ -171,7 +180,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     float z[ROW_MAX][4];
 #pragma unroll
     for (int j = 0; j < ROW_MAX; ++j) if (j < cpt) fetch(j * NT + tid, z[j]);       // every load in flight before the first is used
-    if (tid < 64) s_tab[tid] = exp2_series(tid / 64.0);
+    if (tid < 64) s_tab[tid] = POWERS.v[tid];
 #pragma unroll
     for (int j = 0; j < ROW_MAX; ++j)
       if (j < cpt) {
@@ -184,7 +193,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
         *reinterpret_cast<float4*>(zs + place(g) * 4) = make_float4(z[j][0], z[j][1], z[j][2], z[j][3]);
       }
   } else {
-    if (tid < 64) s_tab[tid] = exp2_series(tid / 64.0);
+    if (tid < 64) s_tab[tid] = POWERS.v[tid];
     each([&](int idx, float z) {
       if (z != z) nan_at = min(nan_at, idx);
       tmax = fmaxf(tmax, z);
@@ -196,8 +205,9 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   s_mass[tid] = 0; s_mass[tid + NT] = 0;
   __syncthreads();
   if (nan_at < V) atomicMin(&s_nan, nan_at);
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) zmax = fmaxf(zmax, s_max[i]);
+  zmax = s_max[lane & 15];
+  zmax = fmaxf(zmax, __uint_as_float(lane_step<0x128, 0xf>(__float_as_uint(zmax)))); zmax = fmaxf(zmax, __uint_as_float(lane_step<0x124, 0xf>(__float_as_uint(zmax))));
+  zmax = fmaxf(zmax, __uint_as_float(lane_step<0x122, 0xf>(__float_as_uint(zmax)))); zmax = fmaxf(zmax, __uint_as_float(lane_step<0x121, 0xf>(__float_as_uint(zmax))));
   __syncthreads();
 
   auto finish = [&](int tok, float lp) {    // one thread
@@ -242,13 +252,10 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   auto find_bin = [&](auto value, auto reached) {
     const auto a = value(2 * tid), b = value(2 * tid + 1);
     const auto inc = wave_scan(a + b);
-    __syncthreads();
-    if (lane == 63) s_red[wave] = inc;
+    if (lane == 63) s_scan[wave] = inc;
     if (tid == 0) { s_bin = NBIN - 1; s_n = 0; }
     __syncthreads();
-    u64 pre = inc - (a + b);
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) pre += i < wave ? s_red[i] : 0;
+    const u64 pre = inc - (a + b) + first_sum(s_scan, wave, lane);
     if (!reached(pre) && reached(pre + a)) { s_bin = 2 * tid; s_base = pre; }
     else if (!reached(pre + a) && reached(pre + a + b)) { s_bin = 2 * tid + 1; s_base = pre + a; }
     __syncthreads();
@@ -332,36 +339,45 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     const u64 base = s_base;
     const float lo = (float)s_bin, hi = (float)(s_bin + 1);
     sure = maybe = 0;
-    auto sort = [&](int b, int idx, float z) {
-      const float far = far_of(z);
-      if (far < hi && in(z, idx)) {
-        if (far < lo) {
-          if constexpr (ROW) sure |= 1u << b;
-        } else {
-          if constexpr (ROW) maybe |= 1u << b;
-          const int at = atomicAdd(&s_n, 1);
-          if (at < CAP) { s_key[at] = order_key(z, idx); s_w[at] = value(z); }
-        }
-      }
+    auto put = [&](int idx, float z) {
+      const int at = atomicAdd(&s_n, 1);
+      if (at < CAP) s_key[at] = order_key(z, idx);
     };
     if (ROW && few) {
-      visit(pass, sort);
+      visit(pass, [&](int b, int idx, float z) {
+        const float far = far_of(z);
+        if (far < lo) sure |= 1u << b;
+        else if (far < hi) { maybe |= 1u << b; put(idx, z); }
+      });
     } else {
 #pragma unroll 1
       for (int j = 0; j < nj; ++j) {
         float z[4];
         get(j, z);
+        uint32_t before = 0, here = 0;      // without branches for the many, the few of the boundary's bin one by one
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sort(j * 4 + i, group(j) * 4 + i, z[i]);
+        for (int i = 0; i < 4; ++i) {
+          const float far = far_of(z[i]);
+          before |= far < lo ? 1u << i : 0u;
+          here |= far >= lo && far < hi ? 1u << i : 0u;
+        }
+        for (uint32_t m = here; m; m &= m - 1) {
+          const int i = __builtin_ctz(m);
+          const float zi = i == 0 ? z[0] : i == 1 ? z[1] : i == 2 ? z[2] : z[3];
+          if (in(zi, group(j) * 4 + i)) put(group(j) * 4 + i, zi); else here &= ~(1u << i);
+        }
+        if constexpr (ROW) { sure |= before << (j * 4); maybe |= here << (j * 4); }
       }
     }
     __syncthreads();
     const int n = s_n, n8 = (n + 7) & ~7;
     if (n <= CAP) {
-      if (tid >= n && tid < n8) { s_key[tid] = ~0ull; s_w[tid] = 0; }
+      u64 key = ~0ull, w = 0;
+      if (tid < n) { key = s_key[tid]; w = value(key_logit(key)); }
+      else if (tid < n8) s_key[tid] = key;
+      if (tid < n8) s_w[tid] = w;
       __syncthreads();
       if (tid < n) {
-        const u64 key = s_key[tid], w = s_w[tid];
         u64 pre = base;
         list_loop(n8, [&](int i) { pre += s_key[i] < key ? s_w[i] : 0; });
         if (!reached(pre) && reached(pre + w)) s_thr = key;
@@ -469,26 +485,22 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     __syncthreads();
     if (lane == 63) s_red[wave] = inc;
     __syncthreads();
-    u64 pre = inc - own, total = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) { const u64 x = s_red[i]; pre += i < wave ? x : 0; total += x; }
+    const u64 pre = inc - own + first_sum(s_red, wave, lane), total = first_sum(s_red, NT / 64, lane);
     const double goal = u * (double)total;
     const bool here = own > 0 && ((double)(pre + own) > goal ? !((double)pre > goal) : pre + own == total && !((double)total > goal));
-    if (here) {                             // one thread of the block
-      u64 run = pre;
-      int tok = -1;
-      float zt = 0.f;
-      for (uint32_t m = pass; m; m &= m - 1) {
-        const int b = __builtin_ctz(m);
-        const float z = logit(b);
-        const u64 x = mass_kept(z);
-        if (x > 0) {
-          run += x;
-          tok = tid * cpt * 4 + b; zt = z;
-          if ((double)run > goal) break;
-        }
+    const u64 owner = __ballot(here);       // one thread of the block: its wave looks at that thread's tokens, a lane each
+    if (owner) {
+      const int src = __builtin_ctzll(owner), t = wave * 64 + src;
+      const uint32_t m = (uint32_t)__builtin_amdgcn_readlane((int)pass, src);
+      const u64 before = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)pre, src) | ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(pre >> 32), src) << 32);
+      float z = 0.f;
+      u64 x = 0;
+      if (lane < 32 && (m >> lane & 1)) {
+        z = zs[place(t * cpt + (lane >> 2)) * 4 + (lane & 3)];
+        x = mass_kept(z);
       }
-      finish(tok, log_prob(zt, total));
+      const u64 run = before + wave_scan(x), past = __ballot(x > 0 && (double)run > goal), any = __ballot(x > 0);
+      if (lane == (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any))) finish(t * cpt * 4 + lane, log_prob(z, total));
     }
   } else {
     // mass of each segment of 256 consecutive tokens (one wave of one step), segments in index order: [nj][16] <= 512; then within the drawn one
@@ -534,7 +546,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
 template <typename T> int sample_launch(SampleP& p, int rows, hipStream_t s) {
   const int nj = (p.V + STEP - 1) / STEP;
   p.log_cpt = nj <= 1 ? 0 : (nj <= 2 ? 1 : (nj <= 4 ? 2 : 3)); p.cpt = 1 << p.log_cpt;
-  p.vec = ((uintptr_t)p.logits % (4 * sizeof(T))) == 0 && p.ld % 4 == 0;
   if (nj <= ROW_MAX) {
     static bool attr = false;
     if (!attr) { (void)hipFuncSetAttribute((const void*)sample_kernel<T, true>, hipFuncAttributeMaxDynamicSharedMemorySize, ROW_MAX * STEP * 4); attr = true; }
