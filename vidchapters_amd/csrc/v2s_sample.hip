@@ -150,10 +150,11 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   };
   auto settle = [&](float z, int idx) { return edge > 0 ? (z == INFINITY ? 0.f : -INFINITY) : (edge < 0 && idx < V ? 0.f : z); };
   auto group = [&](int j) { return ROW ? tid * cpt + j : j * NT + tid; };
+  auto own = [&](int j) { return tid * cpt + ((j ^ tid) & (cpt - 1)); };      // place(group(j))
   auto place = [&](int g) { return (g & ~(cpt - 1)) | ((g ^ (g >> p.log_cpt)) & (cpt - 1)); };
   auto get = [&](int j, float (&z)[4]) {
     if constexpr (ROW) {
-      const float4 v = *reinterpret_cast<const float4*>(zs + place(group(j)) * 4);
+      const float4 v = *reinterpret_cast<const float4*>(zs + own(j) * 4);
       z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w;
     } else {
       fetch(group(j), z);
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   // before the boundary's, and those in it.  After a cut `pass` has the thread's tokens that it left, and the next passes visit only these.
   uint32_t sure = 0, maybe = 0, pass = 0;
   bool told = false, few = false;           // pass describes the cut; it left so few tokens that visiting them one by one is faster than all in order
-  auto logit = [&](int b) { return zs[place(group(b >> 2)) * 4 + (b & 3)]; };
+  auto logit = [&](int b) { return zs[own(b >> 2) * 4 + (b & 3)]; };
   auto visit = [&](uint32_t m, auto f) {    // f(bit, index, logit)
     for (; m; m &= m - 1) { const int b = __builtin_ctz(m); f(b, tid * cpt * 4 + b, logit(b)); }
   };
