@@ -249,14 +249,16 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   auto weight = [&](float z) -> double { return exp2_mass(((double)z - dmax) * p.exp2_scale, s_tab); };      // 2^46 w
   auto log_prob = [&](float z, u64 total) { return (float)(((double)z - dmax) * p.inv_temp - log((double)total / ONE)); };
 
-  // bin of the boundary: the first one at which the running sum (of counts or masses) reaches the goal; s_base = the sum before it
-  auto find_bin = [&](auto value, auto reached) {
+  // bin of the boundary: the first one at which the running sum (of counts or masses) reaches the goal, which `aim` may take from the whole sum; s_base = the
+  // sum before it
+  auto find_bin = [&](auto value, auto aim, auto reached) {
     const auto a = value(2 * tid), b = value(2 * tid + 1);
     const auto inc = wave_scan(a + b);
     if (lane == 63) s_scan[wave] = inc;
     if (tid == 0) { s_bin = NBIN - 1; s_n = 0; }
     __syncthreads();
     const u64 pre = inc - (a + b) + first_sum(s_scan, wave, lane);
+    aim(first_sum(s_scan, NT / 64, lane));
     if (!reached(pre) && reached(pre + a)) { s_bin = 2 * tid; s_base = pre; }
     else if (!reached(pre + a) && reached(pre + a + b)) { s_bin = 2 * tid + 1; s_base = pre + a; }
     __syncthreads();
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     if (b0 < NBIN - 1) atomicAdd(&s_cnt[b0], 1u);
     __syncthreads();
     const u64 k = (u64)p.top_k;
-    find_bin([&](int b) { return s_cnt[b]; }, [&](u64 s) { return s >= k; });
+    find_bin([&](int b) { return s_cnt[b]; }, [](u64) {}, [&](u64 s) { return s >= k; });
     const int bin = s_bin;
     if (bin < NBIN - 1) {
       const float limit = (float)(bin + 1);
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     each([&](int, float z) { const int b = bin_of(z); if (b < NBIN - 1) atomicAdd(&s_cnt[b], 1u); });
     __syncthreads();
     const u64 k = (u64)p.top_k;
-    find_bin([&](int b) { return s_cnt[b]; }, [&](u64 s) { return s >= k; });
+    find_bin([&](int b) { return s_cnt[b]; }, [](u64) {}, [&](u64 s) { return s >= k; });
     if (s_bin < NBIN - 1) {                 // otherwise every token with any mass is among the first k
       set_thr(resolve([](float, int) { return true; }, [](float) { return (u64)1; }, [&](u64 s) { return s >= k; }));
       few = told && p.top_k < V / 4;
@@ -426,18 +428,17 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
     clear();
   }
   if (p.top_p < 1.0) {
-    u64 total = 0;
     auto add = [&](float z) {
       const float far = far_of(z);
-      if (far < (float)(NBIN - 1)) { const u64 m = mass_of(weight(z)); total += m; atomicAdd(&s_mass[(int)far], m); }
+      if (far < (float)(NBIN - 1)) atomicAdd(&s_mass[(int)far], mass_of(weight(z)));
     };
     if (ROW && few) visit(pass, [&](int, int, float z) { add(z); });
     else if (cut_k) each([&](int idx, float z) { if (upto(z, idx)) add(z); });
     else each([&](int, float z) { add(z); });
-    total = block_sum64(total, s_red, tid);
-    const double goal = p.top_p * (double)total;
+    __syncthreads();
+    double goal = 0.0;
     const auto reached = [&](u64 s) { return (double)s >= goal; };
-    find_bin([&](int b) { return s_mass[b]; }, reached);
+    find_bin([&](int b) { return s_mass[b]; }, [&](u64 total) { goal = p.top_p * (double)total; }, reached);
     if (cut_k) set_thr(resolve(upto, [&](float z) { return mass_of(weight(z)); }, reached));
     else set_thr(resolve([](float, int) { return true; }, [&](float z) { return mass_of(weight(z)); }, reached));
     __syncthreads();
