@@ -9,7 +9,7 @@
 // A row of up to 32768 logits is read from memory once and stays in LDS as fp32 (larger ones are read again for every pass, mostly from L2).  The
 // passes over it are bound by VALU issue, not by memory: one instruction per logit costs a block 0.2 us at V = 32228.  Hence: the weights' exponential
 // is a table and five terms of its own, small top-k never touches most logits, and the last pass compares all tokens but weighs only those it keeps.
-// 64 rows of 32228 logits, top-k 50 and top-p 0.95: 13 us; 256 rows, top-p 0.92 and min-p: 28 us, a third of it the exact masses.
+// 64 rows of 32228 logits, top-k 50 and top-p 0.95: 11.5 us; 256 rows, top-p 0.92 and min-p: 28 us, a third of it the exact masses.
 #include <math.h>
 #include "v2s_common.h"
 
@@ -19,7 +19,7 @@ typedef unsigned long long u64;
 constexpr int NT = 1024, STEP = NT * 4;     // tokens per pass of the block: four consecutive ones per thread
 constexpr int NBIN = 2048, CAP = 512;
 constexpr int ROW_MAX = 8;                  // passes whose logits fit LDS: 32768 fp32 = 128 KiB, next to 24 KiB of tables
-constexpr int SMALL_K = 128, SMALL_N = 256; // top-k by candidate list: every step costs each candidate a walk over the others
+constexpr int SMALL_K = 128, SMALL_N = NT / 4; // top-k by candidate list: every step costs each candidate a walk over the others, four threads share it
 constexpr float BIN_RANGE = 33.0f;          // exp(-33) < 2^-47: what lies further from the maximum has no mass
 constexpr double ONE = 70368744177664.0;    // 2^46: 131072 tokens of weight one sum to 2^63
 
@@ -129,7 +129,7 @@ template <typename T, bool ROW>
 __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
   extern __shared__ __attribute__((aligned(16))) float zs[];
   __shared__ u64 s_mass[NBIN];
-  __shared__ u64 s_key[CAP + 8], s_w[CAP + 8];
+  __shared__ u64 s_key[CAP + 32], s_w[CAP + 32];
   __shared__ double s_tab[64];
   __shared__ u64 s_red[NT / 64], s_scan[NT / 64], s_thr, s_base;
   __shared__ float s_max[NT / 64];
@@ -291,36 +291,43 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
         }
       }
       __syncthreads();
-      const int n = s_n, n8 = (n + 7) & ~7;
+      const int n = s_n, pad = (n + 31) & ~31;
       if (n >= p.top_k && n <= SMALL_N) {   // the same for the whole block
-        if (tid >= n && tid < n8) s_key[tid] = ~0ull;
+        if (tid >= n && tid < pad) s_key[tid] = ~0ull;
         __syncthreads();
+        // four threads per candidate, each with a quarter of the list
+        const int c = tid >> 2, q = tid & 3;
+        auto quarter = [&](auto f) { list_loop(pad >> 2, [&](int i) { f(i * 4 + q); }); };
+        auto quad_sum = [](auto v) { v += lane_step<0xB1, 0xf>(v); return v + lane_step<0x4E, 0xf>(v); };      // quad permutes [1,0,3,2], [2,3,0,1]
         u64 key = ~0ull, w = 0;
         double wd = 0.0;
         float z = 0.f;
         bool in = false;
-        if (tid < n) {
-          key = s_key[tid];
+        if (c < n) {
+          key = s_key[c];
           z = key_logit(key);
-          int rank = 0;
-          list_loop(n8, [&](int i) { rank += s_key[i] < key ? 1 : 0; });
-          in = rank < p.top_k;
+          uint32_t rank = 0;
+          quarter([&](int i) { rank += s_key[i] < key ? 1u : 0u; });
+          in = (int)quad_sum(rank) < p.top_k;
           if (in) { wd = weight(z); w = mass_of(wd); }
         }
-        if (tid < n8) s_w[tid] = w;
+        if (q == 0 && c < pad) s_w[c] = w;
         __syncthreads();
         u64 total = 0, pre = 0;
-        if (tid < n) list_loop(n8, [&](int i) { const u64 x = s_w[i]; total += x; pre += s_key[i] < key ? x : 0; });
+        if (c < n) quarter([&](int i) { const u64 x = s_w[i]; total += x; pre += s_key[i] < key ? x : 0; });
+        total = quad_sum(total); pre = quad_sum(pre);
         __syncthreads();
         const bool keep = in && w > 0 && wd >= min_w && (p.top_p >= 1.0 || (double)pre < p.top_p * (double)total);
-        if (tid < n) s_w[tid] = keep ? w : 0;
+        if (q == 0 && c < n) s_w[c] = keep ? w : 0;
         __syncthreads();
-        if (keep) {
+        if (keep) {                         // the same for the four
           u64 run = 0;
           total = 0;
-          list_loop(n8, [&](int i) { const u64 x = s_w[i]; total += x; run += (uint32_t)s_key[i] <= (uint32_t)key ? x : 0; });
+          quarter([&](int i) { const u64 x = s_w[i]; total += x; run += (uint32_t)s_key[i] <= (uint32_t)key ? x : 0; });
+          total = quad_sum(total); run = quad_sum(run);
           const double goal = u * (double)total;
-          if (((double)run > goal && !((double)(run - w) > goal)) || (!((double)total > goal) && run == total)) finish((int)(uint32_t)key, log_prob(z, total));
+          if (q == 0 && (((double)run > goal && !((double)(run - w) > goal)) || (!((double)total > goal) && run == total)))
+            finish((int)(uint32_t)key, log_prob(z, total));
         }
         return;
       }
