@@ -165,21 +165,40 @@ def test_gemm_q8_every_kernel_gives_the_same_bits(M, N, K, kind):
 
 @pytest.mark.parametrize("kind", [2, 3, 4], ids=["64x64", "128x128", "256x256"])
 @pytest.mark.parametrize("out,act,res", [(BF, L.ACT_RELU, False), (BF, L.ACT_NONE, True), (BF, L.ACT_GELU, True), (torch.float32, L.ACT_NONE, False)])
-def test_gemm_q8_more_tiles_than_blocks(kind, out, act, res):
-    """A block that takes several tiles, with every form of the write-out and rows and columns left over."""
-    M, N, K = 5100, 4104, 144
+@pytest.mark.parametrize("N", [4104, 4099, 4101, 4094])
+def test_gemm_q8_more_tiles_than_blocks(kind, out, act, res, N):
+    """A block that takes several tiles, with every form of the write-out and rows and columns left over; the residual ends with its last value."""
+    M, K = 5100, 144
     A, sa = codes(M, K, 13)
     B, sb = codes(N, K, 14)
-    bias, r = rnd(N, seed=5, dtype=torch.float32), rnd(M, N, seed=6) if res else None
-    C = torch.full((M + 1, N), 7.0, dtype=out, device=DEV)
+    ld = (N + 7) // 8 * 8
+    bias, r = rnd(N, seed=5, dtype=torch.float32), rnd((M - 1) * ld + N, seed=6).as_strided((M, N), (ld, 1)) if res else None
+    C = torch.full((M + 1, ld), 7.0, dtype=out, device=DEV)
     L.set_option("gemm_q8", kind)
     try:
-        L.gemm_q8(A, B, sa, sb, C, M, N, K, bias=bias, act=act, residual=r)
+        L.gemm_q8(A, B, sa, sb, C, M, N, K, bias=bias, act=act, residual=r, ldc=ld, ldr=ld)
     finally:
         L.set_option("gemm_q8", 0)
     want, mag = product_ref(A, B, sa, sb, 1.0, bias, act, r)
     tol = mag * (7 if act != L.ACT_GELU else 16) * U32 + want.abs() * (UBF if out == BF else 0)
-    assert ((C[:M].double() - want).abs() <= tol).all() and (C[M:] == 7).all()
+    assert ((C[:M, :N].double() - want).abs() <= tol).all() and (C[M:] == 7).all() and (C[:, N:] == 7).all()
+
+
+def test_gemm_q8_few_columns_of_many_rows():
+    """Fewer than eight columns go to the few-row kernels, whatever is asked for."""
+    for M, N, K in ((70000, 1, 64), (40000, 5, 48), (66000, 7, 32)):
+        A, sa = codes(M, K, 3)
+        B, sb = codes(N, K, 4)
+        r = rnd((M - 1) * 8 + N, seed=6).as_strided((M, N), (8, 1))
+        want, mag = product_ref(A, B, sa, sb, 1.0, None, L.ACT_NONE, r)
+        for kind in (0, 2, 3, 4):
+            C = torch.full((M, 8), 7.0, dtype=BF, device=DEV)
+            L.set_option("gemm_q8", kind)
+            try:
+                L.gemm_q8(A, B, sa, sb, C, M, N, K, residual=r, ldc=8, ldr=8)
+            finally:
+                L.set_option("gemm_q8", 0)
+            assert ((C[:, :N].double() - want).abs() <= mag * 7 * U32 + want.abs() * UBF).all() and (C[:, N:] == 7).all()
 
 
 def test_gemm_q8_codes_are_summed_exactly():

@@ -47,6 +47,25 @@ template <int W> __device__ __forceinline__ typename Raw<W>::T residual_of(const
   if (m < p.M && n + W <= p.N) z = *reinterpret_cast<const typename Raw<W>::T*>(p.residual + (long)m * p.ldr + n);
   return z;
 }
+// elements e .. 7 of eight bf16 values, moved to the front
+__device__ __forceinline__ u32x4 from_element(u32x4 r, int e) {
+  const int d = e >> 1;
+  const uint32_t a0 = d == 0 ? r[0] : d == 1 ? r[1] : d == 2 ? r[2] : r[3], a1 = d == 0 ? r[1] : d == 1 ? r[2] : d == 2 ? r[3] : 0;
+  const uint32_t a2 = d == 0 ? r[2] : d == 1 ? r[3] : 0, a3 = d == 0 ? r[3] : 0;
+  const uint32_t h = (e & 1) * 16;
+  return u32x4{__builtin_amdgcn_alignbit(a1, a0, h), __builtin_amdgcn_alignbit(a2, a1, h), __builtin_amdgcn_alignbit(a3, a2, h), a3 >> h};
+}
+// 16 bytes, past the caches where a row is whole cache lines (12876 x 11520 x 240 to fp32: 132 instead of 144 us); pieces of a line that another tile completes
+// go through them (8601 x 2696 x 1440: 57 instead of 69)
+__device__ __forceinline__ void store16(u32x4 o, void* to, bool stream) {
+  if (stream) {
+    __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(to));
+  } else {
+    asm volatile("");                       // the two stay apart: merged into one store, they lose the hint
+    *reinterpret_cast<u32x4*>(to) = o;
+    asm volatile("");
+  }
+}
 // exact-erf GELU: v Phi(v) with Phi(v) = 1 / (1 + exp(-L(v))), L(v) = log(Phi(v) / Phi(-v)) = v P(v^2).  P is the weighted minimax polynomial of degree six
 // on v^2 <= 36 (error of v Phi below 7e-8, with the fp32 evaluation below 3 roundings of v), held at its last value beyond, where Phi is 0 or 1 to fp32; its
 // coefficients carry the factor -log2 e.  19 cycles' worth of instructions a value, a quarter less than a form with the two tails of erfc apart.
@@ -124,6 +143,14 @@ __device__ __forceinline__ void dma16(uint32_t off, const void* base, uint32_t d
 }
 // every DMA but the youngest N operations of this wave has landed and its LDS reads are done; then the same for the block
 template <int N> __device__ __forceinline__ void wait_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+
+// What lanes of a wave pass to each other through LDS needs no wait (a wave's LDS operations keep their order), but the compiler, which sees one lane, has to
+// be told that the words may have changed
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 template <int BM_, int BN_, int WM_, int WN_, int OCC_>
 struct Tile {
@@ -284,122 +311,106 @@ __global__ __launch_bounds__(G::THREADS, G::WAVES * G::OCC / 4) void gemm_q8_til
     const int m0w = m0 + wm, n0w = n0 + wn, tm = m0w + fr, tn = n0w + fg * (NI * 4);
     const bool more = (r + 1) * nwg + (int)blockIdx.x < ntiles;
     wait_barrier<0>();                      // scales visible, both stage images free
-    if (n0 + BN <= p.N || p.N % 8 == 0) {
-      // the next tile's first stages are requested, then 16 rows of the wave at a time: a lane finishes its 4 NI columns of one row, and the rows pass
-      // through LDS of the wave's own (fp32 ones in two halves) so that its stores write whole cache lines.  The residual is requested AHEAD steps early
-      constexpr int Q = NI / 2, CPL = NI * 2, AHEAD = MI < 4 ? MI : 4;      // groups of 8 columns of a lane, 16-byte chunks per row
-      const bf16_t* rp = p.residual + (long)tm * p.ldr + tn;
-      u32x4 res[AHEAD][Q];
-      auto fetch = [&](int i) {
+    // the next tile's first stages are requested, then 16 rows of the wave at a time: a lane finishes its 4 NI columns of one row, and the rows pass
+    // through LDS of the wave's own (fp32 ones in two halves) so that its stores write whole cache lines.  The residual is requested AHEAD steps early.  A
+    // group of 8 columns that N cuts takes the row's last 8 residuals from the right one on, and is stored by elements
+    constexpr int Q = NI / 2, CPL = NI * 2, AHEAD = MI < 4 ? MI : 4;      // groups of 8 columns of a lane, 16-byte chunks per row
+    const bf16_t* rp = p.residual + (long)tm * p.ldr + tn;
+    typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t U4;
+    const bool odd = p.N & 7;
+    int cut[Q];                             // columns of a lane's group behind N
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          res[i % AHEAD][q] = u32x4{0, 0, 0, 0};
-          if (tm + i * 16 < p.M && tn + q * 8 < p.N) res[i % AHEAD][q] = *reinterpret_cast<const u32x4*>(rp + (long)i * 16 * p.ldr + q * 8);
-        }
-      };
-      if (has_res) {
+    for (int q = 0; q < Q; ++q) cut[q] = max(0, tn + q * 8 + 8 - p.N);
+    u32x4 res[AHEAD][Q];
+    auto fetch = [&](int i) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) fetch(i);
+      for (int q = 0; q < Q; ++q) {
+        res[i % AHEAD][q] = u32x4{0, 0, 0, 0};
+        if (tm + i * 16 < p.M && cut[q] < 8) res[i % AHEAD][q] = *reinterpret_cast<const U4*>(rp + (long)i * 16 * p.ldr + q * 8 - cut[q]);
       }
-      const int mlim = p.M - m0w, nlim = p.N - n0w;
-      stored = m0 + BM <= p.M && n0 + BN <= p.N;
-      if (more) {
-        place(r + 1);
-        issue(0);
-        if (nst > 1) issue(1);
-      }
-      char* const out = smem + 2 * STG + wave * G::OUT;
-      const float *sb = s_b + wn + fg * (NI * 4), *sa = s_a + wm + fr;
-      const int sw = fr & (CPL - 1);
-      const int ch = lane % CPL, row0 = lane / CPL;      // what the lane stores: chunk ch of the rows row0 + q * 64 / CPL
-      const long at = (long)(m0w + row0) * p.ldc + n0w + ch * (f32 ? 4 : 8);
-      Cols<8> c[Q];
+    };
+    if (has_res) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q)
-#pragma unroll
-        for (int x = 0; x < 8; ++x) { c[q].s[x] = sb[q * 8 + x]; c[q].b[x] = sb[BN + q * 8 + x]; }
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const float a = sa[i * 16];
-        float v[Q][8];
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-#pragma unroll
-          for (int x = 0; x < 8; ++x) v[q][x] = (float)acc[i][q * 2 + (x >> 2)][x & 3] * a;
-          activate<8, EPI == EPI_ANY>(p, v[q], c[q]);
-          if (has_res) add_residual<8>(v[q], res[i % AHEAD][q]);
-        }
-        if (has_res && i + AHEAD < MI) fetch(i + AHEAD);
-        if (!f32) {
-#pragma unroll
-          for (int q = 0; q < Q; ++q) *reinterpret_cast<u32x4*>(out + fr * (NI * 32) + ((fg * Q + q) ^ sw) * 16) = pack<8>(v[q]);
-#pragma unroll
-          for (int q = 0; q < Q; ++q) {
-            const int row = row0 + q * (64 / CPL);
-            const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
-            if (i * 16 + row < mlim && ch * 8 < nlim) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>((bf16_t*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc));
-          }
-        } else {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            if (fg >> 1 == hf) {
-#pragma unroll
-              for (int x = 0; x < NI; ++x)
-                *reinterpret_cast<float4*>(out + fr * (NI * 32) + (((fg & 1) * NI + x) ^ sw) * 16) =
-                    make_float4(v[x >> 1][(x & 1) * 4], v[x >> 1][(x & 1) * 4 + 1], v[x >> 1][(x & 1) * 4 + 2], v[x >> 1][(x & 1) * 4 + 3]);
-            }
-#pragma unroll
-            for (int q = 0; q < Q; ++q) {
-              const int row = row0 + q * (64 / CPL);
-              const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
-              if (i * 16 + row < mlim && hf * (NI * 8) + ch * 4 < nlim)
-                __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>((float*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc + hf * (NI * 8)));
-            }
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      continue;
+      for (int i = 0; i < AHEAD; ++i) fetch(i);
     }
-    // a tile whose columns N cuts within a group of 8: as fp32 through the stage images (a half of the wave's rows at a time where they do not hold it all), then four columns per lane
-    constexpr int HALVES = BM * BN * 4 > 2 * STG ? 2 : 1, HI = MI / HALVES, HR = BM / HALVES, CH = BN / 4;
-    static_assert(HR * BN * 4 <= 2 * STG, "a half fits the stage images");
-    float* const cs = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int hf = 0; hf < HALVES; ++hf) {
-#pragma unroll
-      for (int i = 0; i < HI; ++i) {
-        const float a = s_a[wm + (hf * HI + i) * 16 + fr];
-        const int row = wm / HALVES + i * 16 + fr;
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const i32x4 v = acc[hf * HI + i][j];
-          *reinterpret_cast<float4*>(cs + row * BN + ((((wn + fg * (NI * 4)) >> 2) + j) ^ (row & 7)) * 4) =
-              make_float4((float)v[0] * a, (float)v[1] * a, (float)v[2] * a, (float)v[3] * a);
-        }
-      }
-      __syncthreads();
-#pragma unroll 1
-      for (int x = tid; x < HR * CH; x += G::THREADS) {
-        const int row = x / CH, ch = x % CH, n = n0 + ch * 4;
-        const int m = m0 + row / (HI * 16) * (MI * 16) + hf * (HI * 16) + row % (HI * 16);
-        if (m < p.M && n < p.N) {
-          const float4 f = *reinterpret_cast<const float4*>(cs + row * BN + (ch ^ (row & 7)) * 4);
-          float v[4] = {f.x, f.y, f.z, f.w};
-          Cols<4> c;
-#pragma unroll
-          for (int y = 0; y < 4; ++y) { c.s[y] = s_b[ch * 4 + y]; c.b[y] = s_b[BN + ch * 4 + y]; }
-          finish4(p, v, c, p.residual ? residual_of<4>(p, m, n) : u32x2{}, m, n);
-        }
-      }
-      __syncthreads();
-    }
+    const int mlim = p.M - m0w, nlim = p.N - n0w;
+    stored = m0 + BM <= p.M && n0 + BN <= p.N;
     if (more) {
       place(r + 1);
       issue(0);
       if (nst > 1) issue(1);
     }
-    stored = false;
+    char* const out = smem + 2 * STG + wave * G::OUT;
+    const float *sb = s_b + wn + fg * (NI * 4), *sa = s_a + wm + fr;
+    const int sw = fr & (CPL - 1);
+    const int ch = lane % CPL, row0 = lane / CPL;      // what the lane stores: chunk ch of the rows row0 + q * 64 / CPL
+    const bool stream = (p.ldc * (f32 ? 4 : 2) | (long)(uintptr_t)p.C) % 128 == 0;
+    const int left = nlim - ch * (f32 ? 4 : 8);          // columns from the lane's chunk on
+    const long at = (long)(m0w + row0) * p.ldc + n0w + ch * (f32 ? 4 : 8);
+    Cols<8> c[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) { c[q].s[x] = sb[q * 8 + x]; c[q].b[x] = sb[BN + q * 8 + x]; }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const float a = sa[i * 16];
+      float v[Q][8];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[q][x] = (float)acc[i][q * 2 + (x >> 2)][x & 3] * a;
+        activate<8, EPI == EPI_ANY>(p, v[q], c[q]);
+        if (has_res) add_residual<8>(v[q], odd ? from_element(res[i % AHEAD][q], cut[q]) : res[i % AHEAD][q]);
+      }
+      if (has_res && i + AHEAD < MI) fetch(i + AHEAD);
+      if (!f32) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) *reinterpret_cast<u32x4*>(out + fr * (NI * 32) + ((fg * Q + q) ^ sw) * 16) = pack<8>(v[q]);
+        wave_sync();
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int row = row0 + q * (64 / CPL);
+          const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
+          bf16_t* const to = (bf16_t*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc;
+          if (i * 16 + row < mlim) {
+            if (left >= 8) store16(o, to, stream);
+            else if (odd) {
+#pragma unroll
+              for (int x = 0; x < 7; ++x) if (x < left) to[x] = (bf16_t)(o[x >> 1] >> (x & 1) * 16);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if (fg >> 1 == hf) {
+#pragma unroll
+            for (int x = 0; x < NI; ++x)
+              *reinterpret_cast<u32x4*>(out + fr * (NI * 32) + (((fg & 1) * NI + x) ^ sw) * 16) =
+                  u32x4{__float_as_uint(v[x >> 1][(x & 1) * 4]), __float_as_uint(v[x >> 1][(x & 1) * 4 + 1]), __float_as_uint(v[x >> 1][(x & 1) * 4 + 2]),
+                        __float_as_uint(v[x >> 1][(x & 1) * 4 + 3])};
+          }
+          wave_sync();
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            const int row = row0 + q * (64 / CPL);
+            const u32x4 o = *reinterpret_cast<const u32x4*>(out + row * (NI * 32) + (ch ^ (row & (CPL - 1))) * 16);
+            uint32_t* const to = (uint32_t*)p.C + at + (long)(i * 16 + q * (64 / CPL)) * p.ldc + hf * (NI * 8);
+            if (i * 16 + row < mlim) {
+              if (left - hf * (NI * 8) >= 4) store16(o, to, stream);
+              else if (odd) {
+#pragma unroll
+                for (int x = 0; x < 3; ++x) if (x < left - hf * (NI * 8)) to[x] = o[x];
+              }
+            }
+          }
+          wave_sync();
+        }
+      }
+      wave_sync();
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
@@ -514,12 +525,13 @@ extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   int kind = v2s_opt_gemm_q8();
   const bool plain = !p.c_f32 && p.act != V2S_ACT_GELU;
   if (kind == 0) kind = (int64_t)p.M * p.N <= (p.M <= 64 ? 1 << 18 : 1 << 17) ? 1 : (plain && t4 <= t3 && t4 <= t2 ? 4 : (t3 <= t2 ? 3 : 2));
+  if (p.N < 8) kind = 1;                    // the tiles read a cut group's residual as a row's last eight
   if (kind == 4 && plain) return p.residual ? tile_launch<Tile256, EPI_RESIDUAL>(p, s) : tile_launch<Tile256, EPI_PLAIN>(p, s);
   if (kind >= 3) return tile_any<Tile128>(p, plain, s);
   if (kind == 2) return tile_any<Tile64>(p, plain, s);
   const bool deep = p.K > 1024;
   const int64_t mb = (p.M + 15) / 16, nb = (p.N + 15) / 16;
-  V2S_CHECK(mb <= 65535, V2S_ERR_SHAPE, "v2s_gemm_q8: too many rows for the few-row kernels");
+  V2S_CHECK((mb + 3) / 4 <= 65535, V2S_ERR_SHAPE, "v2s_gemm_q8: too many rows for the few-row kernels");
   // rows of one block: 16 as long as that leaves the chip under two blocks per CU (64 x 1024 x 4096: 6.2 us, 64 rows 11.7), as many as there are otherwise
   // (64 x 4096 x 4096: 17 and 12 us)
   if (mb == 1 || mb * nb < 512) return deep ? skinny_launch<8, 1>(p, s) : skinny_launch<4, 1>(p, s);

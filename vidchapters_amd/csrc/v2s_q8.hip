@@ -319,6 +319,13 @@ __device__ float attn_q8_mean(const i8* vq, const float* vs, int n, float* lds) 
   return n > 0 ? s / (float)n : 0.f;
 }
 
+// What lanes of a wave pass to each other through LDS needs no wait (a wave's LDS operations keep their order), but the compiler, which sees one lane, has to
+// be told that the words may have changed
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 // eight codes as bf16, exactly
 __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
   float f[8];
@@ -418,6 +425,7 @@ __global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
     // all of the chunk's LDS traffic but the values' scales in one go (a wave's LDS operations keep their order, so the values may follow the keys in place)
 #pragma unroll
     for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(vt + tile_at(i * 16 + (lane >> 2), lane & 3)) = kr[i];
+    wave_sync();
     u32x4 kf[4];
     float4 sk[4], sb[4];
 #pragma unroll
@@ -426,14 +434,17 @@ __global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
       const int at = ch * 64 + (i >> 1) * 32 + 8 * g + 4 * (i & 1);
       sk[i] = *reinterpret_cast<const float4*>(s_ks + at); sb[i] = *reinterpret_cast<const float4*>(s_b + at);
     }
+    wave_sync();
 #pragma unroll
     for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(vt + tile_at(i * 16 + (lane >> 2), lane & 3)) = vr[i];
+    wave_sync();
     i32x2 vc[2][4];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
         vc[kb][dt] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((V2S_LDS i32x2*)(vt + tile_at(kb * 32 + 8 * g + (qi >> 1), dt) + (qi & 1) * 8));
+    wave_sync();
     __builtin_amdgcn_sched_barrier(0);
     float sc[16];
 #pragma unroll
