@@ -9,7 +9,7 @@
 // A row of up to 32768 logits is read from memory once and stays in LDS as fp32 (larger ones are read again for every pass, mostly from L2).  The
 // passes over it are bound by VALU issue, not by memory: one instruction per logit costs a block 0.2 us at V = 32228.  Hence: the weights' exponential
 // is a table and five terms of its own, small top-k never touches most logits, and the last pass compares all tokens but weighs only those it keeps.
-// 64 rows of 32228 logits, top-k 50 and top-p 0.95: 11.5 us; 256 rows, top-p 0.92 and min-p: 28 us, a third of it the exact masses.
+// 64 rows of 32228 logits, top-k 50 and top-p 0.95: 11.5 us; 256 rows, top-p 0.92 and min-p: 27.5 us, a third of it the exact masses.
 #include <math.h>
 #include "v2s_common.h"
 

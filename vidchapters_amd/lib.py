@@ -4,6 +4,7 @@ PyTorch is used only for device memory and streams: every wrapper below takes to
 device pointers + sizes + the current HIP stream to the library, and raises ``RuntimeError`` with
 ``v2s_last_error()`` on a non-zero return.  There is NO fallback: if the shared library is missing the
 import of :func:`lib` fails loudly (product path never routes through the CPU oracle).
+The 8-bit decoding calls take their tensors apart in native code (csrc/v2s_bind.cpp, :func:`_bind`) and call the same library.
 """
 from __future__ import annotations
 
