@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
   }
 }
 
-// y[row][c] = scale[row] * q[row][c], 8 columns per lane
+// y[row][c] = scale[row] * q[row][c], 8 columns per lane: bytes in, bytes out (32000 x 768: 12.4 us, 6 TB/s out of a cache that still holds the codes)
 __global__ __launch_bounds__(256) void dequant_q8_kernel(const i8* __restrict__ q, long ldq, const float* __restrict__ scale, bf16_t* __restrict__ y,
                                                          long ldy, int rows, int nch) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -202,6 +202,7 @@ struct KvQ8 {
   int pos0;
 };
 
+// Bound by HBM: 32 entries x 12 heads x up to 1100 tokens 23.5 us in and 21.6 us back, 4.7 and 5.1 TB/s; a single token by its chain of loads (2.9 us).
 // eight lanes per (entry, head, token); TOKENS: eight tokens of one head per wave (512 contiguous bytes of codes), else eight heads of one token
 template <bool TOKENS>
 __device__ __forceinline__ bool kv_unit(const KvQ8& p, int& e, int& h, int& t) {
