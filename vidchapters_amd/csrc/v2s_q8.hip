@@ -202,7 +202,7 @@ struct KvQ8 {
   int pos0;
 };
 
-// Bound by HBM: 32 entries x 12 heads x up to 1100 tokens 23.5 us in and 21.6 us back, 4.7 and 5.1 TB/s; a single token by its chain of loads (2.9 us).
+// Bound by HBM: 32 entries x 12 heads x up to 1100 tokens 23.5 us in and 21.6 us back, 5.3 and 5.7 TB/s; a single token by its chain of loads (2.9 us).
 // eight lanes per (entry, head, token); TOKENS: eight tokens of one head per wave (512 contiguous bytes of codes), else eight heads of one token
 template <bool TOKENS>
 __device__ __forceinline__ bool kv_unit(const KvQ8& p, int& e, int& h, int& t) {
