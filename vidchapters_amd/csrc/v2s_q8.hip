@@ -346,8 +346,8 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
 //            fp32.  Tile t of a group of 32 keys holds the keys 8 (row >> 2) + 4 t + (row & 3), so that the eight scores a lane gets of its query are
 //            those of the consecutive keys 8 g .. 8 g + 7 (g = lane >> 4), which is the B operand of the second product without any movement.
 //   output   O^T[d][query] += V^T[d][key] . P^T[key][query]: the value codes follow the keys in the wave's LDS tile, the transposing read
-//            (ds_read_b64_tr_b8) returns the codes of eight keys for one d.  The weights carry the values' scales and are split into bf16 high and low
-//            parts (16 bits, two products).
+//            (ds_read_b64_tr_b8) returns the codes of eight keys for one d.  The weights carry the values' scales and are split into three bf16 parts
+//            of eight bits each, which is all of fp32 (three products): every product is exact and the sums are fp32, as for a single query.
 // The running maximum of a query is shared by its four lanes; scales and bias of the piece wait in LDS, where a key without a part has bias -infinity
 // and scales of zero.  4 x 4 queries x 16 heads x 40000 keys: 66 us, 5.3 TB/s, the rate of a large copy.  A value-per-lane form without the matrix pipe was
 // bound by VALU issue (127 us); eight waves per block or five blocks per CU were slower on large caches, requesting the next chunk ahead did not pay.
@@ -482,18 +482,23 @@ __global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
         l += x;
         w[i] = x * sv[i];
       }
-      uint4 hi, lo;
-      hi = round8(w);
-      float hf[8];
-      unpack8(hi, hf);
+      bf16x8 part[3];                   // hi, mid, lo: 24 bits
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] -= hf[i];
-      lo = round8(w);
+      for (int x = 0; x < 3; ++x) {
+        const uint4 r = round8(w);
+        part[x] = __builtin_bit_cast(bf16x8, r);
+        if (x < 2) {
+          float f[8];
+          unpack8(r, f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] -= f[i];
+        }
+      }
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
         const bf16x8 vf = codes_bf16((uint32_t)vc[kb][dt][0], (uint32_t)vc[kb][dt][1]);
-        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, hi), acc[dt], 0, 0, 0);
-        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, lo), acc[dt], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < 3; ++x) acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, part[x], acc[dt], 0, 0, 0);
       }
     }
   }
