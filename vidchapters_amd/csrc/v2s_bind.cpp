@@ -35,10 +35,10 @@ int32_t small(PyObject* o, const char* name) {
   if (v != (int32_t)v) raise(PyExc_ValueError, std::string(name) + " does not fit 32 bits");
   return (int32_t)v;
 }
-int64_t or_default(PyObject* o, int64_t d) {          // None and 0 stand for the default
+int64_t given_stride(PyObject* o) {                   // 0: not given
   const int64_t v = o == Py_None ? 0 : integer(o);
   if (v > INT32_MAX) raise(PyExc_ValueError, "a row stride does not fit 32 bits");
-  return v ? v : d;
+  return v;
 }
 double number(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
@@ -46,10 +46,30 @@ double number(PyObject* o) {
   return v;
 }
 
+// Elements of a tensor that lie one behind the other from its first one on, and the dimension next to them as rows (none: one row)
+struct Layout { int64_t run = 1, rows = 1, stride = -1; };
+Layout layout_of(const at::Tensor& t) {
+  Layout l;
+  int64_t d = t.dim() - 1;
+  for (; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (t.stride(d) != l.run) break;
+    l.run *= t.size(d);
+  }
+  for (; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (l.stride < 0) { l.rows = t.size(d); l.stride = t.stride(d); }
+    else if (t.stride(d) == l.rows * l.stride) l.rows *= t.size(d);
+    else break;
+  }
+  return l;
+}
+
 // The operands of one call: all on the current device, on whose current stream the launch goes out.
 struct Call {
   const char* name;
   int64_t device = -2;                                // not looked up yet
+  const char* elsewhere = nullptr;                    // an operand that is not on the GPU: said when every operand has been looked at
 
   const at::Tensor& tensor(PyObject* o, const char* arg) const {
     if (!THPVariable_Check(o)) raise(PyExc_TypeError, label(arg) + ": a tensor is expected");
@@ -58,9 +78,16 @@ struct Call {
   std::string label(const char* arg) const { return std::string(name) + " " + arg; }
   // address of an operand of this type with `need` elements of storage from its first one on
   void* at_least(const at::Tensor& t, at::ScalarType type, int64_t need, const char* arg) {
-    if (!t.is_cuda()) raise(PyExc_RuntimeError, label(arg) + ": tensor must live on the GPU (HIP path has no CPU fallback)");
+    if (t.dim() > 0 && t.size(-1) > 1 && t.stride(-1) != 1) raise(PyExc_ValueError, label(arg) + ": the last dimension must be contiguous");
     if (t.scalar_type() != type)
       raise(PyExc_RuntimeError, label(arg) + ": expected dtype " + c10::toString(type) + ", got " + c10::toString(t.scalar_type()));
+    const int64_t have = (int64_t)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
+    if (have < need)
+      raise(PyExc_ValueError, label(arg) + ": " + std::to_string(need) + " elements are read or written, the tensor's storage holds " + std::to_string(have));
+    if (!t.is_cuda()) {
+      if (!elsewhere) elsewhere = arg;
+      return nullptr;
+    }
     if (device < 0) {
       PyObject* d = PyObject_CallNoArgs(current_device);
       if (!d) throw Raised();
@@ -69,15 +96,39 @@ struct Call {
     }
     if (t.get_device() != device)
       raise(PyExc_RuntimeError, label(arg) + ": tensor lives on cuda:" + std::to_string(t.get_device()) + ", the launch goes to cuda:" + std::to_string(device));
-    if (t.dim() > 0 && t.size(-1) > 1 && t.stride(-1) != 1) raise(PyExc_ValueError, label(arg) + ": the last dimension must be contiguous");
-    const int64_t have = (int64_t)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
-    if (have < need)
-      raise(PyExc_ValueError, label(arg) + ": " + std::to_string(need) + " elements are read or written, the tensor's storage holds " + std::to_string(have));
     return t.data_ptr();
   }
   void* operand(PyObject* o, at::ScalarType type, int64_t need, const char* arg) { return at_least(tensor(o, arg), type, need, arg); }
-  void* optional(PyObject* o, at::ScalarType type, int64_t need, const char* arg) { return o == Py_None ? nullptr : operand(o, type, need, arg); }
+  // `need` numbers that lie one behind the other
+  void* vector(const at::Tensor& t, at::ScalarType type, int64_t need, const char* arg) {
+    if (!t.is_contiguous() && layout_of(t).run < need)
+      raise(PyExc_ValueError, label(arg) + ": " + std::to_string(need) + " elements are expected one behind the other (contiguous) in its storage");
+    return at_least(t, type, need, arg);
+  }
+  void* vector(PyObject* o, at::ScalarType type, int64_t need, const char* arg) { return vector(tensor(o, arg), type, need, arg); }
+  void* optional(PyObject* o, at::ScalarType type, int64_t need, const char* arg) { return o == Py_None ? nullptr : vector(o, type, need, arg); }
+  // Rows of `cols` elements, ld apart.  A stride of 0 stands for the tensor's own: the rows of a tensor that has so many, each of `cols` elements or more; else
+  // rows laid end to end, if so many elements lie one behind the other.
+  void* matrix(const at::Tensor& t, at::ScalarType type, int64_t rows, int64_t cols, int64_t& ld, const char* arg) {
+    if (ld == 0) {
+      ld = cols;
+      const bool whole = t.is_contiguous(), wide = t.dim() > 1 && cols > 0 && t.size(-1) > cols;
+      if (!whole || wide) {
+        const Layout l = whole ? Layout{t.size(-1), t.numel() / t.size(-1), t.size(-1)} : layout_of(t);
+        if (rows > 1 && l.run >= cols && l.rows >= rows) ld = l.stride;
+        else if (!whole && l.run < rows * cols)
+          raise(PyExc_ValueError, label(arg) + ": " + std::to_string(rows) + " rows of " + std::to_string(cols) + " elements at one distance are expected; give their stride");
+      }
+      if (ld > INT32_MAX) raise(PyExc_ValueError, "a row stride does not fit 32 bits");
+    }
+    return at_least(t, type, (rows - 1) * ld + cols, arg);
+  }
+  void* matrix(PyObject* o, at::ScalarType type, int64_t rows, int64_t cols, int64_t& ld, const char* arg) { return matrix(tensor(o, arg), type, rows, cols, ld, arg); }
+  void* optional_matrix(PyObject* o, at::ScalarType type, int64_t rows, int64_t cols, int64_t& ld, const char* arg) {
+    return o == Py_None ? nullptr : matrix(o, type, rows, cols, ld, arg);
+  }
   void* stream() const {
+    if (elsewhere) raise(PyExc_RuntimeError, label(elsewhere) + ": tensor must live on the GPU (HIP path has no CPU fallback)");
     PyObject* d = PyLong_FromLongLong(device);
     PyObject* s = d ? PyObject_CallOneArg(raw_stream, d) : nullptr;
     Py_XDECREF(d);
@@ -123,9 +174,9 @@ PyObject* quant_rows_q8(PyObject* const* a) {
   const at::Tensor& x = c.tensor(a[0], "x");
   const bool f32 = x.scalar_type() == at::kFloat;
   const int32_t rows = small(a[3], "rows"), cols = small(a[4], "cols");
-  const int64_t ldx = or_default(a[5], cols), ldq = or_default(a[6], cols), last = rows - 1;
-  void* px = c.at_least(x, f32 ? at::kFloat : at::kBFloat16, last * ldx + cols, "x");
-  void *pq = c.operand(a[1], at::kChar, last * ldq + cols, "q"), *ps = c.operand(a[2], at::kFloat, rows, "scale");
+  int64_t ldx = given_stride(a[5]), ldq = given_stride(a[6]);
+  void* px = c.matrix(x, f32 ? at::kFloat : at::kBFloat16, rows, cols, ldx, "x");
+  void *pq = c.matrix(a[1], at::kChar, rows, cols, ldq, "q"), *ps = c.vector(a[2], at::kFloat, rows, "scale");
   return launch(f_quant, px, f32 ? V2S_F32 : V2S_BF16, ldx, (int8_t*)pq, ldq, (float*)ps, rows, cols, c.stream());
 }
 
@@ -133,10 +184,10 @@ PyObject* quant_rows_q8(PyObject* const* a) {
 PyObject* rmsnorm_q8(PyObject* const* a) {
   Call c{"rmsnorm_q8"};
   const int32_t rows = small(a[4], "rows"), cols = small(a[5], "cols");
-  const int64_t ldx = or_default(a[9], cols), ldd = or_default(a[10], cols), ldh = or_default(a[11], cols), ldq = or_default(a[12], cols), last = rows - 1;
-  void *x = c.operand(a[0], at::kBFloat16, last * ldx + cols, "x"), *w = c.operand(a[1], at::kFloat, cols, "w");
-  void *d = c.optional(a[7], at::kBFloat16, last * ldd + cols, "delta"), *h = c.optional(a[8], at::kBFloat16, last * ldh + cols, "h");
-  void *q = c.operand(a[2], at::kChar, last * ldq + cols, "q"), *s = c.operand(a[3], at::kFloat, rows, "scale");
+  int64_t ldx = given_stride(a[9]), ldd = given_stride(a[10]), ldh = given_stride(a[11]), ldq = given_stride(a[12]);
+  void *x = c.matrix(a[0], at::kBFloat16, rows, cols, ldx, "x"), *w = c.vector(a[1], at::kFloat, cols, "w");
+  void *d = c.optional_matrix(a[7], at::kBFloat16, rows, cols, ldd, "delta"), *h = c.optional_matrix(a[8], at::kBFloat16, rows, cols, ldh, "h");
+  void *q = c.matrix(a[2], at::kChar, rows, cols, ldq, "q"), *s = c.vector(a[3], at::kFloat, rows, "scale");
   return launch(f_norm, x, ldx, d, ldd, (float*)w, h, ldh, (int8_t*)q, ldq, (float*)s, rows, cols, (float)number(a[6]), c.stream());
 }
 
@@ -144,9 +195,9 @@ PyObject* rmsnorm_q8(PyObject* const* a) {
 PyObject* dequant_q8(PyObject* const* a) {
   Call c{"dequant_q8"};
   const int32_t rows = small(a[3], "rows"), cols = small(a[4], "cols");
-  const int64_t ldq = or_default(a[5], cols), ldy = or_default(a[6], cols), last = rows - 1;
-  void *q = c.operand(a[0], at::kChar, last * ldq + cols, "q"), *s = c.operand(a[1], at::kFloat, rows, "scale");
-  void* y = c.operand(a[2], at::kBFloat16, last * ldy + cols, "y");
+  int64_t ldq = given_stride(a[5]), ldy = given_stride(a[6]);
+  void *q = c.matrix(a[0], at::kChar, rows, cols, ldq, "q"), *s = c.vector(a[1], at::kFloat, rows, "scale");
+  void* y = c.matrix(a[2], at::kBFloat16, rows, cols, ldy, "y");
   return launch(f_dequant, (int8_t*)q, ldq, (float*)s, y, ldy, rows, cols, c.stream());
 }
 
@@ -157,14 +208,13 @@ PyObject* gemm_q8(PyObject* const* a) {
   const at::Tensor& out = c.tensor(a[4], "C");
   const bool f32 = out.scalar_type() == at::kFloat;
   g.M = small(a[5], "M"); g.N = small(a[6], "N"); g.K = small(a[7], "K");
-  g.lda = or_default(a[8], g.K); g.ldb = or_default(a[9], g.K); g.ldc = or_default(a[10], g.N); g.ldr = or_default(a[15], g.N);
-  const int64_t last = (int64_t)g.M - 1;
-  g.A = (int8_t*)c.operand(a[0], at::kChar, last * g.lda + g.K, "A"); g.B = (int8_t*)c.operand(a[1], at::kChar, ((int64_t)g.N - 1) * g.ldb + g.K, "B");
-  g.sA = (float*)c.operand(a[2], at::kFloat, g.M, "sA"); g.sB = (float*)c.operand(a[3], at::kFloat, g.N, "sB");
-  g.C = c.at_least(out, f32 ? at::kFloat : at::kBFloat16, last * g.ldc + g.N, "C");
+  g.lda = given_stride(a[8]); g.ldb = given_stride(a[9]); g.ldc = given_stride(a[10]); g.ldr = given_stride(a[15]);
+  g.A = (int8_t*)c.matrix(a[0], at::kChar, g.M, g.K, g.lda, "A"); g.B = (int8_t*)c.matrix(a[1], at::kChar, g.N, g.K, g.ldb, "B");
+  g.sA = (float*)c.vector(a[2], at::kFloat, g.M, "sA"); g.sB = (float*)c.vector(a[3], at::kFloat, g.N, "sB");
+  g.C = c.matrix(out, f32 ? at::kFloat : at::kBFloat16, g.M, g.N, g.ldc, "C");
   g.c_dtype = f32 ? V2S_F32 : V2S_BF16; g.alpha = (float)number(a[11]); g.act = small(a[13], "act");
   g.bias = (float*)c.optional(a[12], at::kFloat, g.N, "bias");
-  g.residual = c.optional(a[14], at::kBFloat16, last * g.ldr + g.N, "residual");
+  g.residual = c.optional_matrix(a[14], at::kBFloat16, g.M, g.N, g.ldr, "residual");
   return launch(f_gemm, &g, c.stream());
 }
 
@@ -202,7 +252,7 @@ PyObject* decode_attn_q8(PyObject* const* a) {
   c.locate(d.cache, a + 1);
   d.q = c.at_least(q, at::kBFloat16, 0, "q"); d.q_bs = q.stride(0);
   d.o = c.at_least(o, at::kBFloat16, 0, "o"); d.o_bs = o.stride(0);
-  if (a[9] != Py_None) { d.pos_dev = (int32_t*)c.operand(a[9], at::kInt, 1, "pos_dev"); d.bias_maxlen = small(a[10], "bias_maxlen"); }
+  if (a[9] != Py_None) { d.pos_dev = (int32_t*)c.vector(a[9], at::kInt, 1, "pos_dev"); d.bias_maxlen = small(a[10], "bias_maxlen"); }
   if (a[11] != Py_None) {
     const at::Tensor& b = c.tensor(a[11], "bias_row");
     if (b.dim() != 2 || b.size(0) != H) raise(PyExc_ValueError, "decode_attn_q8: bias_row is [heads, keys]");
@@ -218,7 +268,7 @@ PyObject* decode_attn_q8(PyObject* const* a) {
   d.klen = (int32_t*)c.optional(a[8], at::kInt, E, "klen");
   if (a[14] != Py_None) {
     const at::Tensor& w = c.tensor(a[14], "workspace");
-    d.workspace = c.at_least(w, at::kFloat, w.numel(), "workspace"); d.workspace_bytes = w.numel() * 4;
+    d.workspace = c.vector(w, at::kFloat, w.numel(), "workspace"); d.workspace_bytes = w.numel() * 4;
   }
   return launch(f_attn, &d, c.stream());
 }
@@ -229,13 +279,14 @@ PyObject* sample_step(PyObject* const* a) {
   const at::Tensor &z = c.tensor(a[0], "logits"), &u = c.tensor(a[3], "u");
   const bool f32 = z.scalar_type() == at::kFloat, table = a[16] != Py_None;
   const int32_t rows = small(a[1], "rows"), V = small(a[2], "V");
-  const int64_t ld = or_default(a[5], z.dim() == 2 && rows > 1 ? z.stride(0) : V), seq_ld = or_default(a[15], 0);
+  int64_t ld = given_stride(a[5]);
+  const int64_t seq_ld = given_stride(a[15]);
   if (u.dim() != (table ? 2 : 1) || u.size(-1) < rows)
     raise(PyExc_ValueError, "sample_step: u is [rows], or [steps, rows] with pos_dev, for " + std::to_string(rows) + " rows");
   const int64_t steps = table ? u.size(0) : 0, u_ld = !table ? 0 : (steps > 1 ? u.stride(0) : u.size(1));
   if (steps > INT32_MAX) raise(PyExc_ValueError, "sample_step: too many steps");
-  void *pz = c.at_least(z, f32 ? at::kFloat : at::kBFloat16, ((int64_t)rows - 1) * ld + V, "logits"), *pu = c.at_least(u, at::kFloat, rows, "u");
-  void *tok = c.operand(a[4], at::kLong, rows, "next_tok"), *lp = c.optional(a[10], at::kFloat, rows, "logp");
+  void *pz = c.matrix(z, f32 ? at::kFloat : at::kBFloat16, rows, V, ld, "logits"), *pu = c.at_least(u, at::kFloat, rows, "u");
+  void *tok = c.vector(a[4], at::kLong, rows, "next_tok"), *lp = c.optional(a[10], at::kFloat, rows, "logp");
   void *un = c.optional(a[11], at::kInt, rows, "unfinished"), *seq = c.optional(a[14], at::kLong, rows * seq_ld, "seq_out");
   void* ctr = c.optional(a[16], at::kInt, 1, "pos_dev");
   return launch(f_sample, pz, f32 ? V2S_F32 : V2S_BF16, ld, rows, V, number(a[6]), small(a[7], "top_k"), number(a[8]), number(a[9]), (float*)pu, u_ld, (int32_t)steps,

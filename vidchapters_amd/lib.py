@@ -767,7 +767,8 @@ def beam_sample_cand(logits, ld, rows, V, K, beam_scores, top_p, temperature, to
 # --------------------------------------------------------------------------------------------- 8-bit decoding
 # A decode step is a chain of launches of a few microseconds, so these calls look at their operands in native code (csrc/v2s_bind.cpp).  Every operand
 # lives on the current device, and the launch goes to its current stream; wrong types and devices raise RuntimeError, shapes, strides and tensors whose
-# storage is too small ValueError.
+# storage is too small ValueError.  A matrix whose row stride (ld...) is not given has its own: the rows of a tensor that holds so many of them, each of so many
+# elements or more, a view's among them; any other contiguous tensor is taken as rows laid end to end.
 _BIND = None
 
 
