@@ -2,7 +2,7 @@
 // A decode step is a chain of launches of a few microseconds, and a launch alone costs the host 3 us.  Reading shapes, strides, types and addresses of six
 // to eight tensors from Python added as much again: a call through ctypes took 4.7 (dequant_q8), 6.1 (gemm_q8), 8.0 (kv_append_q8) us of host time, from
 // here 3.4, 3.4 and 4.0.
-// The library is not linked: lib.py hands over the addresses of the functions it has loaded and checked.
+// The library is not linked: lib.py hands over the addresses of its functions, and attach() checks that both were built from one header.
 #include <torch/csrc/autograd/python_variable.h>
 #include <exception>
 #include <stdexcept>
@@ -309,18 +309,34 @@ template <PyObject* (*F)(PyObject* const*), int N> PyObject* entry(PyObject*, Py
   return nullptr;
 }
 
-// current_device raw_stream, then the addresses of the library's functions in the order of the pointers above
+// current_device raw_stream v2s_version v2s_sizeof, then the addresses of the library's functions in the order of the pointers above.  The structs filled here
+// are laid out by the header that this file was compiled with: a library of another version, or with other sizes, is refused and nothing is attached.
 PyObject* attach(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 10) { PyErr_SetString(PyExc_TypeError, "attach: ten arguments"); return nullptr; }
-  void* f[8];
-  for (int i = 0; i < 8; ++i) {
+  if (n != 12) { PyErr_SetString(PyExc_TypeError, "attach: twelve arguments"); return nullptr; }
+  void* f[10];
+  for (int i = 0; i < 10; ++i) {
     f[i] = PyLong_AsVoidPtr(a[2 + i]);
     if (!f[i]) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "attach: a function's address is NULL"); return nullptr; }
   }
+  const int version = ((decltype(&v2s_version))f[0])();
+  if (version != V2S_ABI_VERSION) {
+    PyErr_Format(PyExc_RuntimeError, "ABI mismatch: the library reports V2S_ABI_VERSION %d, _bind.so was built for %d (vidchapters_amd/csrc/build.sh builds both)", version,
+                 V2S_ABI_VERSION);
+    return nullptr;
+  }
+  const struct { const char* name; size_t size; } structs[] = {
+      {"v2s_gemm_q8_args", sizeof(v2s_gemm_q8_args)}, {"v2s_kv_q8", sizeof(v2s_kv_q8)}, {"v2s_decode_attn_q8_args", sizeof(v2s_decode_attn_q8_args)}};
+  for (const auto& t : structs) {
+    const long long size = ((decltype(&v2s_sizeof))f[1])(t.name);
+    if (size != (long long)t.size) {
+      PyErr_Format(PyExc_RuntimeError, "ABI mismatch: %s has %lld bytes in the library and %zu in _bind.so (vidchapters_amd/csrc/build.sh builds both)", t.name, size, t.size);
+      return nullptr;
+    }
+  }
   Py_INCREF(a[0]); Py_INCREF(a[1]);
   current_device = a[0]; raw_stream = a[1];
-  f_quant = (decltype(f_quant))f[0]; f_norm = (decltype(f_norm))f[1]; f_dequant = (decltype(f_dequant))f[2]; f_gemm = (decltype(f_gemm))f[3];
-  f_append = (decltype(f_append))f[4]; f_read = (decltype(f_read))f[5]; f_attn = (decltype(f_attn))f[6]; f_sample = (decltype(f_sample))f[7];
+  f_quant = (decltype(f_quant))f[2]; f_norm = (decltype(f_norm))f[3]; f_dequant = (decltype(f_dequant))f[4]; f_gemm = (decltype(f_gemm))f[5];
+  f_append = (decltype(f_append))f[6]; f_read = (decltype(f_read))f[7]; f_attn = (decltype(f_attn))f[8]; f_sample = (decltype(f_sample))f[9];
   Py_RETURN_NONE;
 }
 

@@ -784,7 +784,7 @@ def _bind():
         address = lambda name: C.cast(getattr(lib(), "v2s_" + name), _vp).value  # noqa: E731
         m.attach(getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
                  getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream),
-                 *(address(n) for n in ("quant_rows_q8", "rmsnorm_q8", "dequant_q8", "gemm_q8", "kv_append_q8", "kv_read_q8", "decode_attn_q8", "sample_step")))
+                 *(address(n) for n in ("version", "sizeof", "quant_rows_q8", "rmsnorm_q8", "dequant_q8", "gemm_q8", "kv_append_q8", "kv_read_q8", "decode_attn_q8", "sample_step")))
         _BIND = m
     return _BIND
 
