@@ -208,13 +208,6 @@ class Block:
         if op == "v_mul_u32_u24":
             r = (u64(V(ops[1])) & np.uint64(0xFFFFFF)) * (u64(V(ops[2])) & np.uint64(0xFFFFFF))
             self.setv(w, ops[0], (r & np.uint64(0xFFFFFFFF)).astype(np.uint32)); return
-        if op == "v_pk_mul_f32":
-            (kd, d0, dn), (ka, a0, an), (kb, b0, bn) = self.rng(ops[0]), self.rng(ops[1]), self.rng(ops[2])
-            assert dn == an == bn == 2 and kd == ka == kb == "v", ins
-            with np.errstate(all="ignore"):
-                lo = (w.v[a0].view(np.float32) * w.v[b0].view(np.float32)).astype(np.float32).view(np.uint32)
-                hi = (w.v[a0 + 1].view(np.float32) * w.v[b0 + 1].view(np.float32)).astype(np.float32).view(np.uint32)
-            w.v[d0], w.v[d0 + 1] = lo.copy(), hi.copy(); return
         if op == "v_lshl_add_u32":
             r = (u64(V(ops[1])) << (u64(V(ops[2])) & np.uint64(31))) + u64(V(ops[3]))
             self.setv(w, ops[0], (r & np.uint64(0xFFFFFFFF)).astype(np.uint32)); return

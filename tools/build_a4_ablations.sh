@@ -5,7 +5,7 @@ set -e
 cd "$(dirname "$0")/../vidchapters_amd/csrc"
 bash build.sh > /dev/null
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -munsafe-fp-atomics"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops"
 OBJS=""; for s in v2s_api v2s_norm v2s_attn v2s_misc v2s_optim v2s_decode v2s_memattn v2s_data; do OBJS="$OBJS build/$s.o"; done
 # one library per slot plan of the generator (A4_PLAN): the committed one ("spread") and the experimental ones
 for plan in ${A4_PLANS:-spread early}; do

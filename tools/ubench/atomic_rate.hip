@@ -1,5 +1,5 @@
 // Throughput of coalesced fp32 global atomic adds (fire-and-forget) by memory scope, gfx950.
-// build: hipcc --offload-arch=gfx950 -O3 -munsafe-fp-atomics atomic_rate.hip -o atomic_rate
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -munsafe-fp-atomics atomic_rate.hip -o atomic_rate
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 template <int SCOPE>

@@ -1,7 +1,7 @@
 // How fast do the workgroups of ONE short kernel get onto the chip?  Every block records the 100 MHz reference clock at entry, then holds its CU for
 // `hold` us (a decode-step skinny GEMM block lives ~3 us).  Printed per (grid, block size): when the n-th block (by entry order) started, relative
 // to the first one -- i.e. whether a grid larger than the CU count is dispatched at once or the blocks past one-per-CU wait.
-// build: hipcc --offload-arch=gfx950 -O3 dispatch_rate.hip -o dispatch_rate
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops dispatch_rate.hip -o dispatch_rate
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <stdio.h>

@@ -3,7 +3,7 @@
 // cache holds, reduces them with a value another block wrote in the previous phase, writes one value, barrier -- with the next phase's
 // weights requested after or BEFORE the barrier; (3) the same chain as separate launches: eager, and as a replayed hipGraph (device time per
 // node, host time per hipGraphLaunch).  Every spin is bounded (err flag) so that a lost block cannot hang the GPU.
-// build: hipcc --offload-arch=gfx950 -O3 grid_barrier.hip -o grid_barrier
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops grid_barrier.hip -o grid_barrier
 #include <hip/hip_runtime.h>
 #include <chrono>
 #include <stdio.h>

@@ -3,7 +3,7 @@
 // (a) in one 128-byte struct passed by value (what the library's GEMM / attention / decode kernels do: the compiler passes it by reference and
 // s_loads the fields), (b) as leading scalar parameters.  Build the file twice -- plain, and with -mllvm -amdgpu-kernarg-preload-count=16 (the
 // first 16 dwords of (b) then arrive in SGPRs with the wave, (a) is not preloadable) -- and compare the device time per node.
-// build: hipcc --offload-arch=gfx950 -O3 kernarg_chain.hip -o kernarg_chain ; hipcc ... -mllvm -amdgpu-kernarg-preload-count=16 -o kernarg_chain_preload
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops kernarg_chain.hip -o kernarg_chain ; hipcc ... -mllvm -amdgpu-kernarg-preload-count=16 -o kernarg_chain_preload
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #define CK(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) { printf("HIP error %s at line %d\n", hipGetErrorString(e_), __LINE__); return 1; } } while (0)

@@ -2,7 +2,7 @@
 //   32x32x16 (16 blocks of 16 accumulators, 8 passes)  vs  16x16x32 (64 blocks of 4 accumulators, 4 passes).
 // The 32x32 form moves 25 % more register bytes per flop (accumulators in + out dominate); which one the chip sustains longer at its power
 // limit decides the MFMA shape of a GEMM whose main loop is power-bound (gemm_a4's ablations).  ~30 ms per variant.
-// build: hipcc --offload-arch=gfx950 -O3 mfma_power.hip -o mfma_power
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_power.hip -o mfma_power
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 typedef __attribute__((ext_vector_type(4))) float f32x4;

@@ -1,6 +1,6 @@
 // How fast can ONE wave per SIMD (and two) issue independent bf16 MFMAs on gfx950?  16x16x32 (4 passes) vs 32x32x16 (8 passes), accumulators
 // in VGPRs or AGPRs, with and without an LDS read between groups of MFMAs (the shape of a GEMM main loop).  Cycles by clock64() of wave 0.
-// build: hipcc --offload-arch=gfx950 -O3 mfma_rate.hip -o mfma_rate
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_rate.hip -o mfma_rate
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 typedef __attribute__((ext_vector_type(4))) float f32x4;

@@ -1,37 +1,32 @@
 // Issue rates of the VALU instructions that make up the attention softmax / dropout code on gfx950, and whether MFMA and VALU
 // work of DIFFERENT waves on one SIMD overlaps.  One block of 256 (or 512) threads per CU = 1 (or 2) waves per SIMD; every lane
 // runs 8 independent dependency chains, 64 instructions per loop trip, cycles read with s_memtime by wave 0.
-// build: hipcc --offload-arch=gfx950 -O3 valu_rate.hip -o valu_rate
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops valu_rate.hip -o valu_rate
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>
 
-typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 
 #define REP8(X) X(0) X(1) X(2) X(3) X(4) X(5) X(6) X(7)
 #define BODY64(X) REP8(X) REP8(X) REP8(X) REP8(X) REP8(X) REP8(X) REP8(X) REP8(X)
 
-enum { OP_ADD, OP_PK_ADD, OP_FMA, OP_PK_FMA, OP_PK_MUL, OP_EXP, OP_CVT_PK, OP_MUL24, OP_MUL_LO, OP_XOR, OP_CNDMASK, OP_CMP_CND, OP_PERM,
+enum { OP_ADD, OP_FMA, OP_EXP, OP_CVT_PK, OP_MUL24, OP_MUL_LO, OP_XOR, OP_CNDMASK, OP_CMP_CND, OP_PERM,
        OP_MAX3, OP_ADD_F64, OP_CVT_F64, OP_NOPS };
-static const char* NAMES[] = {"v_add_f32", "v_pk_add_f32", "v_fma_f32", "v_pk_fma_f32", "v_pk_mul_f32", "v_exp_f32", "v_cvt_pk_bf16_f32",
+static const char* NAMES[] = {"v_add_f32", "v_fma_f32", "v_exp_f32", "v_cvt_pk_bf16_f32",
                               "v_mul_u32_u24", "v_mul_lo_u32", "v_xor_b32", "v_cndmask_b32", "v_cmp+v_cndmask", "v_perm_b32", "v_max3_f32",
                               "v_add_f64", "v_cvt_f64_f32"};
 
 template <int OP>
 __global__ __launch_bounds__(512) void rate_kernel(long long* out, float seed, int trips) {
-  float a[8]; f32x2 p[8]; double d[8]; uint32_t u[8];
+  float a[8]; double d[8]; uint32_t u[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { a[i] = seed + i + threadIdx.x; p[i] = f32x2{a[i], a[i] + 1.f}; d[i] = a[i]; u[i] = (uint32_t)a[i]; }
-  const f32x2 c2 = {seed, seed * 0.5f};
+  for (int i = 0; i < 8; ++i) { a[i] = seed + i + threadIdx.x; d[i] = a[i]; u[i] = (uint32_t)a[i]; }
   const long long t0 = clock64();
   for (int t = 0; t < trips; ++t) {
 #define X_ADD(i) asm volatile("v_add_f32 %0, %0, %1" : "+v"(a[i]) : "v"(seed));
-#define X_PK_ADD(i) asm volatile("v_pk_add_f32 %0, %0, %1" : "+v"(p[i]) : "v"(c2));
 #define X_FMA(i) asm volatile("v_fma_f32 %0, %0, %1, %1" : "+v"(a[i]) : "v"(seed));
-#define X_PK_FMA(i) asm volatile("v_pk_fma_f32 %0, %0, %1, %1" : "+v"(p[i]) : "v"(c2));
-#define X_PK_MUL(i) asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(p[i]) : "v"(c2));
 #define X_EXP(i) asm volatile("v_exp_f32 %0, %0" : "+v"(a[i]));
 #define X_CVT_PK(i) asm volatile("v_cvt_pk_bf16_f32 %0, %0, %1" : "+v"(a[i]) : "v"(seed));
 #define X_MUL24(i) asm volatile("v_mul_u32_u24 %0, %0, %1" : "+v"(u[i]) : "v"(u[(i + 1) & 7]));
@@ -44,10 +39,7 @@ __global__ __launch_bounds__(512) void rate_kernel(long long* out, float seed, i
 #define X_ADD_F64(i) asm volatile("v_add_f64 %0, %0, %1" : "+v"(d[i]) : "v"(d[(i + 1) & 7]));
 #define X_CVT_F64(i) asm volatile("v_cvt_f64_f32 %0, %1" : "=v"(d[i]) : "v"(a[i]));
     if (OP == OP_ADD) { BODY64(X_ADD) }
-    if (OP == OP_PK_ADD) { BODY64(X_PK_ADD) }
     if (OP == OP_FMA) { BODY64(X_FMA) }
-    if (OP == OP_PK_FMA) { BODY64(X_PK_FMA) }
-    if (OP == OP_PK_MUL) { BODY64(X_PK_MUL) }
     if (OP == OP_EXP) { BODY64(X_EXP) }
     if (OP == OP_CVT_PK) { BODY64(X_CVT_PK) }
     if (OP == OP_MUL24) { BODY64(X_MUL24) }
@@ -63,7 +55,7 @@ __global__ __launch_bounds__(512) void rate_kernel(long long* out, float seed, i
   const long long t1 = clock64();
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s += a[i] + p[i][0] + p[i][1] + (float)d[i] + (float)u[i];
+  for (int i = 0; i < 8; ++i) s += a[i] + (float)d[i] + (float)u[i];
   if (s == 12345.678f) out[1] = 1;                // keep the chains alive
   if (blockIdx.x == 0 && threadIdx.x == 0) out[0] = t1 - t0;
 }

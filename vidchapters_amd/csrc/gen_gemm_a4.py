@@ -477,7 +477,7 @@ S_HC = 93                    # s93..s96: the four pair multipliers of v2s_keep8
 NS_CLOBBER_P = 98
 V_HL = 239                   # (reludrop form; = V_ZO's register) lane part of the chunk index + seed term
 V_HB, V_HT = 240, 241        # hash temporaries
-V_SC2 = 248                  # v248..v249: the dropout scale twice (v_pk_mul_f32 operand)
+V_SC = 248                   # the dropout scale
 RING = 4 * STAGE
 
 
@@ -560,8 +560,7 @@ class GenP(Gen):
             e(f"s_mov_b32 s{S_HPP}, %[hpp]")
             for i in range(4):
                 e(f"s_mov_b32 s{S_HC + i}, 0x{0x00EBCA77 + 0x2468 * i:x}")
-            e(f"v_mov_b32 v{V_SC2}, %[scale]")
-            e(f"v_mov_b32 v{V_SC2 + 1}, %[scale]")
+            e(f"v_mov_b32 v{V_SC}, %[scale]")
         if self.epi == "dact":
             e(f"v_and_b32 v{T + 5}, 31, v{T}")
             e(f"v_lshrrev_b32 v{T + 6}, 5, v{T}")
@@ -655,7 +654,8 @@ class GenP(Gen):
             return
         if self.epi == "reludrop":                   # held[8 b + i] holds the keep masks of the pair (hash_stream): out = max(round(acc * scale), 0) & mask
             for i in range(8):
-                e(f"v_pk_mul_f32 v[{V_T + 2 * i}:{V_T + 2 * i + 1}], v[{V_T + 2 * i}:{V_T + 2 * i + 1}], v[{V_SC2}:{V_SC2 + 1}]")
+                e(f"v_mul_f32 v{V_T + 2 * i}, v{V_SC}, v{V_T + 2 * i}")
+                e(f"v_mul_f32 v{V_T + 2 * i + 1}, v{V_SC}, v{V_T + 2 * i + 1}")
             for i in range(8):
                 e(f"v_cvt_pk_bf16_f32 v{V_T + 2 * i}, v{V_T + 2 * i}, v{V_T + 2 * i + 1}")
             for i in range(8):

@@ -21,9 +21,8 @@
 //     moves K/V (or Q/dO) tiles: four buffer_load_dwordx4 per thread whose out-of-range rows the hardware bounds check zero-fills
 //     (no address compares, no branches) and four ds_write_b128;
 //   * the bias enters through the ACCUMULATOR: the score MFMAs start from bias / scale read straight from the LDS window, so the
-//     softmax needs no bias add; max(), the exponent argument (one packed fma per two elements: s * scale*log2e - m), the row sum,
-//     the rescale of the output accumulator (skipped when no row maximum of the wave moved), the bf16 packing and the backward
-//     products all run on two elements per instruction (v_pk_fma/mul/add_f32, v_max3_f32, v_cvt_pk_bf16_f32);
+//     softmax needs no bias add; max() takes three elements per instruction, the bf16 packing and the dropout masks two (v_max3_f32,
+//     v_cvt_pk_bf16_f32, v_pk_*_i16), the output accumulator is rescaled only where a row maximum of the wave moved;
 //   * attention-probability dropout draws TWO 16-bit numbers from one 32-bit hash (see drop_* below) and applies them without
 //     v_cmp / v_cndmask: in the forward as an AND mask on the packed bf16 pair (5 instructions per 2 elements instead of 8);
 //   * "clean" tiles (no masked or out-of-range key, no causal edge) take a branch-free path; tiles whose keys are all masked
@@ -167,29 +166,23 @@ __device__ __forceinline__ void tile_store(char* tile, int tid, const uint4 (&r)
   for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(tile + tile_off(rr + i * 32, chunk * 8)) = r[i];
 }
 
-// ---- two-elements-per-instruction fp32 helpers ------------------------------------------------------------
+// ---- helpers on pairs ---------------------------------------------------------------------------------------
 // two fp32 -> one packed bf16 pair with a single v_cvt_pk_bf16_f32 (element-wise casts compile to one conversion per element
 // plus a v_perm to merge them)
 __device__ __forceinline__ uint32_t cvt_pk(float lo, float hi) {
   const f32x2 v = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
-// (the compiler splits <2 x float> arithmetic that feeds scalar transcendental ops: force the packed forms)
-__device__ __forceinline__ f32x2 pk_add(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("v_pk_add_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-  return d;
+// sums, products and fused multiply-adds of pairs, one instruction per element.  Each rounds on its own: contraction is off, also where one feeds another
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+#pragma clang fp contract(off)
+  return f32x2{a[0] + b[0], a[1] + b[1]};
 }
-__device__ __forceinline__ f32x2 pk_mul(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("v_pk_mul_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-  return d;
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+#pragma clang fp contract(off)
+  return f32x2{a[0] * b[0], a[1] * b[1]};
 }
-__device__ __forceinline__ f32x2 pk_fma(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 d;
-  asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-  return d;
-}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { return f32x2{fmaf(a[0], b[0], c[0]), fmaf(a[1], b[1], c[1])}; }
 __device__ __forceinline__ float vmax(float a, float b) {       // v_max_f32 without the canonicalising v_max x, x, x hipcc puts in front of fmaxf
   float d;
   asm("v_max_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
@@ -201,28 +194,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32; x <= ~0 here
-// hipcc does not pad hardware hazards around inline asm (cdna_hip_programming.md 5.7):
-//   * a v_exp_f32 result needs one wait state before a non-transcendental VALU reads it -> the packed ops whose operands may come
-//     straight from fast_exp2 start with s_nop 0 (the *_t variants);
-//   * an MFMA result must not be read by an asm statement before the matrix pipe has written it back (up to 18 wait states after
-//     the issue of an 8-pass MFMA).  mfma_settle() sits between a group of MFMAs and the first asm reader of their accumulators: the
-//     "+v" operands order it after every MFMA of the group and before every reader, the nops inside cover the write-back.
-__device__ __forceinline__ f32x2 pk_add_t(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("s_nop 0\n\tv_pk_add_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-  return d;
-}
-__device__ __forceinline__ f32x2 pk_mul_t(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("s_nop 0\n\tv_pk_mul_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b));
-  return d;
-}
+// hipcc does not pad hardware hazards around inline asm: an MFMA result must not be read by an asm statement before the matrix pipe has written it back (up to
+// 18 wait states after the issue of an 8-pass MFMA).  mfma_settle() sits between a group of MFMAs and the first asm reader of their accumulators (the maxima of
+// the forward): the "+v" operands order it after every MFMA of the group and before every reader, the nops inside cover the write-back.
 __device__ __forceinline__ void mfma_settle(f32x4& a0, f32x4& a1, f32x4& a2, f32x4& a3, f32x4& a4, f32x4& a5, f32x4& a6, f32x4& a7) {
   asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3), "+v"(a4), "+v"(a5), "+v"(a6), "+v"(a7));
-}
-
-__device__ __forceinline__ void mfma_settle4(f32x4& a0, f32x4& a1, f32x4& a2, f32x4& a3) {
-  asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3));
 }
 
 // wave priority: the wave that is in an MFMA phase (latency-bound: LDS fragment reads -> MFMA) is preferred by the issue arbiter over a wave of
@@ -547,11 +523,11 @@ __global__ __launch_bounds__(256, CAUSAL ? 2 : 3) void attn_fwd_kernel(const Att
         uint32_t pw[4][2];
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-          const f32x2 x01 = pk_fma(f32x2{st[qb][kb][0], st[qb][kb][1]}, mult2, nmn2);
-          const f32x2 x23 = pk_fma(f32x2{st[qb][kb][2], st[qb][kb][3]}, mult2, nmn2);
+          const f32x2 x01 = fma2(f32x2{st[qb][kb][0], st[qb][kb][1]}, mult2, nmn2);
+          const f32x2 x23 = fma2(f32x2{st[qb][kb][2], st[qb][kb][3]}, mult2, nmn2);
           const f32x2 p01 = {fast_exp2(x01[0]), fast_exp2(x01[1])}, p23 = {fast_exp2(x23[0]), fast_exp2(x23[1])};
-          rs2 = pk_add_t(rs2, p01);
-          rs2 = pk_add_t(rs2, p23);
+          rs2 = add2(rs2, p01);
+          rs2 = add2(rs2, p23);
           pw[kb][0] = cvt_pk(p01[0], p01[1]);
           pw[kb][1] = cvt_pk(p23[0], p23[1]);
           if (DROP) {                                       // 1/(1-p) is applied once, to the output row
@@ -562,7 +538,7 @@ __global__ __launch_bounds__(256, CAUSAL ? 2 : 3) void attn_fwd_kernel(const Att
         lsum[qb] = lsum[qb] * alpha + (rs2[0] + rs2[1]);
         if (__any(alpha != 1.0f)) {                         // some row maximum of this wave moved: rescale the output accumulators
 #pragma unroll
-          for (int db = 0; db < 4; ++db) ot[qb][db] *= alpha;      // plain C (compiles to v_pk_mul_f32): these are MFMA accumulators
+          for (int db = 0; db < 4; ++db) ot[qb][db] *= alpha;      // plain C: these are MFMA accumulators
         }
         pf[qb][0] = __builtin_bit_cast(bf16x8, make_uint4(pw[0][0], pw[0][1], pw[1][0], pw[1][1]));
         pf[qb][1] = __builtin_bit_cast(bf16x8, make_uint4(pw[2][0], pw[2][1], pw[3][0], pw[3][1]));
@@ -814,8 +790,6 @@ __global__ __launch_bounds__(256, ATTN_BWD_OCC) void attn_bwd_dq_kernel(const At
             dp[qb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, dof[qb][ks], dp[qb][kb], 0, 0, 0);
           }
         }
-      mfma_settle(st[0][0], st[0][1], st[0][2], st[0][3], st[1][0], st[1][1], st[1][2], st[1][3]);
-      mfma_settle(dp[0][0], dp[0][1], dp[0][2], dp[0][3], dp[1][0], dp[1][1], dp[1][2], dp[1][3]);
       prio_lo();
 #if ATTN_DQ_PREF
       // the transposed K fragments of the first half of the dQ product, requested before the softmax / dS phase (LDS latency under its VALU work)
@@ -840,7 +814,7 @@ __global__ __launch_bounds__(256, ATTN_BWD_OCC) void attn_bwd_dq_kernel(const At
         if (clean) {
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb) {
-            const f32x2 x01 = pk_fma(f32x2{st[qb][kb][0], st[qb][kb][1]}, sc22, nm22), x23 = pk_fma(f32x2{st[qb][kb][2], st[qb][kb][3]}, sc22, nm22);
+            const f32x2 x01 = fma2(f32x2{st[qb][kb][0], st[qb][kb][1]}, sc22, nm22), x23 = fma2(f32x2{st[qb][kb][2], st[qb][kb][3]}, sc22, nm22);
             st[qb][kb] = f32x4{x01[0], x01[1], x23[0], x23[1]};
           }
         } else {
@@ -866,7 +840,7 @@ __global__ __launch_bounds__(256, ATTN_BWD_OCC) void attn_bwd_dq_kernel(const At
             drop_dropmask32(rseed ^ ((uint32_t)(kb * 8 + 1) * DROP_C1), p.tpk, mlo, mhi);
             d23 = f32x2{clear_if(mlo, d23[0]), clear_if(mhi, d23[1])};
           }
-          const f32x2 s01 = pk_mul_t(p01, pk_fma(d01, ik2, ndl2)), s23 = pk_mul_t(p23, pk_fma(d23, ik2, ndl2));   // dS = P * (dP/(1-p) - delta)
+          const f32x2 s01 = mul2(p01, fma2(d01, ik2, ndl2)), s23 = mul2(p23, fma2(d23, ik2, ndl2));   // dS = P * (dP/(1-p) - delta)
           st[qb][kb] = f32x4{s01[0], s01[1], s23[0], s23[1]};
         }
       }
@@ -877,11 +851,11 @@ __global__ __launch_bounds__(256, ATTN_BWD_OCC) void attn_bwd_dq_kernel(const At
         for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb) {
-            tsum = pk_add(tsum, f32x2{st[qb][kb][0], st[qb][kb][1]});
-            tsum = pk_add(tsum, f32x2{st[qb][kb][2], st[qb][kb][3]});
+            tsum = add2(tsum, f32x2{st[qb][kb][0], st[qb][kb][1]});
+            tsum = add2(tsum, f32x2{st[qb][kb][2], st[qb][kb][3]});
           }
-        if (troute == 1) acc_lo = pk_add(acc_lo, tsum);
-        else acc_hi = pk_add(acc_hi, tsum);
+        if (troute == 1) acc_lo = add2(acc_lo, tsum);
+        else acc_hi = add2(acc_hi, tsum);
       } else if (troute == 3) {
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
@@ -902,9 +876,9 @@ __global__ __launch_bounds__(256, ATTN_BWD_OCC) void attn_bwd_dq_kernel(const At
                 atomicAdd(&dbw[(k0 + kb * 16 + 4 * g + r) + 127 - qq], bits);
               }
             } else {
-              const f32x2 bs = pk_add(f32x2{st[qb][kb][0], st[qb][kb][1]}, f32x2{st[qb][kb][2], st[qb][kb][3]});
-              if (route == 1) acc_lo = pk_add(acc_lo, bs);
-              else acc_hi = pk_add(acc_hi, bs);
+              const f32x2 bs = add2(f32x2{st[qb][kb][0], st[qb][kb][1]}, f32x2{st[qb][kb][2], st[qb][kb][3]});
+              if (route == 1) acc_lo = add2(acc_lo, bs);
+              else acc_hi = add2(acc_hi, bs);
             }
           }
         }
@@ -1243,8 +1217,6 @@ __global__ __launch_bounds__(256, ATTN_DKV_OCC) void attn_bwd_dkv_kernel(const A
 #endif
       // P (dropped) -> dp registers become Pd ; st registers become dS ; packed to the B operands of the second products
       auto softmax_ds = [&](const int qh, f32x4 (&st)[2][KBW], f32x4 (&dp)[2][KBW], bf16x8 (&pdf)[KBW], bf16x8 (&dsf)[KBW]) {
-        if (KBW == 2) mfma_settle(st[0][0], st[0][KBW - 1], st[1][0], st[1][KBW - 1], dp[0][0], dp[0][KBW - 1], dp[1][0], dp[1][KBW - 1]);
-        else mfma_settle4(st[0][0], st[1][0], dp[0][0], dp[1][0]);
 #pragma unroll
         for (int qi = 0; qi < (ATTN_ABL == 3 ? 0 : 2); ++qi) {      // (ablation 3: no softmax / dS arithmetic, results invalid)
           const int qb = 2 * qh + qi;
@@ -1258,7 +1230,7 @@ __global__ __launch_bounds__(256, ATTN_DKV_OCC) void attn_bwd_dkv_kernel(const A
           if (clean) {
 #pragma unroll
             for (int kb = 0; kb < KBW; ++kb) {
-              const f32x2 x01 = pk_fma(f32x2{st[qi][kb][0], st[qi][kb][1]}, sc22, nm01), x23 = pk_fma(f32x2{st[qi][kb][2], st[qi][kb][3]}, sc22, nm23);
+              const f32x2 x01 = fma2(f32x2{st[qi][kb][0], st[qi][kb][1]}, sc22, nm01), x23 = fma2(f32x2{st[qi][kb][2], st[qi][kb][3]}, sc22, nm23);
               st[qi][kb] = f32x4{x01[0], x01[1], x23[0], x23[1]};
             }
           } else {
@@ -1297,8 +1269,8 @@ __global__ __launch_bounds__(256, ATTN_DKV_OCC) void attn_bwd_dkv_kernel(const A
               pd01 = f32x2{pdv[0], pdv[1]}; pd23 = f32x2{pdv[2], pdv[3]};
             }
             // dS = Pd * dP - P' * (delta / ik)
-            const f32x2 s01 = pk_fma(pd01, f32x2{dp[qi][kb][0], dp[qi][kb][1]}, pk_mul_t(p01, nd01));
-            const f32x2 s23 = pk_fma(pd23, f32x2{dp[qi][kb][2], dp[qi][kb][3]}, pk_mul_t(p23, nd23));
+            const f32x2 s01 = fma2(pd01, f32x2{dp[qi][kb][0], dp[qi][kb][1]}, mul2(p01, nd01));
+            const f32x2 s23 = fma2(pd23, f32x2{dp[qi][kb][2], dp[qi][kb][3]}, mul2(p23, nd23));
             st[qi][kb] = f32x4{s01[0], s01[1], s23[0], s23[1]};
             dp[qi][kb] = f32x4{pd01[0], pd01[1], pd23[0], pd23[1]};
           }
