@@ -510,9 +510,15 @@ template <class G> int tile_any(GemmQ8& p, bool plain, hipStream_t s) {
   if (!plain) return tile_launch<G, EPI_ANY>(p, s);
   return p.residual ? tile_launch<G, EPI_RESIDUAL>(p, s) : tile_launch<G, EPI_PLAIN>(p, s);
 }
-template <int WAVES, int MT> int skinny_launch(const GemmQ8& p, hipStream_t s) {
-  hipLaunchKernelGGL((gemm_q8_skinny_kernel<WAVES, MT>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, s, p);
-  V2S_LAUNCH_CHECK();
+template <int WAVES, int MT> int skinny_launch(GemmQ8 p, hipStream_t s) {
+  constexpr int MOST = 65535 * 16 * MT;     // rows of one launch: a grid's y
+  for (int left = p.M; left > 0; left -= MOST) {
+    p.M = left < MOST ? left : MOST;
+    hipLaunchKernelGGL((gemm_q8_skinny_kernel<WAVES, MT>), dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), dim3(WAVES * 64), 0, s, p);
+    V2S_LAUNCH_CHECK();
+    p.A += p.M * p.lda; p.sA += p.M; p.C = (char*)p.C + p.M * p.ldc * (p.c_f32 ? 4 : 2);
+    if (p.residual) p.residual += p.M * p.ldr;
+  }
   return V2S_OK;
 }
 
@@ -551,7 +557,6 @@ extern "C" int v2s_gemm_q8(const v2s_gemm_q8_args* a, void* stream) {
   if (kind == 2) return tile_any<Tile64>(p, plain, s);
   const bool deep = p.K > 1024;
   const int64_t mb = (p.M + 15) / 16, nb = (p.N + 15) / 16;
-  V2S_CHECK((mb + 3) / 4 <= 65535, V2S_ERR_SHAPE, "v2s_gemm_q8: too many rows for the few-row kernels");
   // rows of one block: 16 as long as that leaves the chip under two blocks per CU (64 x 1024 x 4096: 6.2 us, 64 rows 11.7), as many as there are otherwise
   // (64 x 4096 x 4096: 17 and 12 us)
   if (mb == 1 || mb * nb < 512) return deep ? skinny_launch<8, 1>(p, s) : skinny_launch<4, 1>(p, s);
