@@ -75,3 +75,13 @@ def test_vectors_of_the_other_calls():
                 call(**{name: t})
             with passes():
                 call(**{name: t.contiguous()})
+
+
+def test_sequences_without_a_row_length():
+    z, u, tok, pos = torch.zeros(4, 300), torch.zeros(5, 4), torch.zeros(4, dtype=torch.long), torch.zeros(1, dtype=torch.int32)
+    for bad in (torch.zeros(4 * 9, dtype=torch.long), torch.zeros(3, 9, dtype=torch.long), torch.zeros(4, 20, dtype=torch.long)[:, :9]):
+        with refused():
+            L.sample_step(z, 4, 300, u, tok, seq_out=bad, pos_dev=pos)
+    for fine, ld in ((torch.zeros(4, 9, dtype=torch.long), None), (torch.zeros(4 * 9, dtype=torch.long), 9), (torch.zeros(4, 20, dtype=torch.long)[:, :9], 20)):
+        with passes():
+            L.sample_step(z, 4, 300, u, tok, seq_out=fine, seq_ld=ld, pos_dev=pos)

@@ -85,3 +85,19 @@ def test_logits_of_views():
     for v in (wide(z, 50.0)[0], last[:, -1], last[:, -1:], torch.cat([z, torch.full((rows, 12), 60.0, device=DEV)], 1)):
         L.sample_step(v, rows, V, u, got)
         assert torch.equal(got, tok)
+
+
+def test_sequence_rows_have_their_own_length():
+    """The token of every step also goes into its column, with and without the row length; a step behind the last column writes none."""
+    rows, V, steps = 5, 400, 4
+    g = torch.Generator(device=DEV).manual_seed(3)
+    z, u = torch.randn(rows, V, generator=g, device=DEV), torch.rand(steps, rows, generator=g, device=DEV)
+    pos, tok = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(rows, dtype=torch.long, device=DEV)
+    for kw in ({}, dict(seq_ld=0), dict(seq_ld=steps)):
+        seq, want = torch.full((rows + 1, steps), -1, dtype=torch.long, device=DEV), torch.full((rows + 1, steps), -1, dtype=torch.long, device=DEV)
+        for t in range(steps):
+            pos.fill_(t)
+            L.sample_step(z, rows, V, u, tok, seq_out=seq, pos_dev=pos, **kw)
+            if t + 1 < steps:
+                want[:rows, t + 1] = tok
+        assert torch.equal(seq, want)

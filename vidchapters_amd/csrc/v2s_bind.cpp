@@ -280,14 +280,20 @@ PyObject* sample_step(PyObject* const* a) {
   const bool f32 = z.scalar_type() == at::kFloat, table = a[16] != Py_None;
   const int32_t rows = small(a[1], "rows"), V = small(a[2], "V");
   int64_t ld = given_stride(a[5]);
-  const int64_t seq_ld = given_stride(a[15]);
+  int64_t seq_ld = given_stride(a[15]);
+  if (a[14] != Py_None && seq_ld == 0) {              // the length of its rows: the step behind the last column is not written
+    const at::Tensor& t = c.tensor(a[14], "seq_out");
+    if (t.dim() != 2 || t.size(0) < rows || !t.is_contiguous() || t.size(1) > INT32_MAX)
+      raise(PyExc_ValueError, "sample_step seq_out: [" + std::to_string(rows) + ", columns] is expected, or seq_ld");
+    seq_ld = t.size(1);
+  }
   if (u.dim() != (table ? 2 : 1) || u.size(-1) < rows)
     raise(PyExc_ValueError, "sample_step: u is [rows], or [steps, rows] with pos_dev, for " + std::to_string(rows) + " rows");
   const int64_t steps = table ? u.size(0) : 0, u_ld = !table ? 0 : (steps > 1 ? u.stride(0) : u.size(1));
   if (steps > INT32_MAX) raise(PyExc_ValueError, "sample_step: too many steps");
   void *pz = c.matrix(z, f32 ? at::kFloat : at::kBFloat16, rows, V, ld, "logits"), *pu = c.at_least(u, at::kFloat, rows, "u");
   void *tok = c.vector(a[4], at::kLong, rows, "next_tok"), *lp = c.optional(a[10], at::kFloat, rows, "logp");
-  void *un = c.optional(a[11], at::kInt, rows, "unfinished"), *seq = c.optional(a[14], at::kLong, rows * seq_ld, "seq_out");
+  void *un = c.optional(a[11], at::kInt, rows, "unfinished"), *seq = a[14] == Py_None ? nullptr : c.operand(a[14], at::kLong, rows * seq_ld, "seq_out");
   void* ctr = c.optional(a[16], at::kInt, 1, "pos_dev");
   return launch(f_sample, pz, f32 ? V2S_F32 : V2S_BF16, ld, rows, V, number(a[6]), small(a[7], "top_k"), number(a[8]), number(a[9]), (float*)pu, u_ld, (int32_t)steps,
                          (int64_t*)tok, (float*)lp, (int32_t*)un, small(a[12], "eos_id"), small(a[13], "pad_id"), (int64_t*)seq, seq_ld, (int32_t*)ctr,

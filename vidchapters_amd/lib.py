@@ -841,6 +841,7 @@ def decode_attn_q8(q, kq, ks, vq, vs, o, Nk, *, group=1, klen=None, pos_dev=None
 def sample_step(logits, rows, V, u, next_tok, *, ld=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logp=None, unfinished=None, eos_id=-1, pad_id=0,
                 seq_out=None, seq_ld=0, pos_dev=None, min_length=0):
     """One token per row of ``logits`` (fp32 or bf16 [rows, ld]) from temperature, top-k, top-p, min-p and the given numbers ``u`` (fp32 [rows] in
-    [0, 1), or [steps, rows] with ``pos_dev``): every draw is a function of its arguments.  ``logp``: log-probability of the token among the kept ones."""
+    [0, 1), or [steps, rows] with ``pos_dev``): every draw is a function of its arguments.  ``logp``: log-probability of the token among the kept ones.
+    ``seq_out`` (int64 [rows, columns]): the token also goes to column ``*pos_dev + 1``, where there is one (``seq_ld``: row length, if not the tensor's)."""
     _check(_bind().sample_step(logits, rows, V, u, next_tok, ld, temperature, top_k, top_p, min_p, logp, unfinished, eos_id, pad_id, seq_out, seq_ld, pos_dev,
                                min_length), "v2s_sample_step")
