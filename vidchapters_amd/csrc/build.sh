@@ -57,13 +57,17 @@ PYEOF
   if grep -q BAD build/v2s_gemm_a4.audit; then echo "ERROR: the compiler touched AGPRs / scratch inside gemm_a4_kernel" >&2; rm -f build/v2s_gemm.o; exit 1; fi
   grep -q CLEAN build/v2s_gemm_a4.audit || { echo "ERROR: gemm_a4 ISA audit did not run" >&2; exit 1; }
 fi
-# The decode memory-attention kernel keeps 192 accumulators in AGPRs and ~200 VGPRs: a spill puts scratch reloads (and their vmcnt(0)
-# waits) into every iteration of its loop -- measured 5 us per 16-key group instead of 0.7.  Say so loudly.
-if [ build/v2s_memattn.o -nt build/v2s_memattn.usage ] || [ ! -f build/v2s_memattn.usage ]; then
-  $HIPCC $FLAGS -c v2s_memattn.hip -o /dev/null -Rpass-analysis=kernel-resource-usage 2> build/v2s_memattn.usage.raw || true
-  grep -E "Function Name|ScratchSize" build/v2s_memattn.usage.raw | paste - - > build/v2s_memattn.usage || true
-  grep -vE "lane\]: 0 " build/v2s_memattn.usage | sed 's/.*Function Name: \([^ ]*\).*lane\]: \([0-9]*\).*/WARNING: \1 uses \2 bytes of scratch per lane/' >&2 || true
-fi
+# Registers spilled to scratch cost what these two are built on, so say so loudly.  The decode memory-attention kernel keeps 192 accumulators in AGPRs and ~200 VGPRs:
+# a spill puts scratch reloads (and their vmcnt(0) waits) into every iteration of its loop -- measured 5 us per 16-key group instead of 0.7.  The int8 product counts
+# its VMEM operations by hand (s_waitcnt vmcnt(N)): reloads among them stay correct, as more operations in flight only make a counted wait longer, but a reload waits
+# for all of them.  Its two 256 x 256 kernels are known to spill (64 and 48 bytes per lane).
+for s in v2s_memattn v2s_gemm_q8; do
+  if [ build/$s.o -nt build/$s.usage ] || [ ! -f build/$s.usage ]; then
+    $HIPCC $FLAGS -c $s.hip -o /dev/null -Rpass-analysis=kernel-resource-usage 2> build/$s.usage.raw || true
+    grep -E "Function Name|ScratchSize" build/$s.usage.raw | paste - - > build/$s.usage || true
+    grep -vE "lane\]: 0 " build/$s.usage | sed 's/.*Function Name: \([^ ]*\).*lane\]: \([0-9]*\).*/WARNING: \1 uses \2 bytes of scratch per lane/' >&2 || true
+  fi
+done
 OBJS=""; for s in $SRCS; do OBJS="$OBJS build/$s.o"; done
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o ../libvid2seq_hip.so $OBJS
 echo "built $(realpath ../libvid2seq_hip.so)"

@@ -149,9 +149,12 @@ __device__ __forceinline__ void finish4(const GemmQ8& p, float (&v)[4], const Co
 // Fragment j of B takes the rows (r >> 2) * 4 NI + 4 j + (r & 3) of the wave's 16 NI, so that a lane ends up with 4 NI consecutive columns of a row; the
 // write-out passes them through LDS rows of the wave's own, without a barrier, so that its stores are whole cache lines.
 // Blocks are persistent: the first two stages of the next tile are requested before the write-out of the current one and arrive under it; the counted
-// waits let its stores drain under those two stages.
-// 8192^3: 403 us = 2726 TOPS, 16384 x 1024 x 4096 with residual 57 to 60 us = 2400 TOPS: MFMA rate at the clock that its power allows.  27501 x 2304 x 768: 62 to
-// 64 us = 1500 TOPS: six stages a tile, then a write-out that no products cover (a block fills its CU: the accumulators take half of its registers).
+// waits let its stores drain under those two stages.  In the 256 x 256 kernels that holds in part only: the compiler spills 15 (plain) and 11 (residual) registers,
+// and a reload waits for all that the wave has in flight, which here is requests of the next tile, and stores of the last one (the counted waits stay right: more
+// operations in flight only make them longer).
+// 8192^3: 402 us = 2739 TOPS, 16384 x 1024 x 4096 with residual 57 to 60 us = 2400 TOPS when the same operands come again, 68 when they change: MFMA rate at the clock
+// that its power allows.  27501 x 2304 x 768: 62 to 67 us = 1450 to 1570 TOPS: six stages a tile, then a write-out that no products cover (a block fills its CU: the
+// accumulators take half of its registers).
 // K need not be a multiple of 128: in the last stage lanes whose group lies behind K load the row's first group again (in bounds), and A's fragments
 // are zeroed there.
 __device__ __forceinline__ uint32_t lds_off(const void* p) { return (uint32_t)(uintptr_t)(V2S_LDS const char*)p; }
@@ -185,8 +188,8 @@ struct Tile {
   static __device__ __forceinline__ int swzB(int row) { return ((row >> 1) & 1) | ((row / (NI * 4) & 3) << 1); }
 };
 
-// what a kernel's write-out can do: bf16 with none / ReLU, the same with a residual, everything (the registers of the 256 x 256 tile hold one of the first
-// two without spilling)
+// what a kernel's write-out can do: bf16 with none / ReLU, the same with a residual, everything.  The 256 x 256 tile comes in the first two forms, whose spills are few;
+// GELU and fp32 take 128 x 128 tiles
 enum { EPI_PLAIN, EPI_RESIDUAL, EPI_ANY };
 
 template <class G, int EPI>
