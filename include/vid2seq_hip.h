@@ -486,8 +486,9 @@ int v2s_beam_sample_cand(const float* logits, int64_t ld, int32_t rows, int32_t 
  *   w_i = exp((z_i - max z) / temperature), an entry equal to the maximum has w = 1 (so a row of -infinity is uniform; +infinity wins over all);
  *   top-k keeps the first top_k tokens (0 = all); top-p keeps of those the tokens whose preceding mass is < top_p * their whole mass; min-p keeps
  *   of those the tokens with w_i >= min_p.  The drawn token is the first one, in index order, at which the running kept mass exceeds u * kept mass.
- * The weights are 64-bit fixed-point numbers (2^46 = weight one; below 2^-47 a token has none), so masses do not depend on the order of their sums
- * and every decision is the one exact arithmetic makes, up to 2^-46 of the largest weight.  A row that holds a NaN yields the index of its first
+ * The weights are 64-bit fixed-point numbers (2^46 = weight one; below 2^-47 a token has none), so masses do not depend on the order of their sums.
+ * A weight is off by at most 2^-46 of the largest one, a mass of n tokens by n times that, and masses are compared as doubles (rounded to 2^-53 of
+ * themselves): a decision is the one exact arithmetic makes unless a mass lies that close to its border.  A row that holds a NaN yields the index of its first
  * NaN (as v2s_argmax_step does) and a NaN log-probability.
  *   u: fp32 in [0, 1) (below 0 and NaN count as 0, from 1 on the last kept token is drawn): u[row], or with pos_dev row *pos_dev of a table [u_steps][u_ld]
  *   (a step behind the table reads its last row), so that one table serves a captured loop.

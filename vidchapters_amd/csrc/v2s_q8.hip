@@ -96,8 +96,10 @@ __device__ __forceinline__ void ld8(const float* p, float* f) {
 }
 
 // LPR lanes per row (a wave; fewer for a row shorter than half of one, a block for one longer than two), NCH chunks of 8 LPR columns held in registers: every byte is read once and written
-// once.  32000 x 768 with the residual: 28 us, 5.3 TB/s; 64 x 768: 3.5 us, a launch and one chain of loads and reductions.  A wave per row took 10.3 instead of
-// 4.3 us for 24017 x 48, 7.3 instead of 3.6 for 64 x 4096 and 46 instead of 36 for 4000 x 8192.
+// once.  32000 x 768 with the residual: 34 us, 5.05 TB/s (7 bytes per value); without norm from bf16 15.9 us, 4.6 TB/s, from fp32 22.7 us, 5.4 TB/s; 64 x 768: 3.1 to 3.8 us, a
+// launch and one chain of loads and reductions.  A wave per row, in us for norm with residual / norm / codes of bf16 / of fp32: 24017 x 48 9.5 / 7.7 / 6.0 / 5.7 instead of 4.3 /
+// 3.7 / 3.2 / 3.5, 64 x 4096 7.1 / 5.2 / 4.3 / 3.6 instead of 3.8 / 3.7 / 3.5 / 3.7, 4000 x 8192 97 / 53 / 30 / 33 instead of 47.5 / 25 / 22 / 31; at 4000 x 2048 both are
+// equal (11.0 and 11.4, 7.3 and 7.8, 6.3 and 6.2, 7.6 and 8.0).
 template <typename T, int NCH, int LPR, bool NORM>
 __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
   __shared__ float s_sum[4];
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(256) void rows_q8_kernel(const RowsQ8 p) {
   }
 }
 
-// y[row][c] = scale[row] * q[row][c], 8 columns per lane: bytes in, bytes out (32000 x 768: 12.4 us, 6 TB/s out of a cache that still holds the codes)
+// y[row][c] = scale[row] * q[row][c], 8 columns per lane: bytes in, bytes out (32000 x 768: 14.3 us, 5.1 TB/s; 12.4 us where a cache still holds the codes)
 __global__ __launch_bounds__(256) void dequant_q8_kernel(const i8* __restrict__ q, long ldq, const float* __restrict__ scale, bf16_t* __restrict__ y,
                                                          long ldy, int rows, int nch) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -202,7 +204,8 @@ struct KvQ8 {
   int pos0;
 };
 
-// Bound by HBM: 32 entries x 12 heads x up to 1100 tokens 23.5 us in and 21.6 us back, 5.3 and 5.7 TB/s; a single token by its chain of loads (2.9 us).
+// Bound by HBM: 32 entries x 12 heads x up to 1100 tokens 32 us in and 24 us back, 3.9 and 5.2 TB/s, when operands and cache change from call to call (23.5 and 21.6 us, 5.3 and
+// 5.7 TB/s, when the same come again); a single token by its chain of loads (2.9 us).
 // eight lanes per (entry, head, token); TOKENS: eight tokens of one head per wave (512 contiguous bytes of codes), else eight heads of one token
 template <bool TOKENS>
 __device__ __forceinline__ bool kv_unit(const KvQ8& p, int& e, int& h, int& t) {
@@ -341,7 +344,7 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
 
 // Block = 4 waves = up to PIECE keys of one (entry, head) against up to 16 of its queries, on the matrix pipe; a wave takes 64 keys at a time.
 //   loads    16 whole keys (1 KiB in a row) per instruction.  Keys loaded straight into the fragments' lanes (16 rows of 16 bytes per instruction) asked the
-//            cache for every line four times: 348 MB in 94 us, through LDS in 66.
+//            cache for every line four times: 348 MB in 94 us, through LDS in 66 (both with the same cache again).
 //   scores   S^T[key][query] = K[key][d] . Q^T[d][query] by v_mfma_f32_16x16x32_bf16: codes are exact in bf16, so the products are exact and the sums
 //            fp32.  Tile t of a group of 32 keys holds the keys 8 (row >> 2) + 4 t + (row & 3), so that the eight scores a lane gets of its query are
 //            those of the consecutive keys 8 g .. 8 g + 7 (g = lane >> 4), which is the B operand of the second product without any movement.
@@ -349,7 +352,7 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
 //            (ds_read_b64_tr_b8) returns the codes of eight keys for one d.  The weights carry the values' scales and are split into three bf16 parts
 //            of eight bits each, which is all of fp32 (three products): every product is exact and the sums are fp32, as for a single query.
 // The running maximum of a query is shared by its four lanes; scales and bias of the piece wait in LDS, where a key without a part has bias -infinity
-// and scales of zero.  4 x 4 queries x 16 heads x 40000 keys: 66 us, 5.3 TB/s, the rate of a large copy.  A value-per-lane form without the matrix pipe was
+// and scales of zero.  4 x 4 queries x 16 heads x 40000 keys: 73 to 75 us = 4.7 TB/s with the join (weights in two bf16 parts, 16 bits: 70 to 73).  A value-per-lane form without the matrix pipe was
 // bound by VALU issue (127 us); eight waves per block or five blocks per CU were slower on large caches, requesting the next chunk ahead did not pay.
 constexpr int WG = 4;                 // waves per block
 // byte of the 16-byte chunk c of key k in a wave's tile: the rows of a fragment read and those of a transposing read fall into different banks
@@ -549,7 +552,7 @@ __global__ __launch_bounds__(WG * 64, 4) void attn_q8_kernel(const AttnQ8 p) {
 // One query per entry: block = 4 waves = up to PIECE keys of one (entry, head).  lane = (key slot lane >> 2, 16 dimensions lane & 3): a load of the wave is
 // 16 whole keys (1 KiB).  On the matrix pipe fifteen of the sixteen query columns would be empty while every lane still converts the codes and
 // computes a softmax, so the fp32 pipe needs a third fewer instructions here.
-// 32 x 16 heads x 5000 keys: 68 us with the join, 5.1 TB/s; twice the waves per block: 8 x 12 heads x 1200 keys 7.7 instead of 8.7 us, but 64 x 12 x 300
+// 32 x 16 heads x 5000 keys: 65 us with the join, 5.3 TB/s; twice the waves per block: 8 x 12 heads x 1200 keys 7.7 instead of 8.7 us, but 64 x 12 x 300
 // keys 11.1 instead of 9.6.
 constexpr int W1 = 4;
 __global__ __launch_bounds__(W1 * 64) void attn_q8_one_kernel(const AttnQ8 p) {

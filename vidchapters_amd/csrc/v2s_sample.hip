@@ -395,7 +395,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(const SampleP p) {
       __syncthreads();
       return s_thr;
     }
-    // too many tokens within one bin (a plateau of equal logits): bisection on the order key
+    // more than CAP tokens within one bin (equal logits, a row whose logits lie within a few bins, or over 100000 tokens of any ordinary row): bisection on the order
+    // key, 64 passes over the row at most.  64 rows, top-p 0.9: 32228 logits spread by 0.001 600 us (by 2.5: 24), 131072 unit-normal ones 1.34 ms (spread by 2.5: 0.12)
     u64 first = 0, last = ~0ull;            // sum(keys <= last) reaches the goal
     while (first < last) {
       const u64 mid = first + ((last - first) >> 1);
