@@ -152,8 +152,8 @@ __device__ __forceinline__ void finish4(const GemmQ8& p, float (&v)[4], const Co
 // waits let its stores drain under those two stages.  In the 256 x 256 kernels that holds in part only: the compiler spills 15 (plain) and 11 (residual) registers,
 // and a reload waits for all that the wave has in flight, which here is requests of the next tile, and stores of the last one (the counted waits stay right: more
 // operations in flight only make them longer).
-// 8192^3: 402 us = 2739 TOPS, 16384 x 1024 x 4096 with residual 57 to 60 us = 2400 TOPS when the same operands come again, 68 when they change: MFMA rate at the clock
-// that its power allows.  27501 x 2304 x 768: 62 to 67 us = 1450 to 1570 TOPS: six stages a tile, then a write-out that no products cover (a block fills its CU: the
+// 8192^3: 402 us = 2739 TOPS, 16384 x 1024 x 4096 with residual 57 to 60 us = 2400 TOPS when the same operands come again, 67 to 75 when they change: MFMA rate at the clock
+// that its power allows.  27501 x 2304 x 768: 62 to 69 us = 1400 to 1570 TOPS: six stages a tile, then a write-out that no products cover (a block fills its CU: the
 // accumulators take half of its registers).
 // K need not be a multiple of 128: in the last stage lanes whose group lies behind K load the row's first group again (in bounds), and A's fragments
 // are zeroed there.
